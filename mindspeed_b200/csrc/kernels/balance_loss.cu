@@ -1,0 +1,326 @@
+// Balance loss of a mixture-of-experts router with its per-expert counts, and its gradient.
+//
+//   p = softmax(x) or sigmoid(x) / (sum_e sigmoid(x_e) + 1e-20)      per token over the E experts
+//   P_be = sum of p over the tokens of sequence b,   f_be = entries of the routing map there
+//   loss = C sum_be P_be f_be                        (C = coeff E / (S^2 topk B), from the caller)
+//   dx_e = g C p_e (f_e - sum p f)                   softmax
+//   dx_e = g C s_e (1 - s_e) / n (f_e - sum p f)     sigmoid, n the normaliser
+// Token t belongs to sequence t mod B ([s, b] order); the loss over the whole batch is B = 1.
+//
+// Bound by the memory rate (logits and map read once, gradient written once) or, for short batches, by the launches: two forward, one
+// backward.  A row lives in the registers of 1 to 32 lanes (VEC experts a load, NJ loads), so a warp takes up to 32 rows at once; the
+// sums over tokens stay in registers until the block ends and are joined in a fixed order: the same bits on every run.
+#include "msb_common.cuh"
+#include <algorithm>
+using namespace msb;
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int WARPS = 8;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int VEC> __device__ __forceinline__ void load_row(const float* p, float* f) {
+  if (VEC == 4) { const float4 v = *reinterpret_cast<const float4*>(p); f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+  else f[0] = *p;
+}
+template <int VEC, typename T> __device__ __forceinline__ void load_row(const T* p, float* f) {
+  if (VEC == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_f(h[i]);
+  } else f[0] = to_f(*p);
+}
+template <int VEC> __device__ __forceinline__ void store_row(float* p, const float* f) {
+  if (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  else *p = f[0];
+}
+template <int VEC, typename T> __device__ __forceinline__ void store_row(T* p, const float* f) {
+  if (VEC == 4) {
+    T h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = from_f<T>(f[i]);
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+  } else *p = from_f<T>(f[0]);
+}
+
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float lanes_max(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Scores of one row, in place of its logits: p, and for the sigmoid also d p_e / d x_e without the shared term (slope).  Places past
+// the row hold -inf and come out as 0.
+template <int N, bool SIGMOID>
+__device__ __forceinline__ void scores(float* x, float* slope, int lanes) {
+  if (SIGMOID) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float t = ex2(-fabsf(x[i]) * LOG2E), r = 1.f / (1.f + t);
+      const float big = r, small = t * r;              // sigmoid of |x| and of -|x|: neither is found by subtraction
+      const bool pos = x[i] >= 0.f;
+      const float sg = x[i] != x[i] ? x[i] : pos ? big : small;
+      slope[i] = sg * (pos ? small : big);
+      x[i] = sg;
+      s += sg;
+    }
+    const float inv = 1.f / (lanes_sum(s, lanes) + 1e-20f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) { x[i] *= inv; slope[i] *= inv; }
+  } else {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, x[i]);
+    m = lanes_max(m, lanes);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { x[i] = ex2((x[i] - m) * LOG2E); s += x[i]; }
+    const float inv = 1.f / lanes_sum(s, lanes);
+#pragma unroll
+    for (int i = 0; i < N; ++i) { x[i] *= inv; slope[i] = x[i]; }
+  }
+}
+
+// grid (blocks, B): partial sums of p and counts of the block's tokens.  `lanes` lanes a row; expert of (lane l, load j, element v) is
+// (l + lanes j) VEC + v.
+template <typename T, int VEC, int NJ, bool SIGMOID>
+__global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S,
+                                                                 int B, int E, int lanes, float* __restrict__ psum, int* __restrict__ csum,
+                                                                 unsigned int* __restrict__ ticket) {
+  extern __shared__ float sh[];                 // [WARPS][E]
+  constexpr int N = NJ * VEC;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (lanes - 1), sub = lane / lanes, rows_per_warp = 32 / lanes;
+  const int seq = blockIdx.y;
+  if (blockIdx.x == 0 && seq == 0 && threadIdx.x == 0) *ticket = 0;
+  float P[N];
+  int c[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) { P[i] = 0.f; c[i] = 0; }
+  for (long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp; r0 < S; r0 += (long long)gridDim.x * WARPS * rows_per_warp) {
+    const bool in = r0 + sub < S;
+    const long long at = ((r0 + sub) * B + seq) * E;
+    float x[N], slope[N];
+    uint32_t m[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int e = (l + lanes * j) * VEC;
+      m[j] = 0;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[j * VEC + v] = -INFINITY;
+      if (in && e < E) {
+        load_row<VEC>(logits + at + e, x + j * VEC);
+        m[j] = VEC == 4 ? *reinterpret_cast<const uint32_t*>(map + at + e) : (uint32_t)map[at + e];
+      }
+    }
+    scores<N, SIGMOID>(x, slope, lanes);
+    if (in) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!((l + lanes * (i / VEC)) * VEC >= E)) P[i] += x[i];
+        c[i] += (m[i / VEC] >> (8 * (i % VEC))) & 0xffu ? 1 : 0;
+      }
+    }
+  }
+  for (int o = lanes; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      P[i] += __shfl_xor_sync(0xffffffffu, P[i], o);
+      c[i] += __shfl_xor_sync(0xffffffffu, c[i], o);
+    }
+  const long long out = ((long long)seq * gridDim.x + blockIdx.x) * E;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    if (sub == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = (l + lanes * (i / VEC)) * VEC + i % VEC;
+        if (e < E) sh[warp * E + e] = pass ? __int_as_float(c[i]) : P[i];
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += WARPS * 32) {
+      if (pass) {
+        int t = 0;
+        for (int w = 0; w < WARPS; ++w) t += __float_as_int(sh[w * E + e]);
+        csum[out + e] = t;
+      } else {
+        float t = 0.f;
+        for (int w = 0; w < WARPS; ++w) t += sh[w * E + e];
+        psum[out + e] = t;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// grid (ceil(E / 32), B), 32 experts x 32 slices of the blocks: loads f, the products' sum; the last block to end adds those in order and
+// the counts over the sequences.
+__global__ void __launch_bounds__(1024) balance_join_kernel(const float* __restrict__ psum, const int* __restrict__ csum, int blocks, int B, int E,
+                                                            float scale, float* __restrict__ load, float* __restrict__ lpart,
+                                                            unsigned int* ticket, float* __restrict__ loss, long long* __restrict__ counts) {
+  __shared__ float ps[32][33];
+  __shared__ int cs[32][33];
+  __shared__ bool last;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, seq = blockIdx.y, e = blockIdx.x * 32 + x;
+  float P = 0.f;
+  int c = 0;
+  if (e < E)
+    for (int b = y; b < blocks; b += 32) {
+      const long long at = ((long long)seq * blocks + b) * E + e;
+      P += psum[at];
+      c += csum[at];
+    }
+  ps[y][x] = P;
+  cs[y][x] = c;
+  __syncthreads();
+  if (y == 0) {
+    P = 0.f; c = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) { P += ps[i][x]; c += cs[i][x]; }
+    if (e < E) load[(long long)seq * E + e] = (float)c;
+    const float s = warp_sum(e < E ? P * (float)c : 0.f);
+    if (x == 0) lpart[seq * gridDim.x + blockIdx.x] = s;
+    __threadfence();
+    __syncwarp();
+    if (x == 0) last = atomicAdd(ticket, 1u) == gridDim.x * gridDim.y - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < E; i += 1024) {
+    long long t = 0;
+    for (int b = 0; b < B; ++b) t += (long long)__ldcg(load + (long long)b * E + i);
+    counts[i] = t;
+  }
+  if (y == 0) {
+    float s = 0.f;
+    for (int i = x; i < (int)(gridDim.x * gridDim.y); i += 32) s += __ldcg(lpart + i);
+    s = warp_sum(s);
+    if (x == 0) *loss = s * scale;
+  }
+}
+
+// grid (blocks, B)
+template <typename T, int VEC, int NJ, bool SIGMOID>
+__global__ void __launch_bounds__(WARPS * 32) balance_grad_kernel(const T* __restrict__ logits, const float* __restrict__ load, int S, int B,
+                                                                 int E, int lanes, float scale, const float* __restrict__ g,
+                                                                 T* __restrict__ grad) {
+  constexpr int N = NJ * VEC;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (lanes - 1), sub = lane / lanes, rows_per_warp = 32 / lanes;
+  const int seq = blockIdx.y;
+  const float gs = scale * *g;
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = (l + lanes * (i / VEC)) * VEC + i % VEC;
+    f[i] = e < E ? load[(long long)seq * E + e] : 0.f;
+  }
+  for (long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp; r0 < S; r0 += (long long)gridDim.x * WARPS * rows_per_warp) {
+    const bool in = r0 + sub < S;
+    const long long at = ((r0 + sub) * B + seq) * E;
+    float x[N], slope[N];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int e = (l + lanes * j) * VEC;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[j * VEC + v] = -INFINITY;
+      if (in && e < E) load_row<VEC>(logits + at + e, x + j * VEC);
+    }
+    scores<N, SIGMOID>(x, slope, lanes);
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) d = fmaf(x[i], f[i], d);
+    d = lanes_sum(d, lanes);
+#pragma unroll
+    for (int i = 0; i < N; ++i) slope[i] *= (f[i] - d) * gs;
+    if (in) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int e = (l + lanes * j) * VEC;
+        if (e < E) store_row<VEC>(grad + at + e, slope + j * VEC);
+      }
+    }
+  }
+}
+
+struct Shape { int vec, nj, lanes; };
+
+// VEC = 4 where every row of logits, gradient and map starts on a boundary of four elements (E a multiple of 4, bases aligned).
+Shape shape_of(int E, bool aligned) {
+  Shape s;
+  s.vec = aligned && E % 4 == 0 ? 4 : 1;
+  const int units = E / s.vec;
+  s.lanes = 32;
+  while (s.lanes > 1 && s.lanes / 2 >= units) s.lanes /= 2;
+  s.nj = (units + s.lanes - 1) / s.lanes;
+  return s;
+}
+
+#define BAL_NJ(T, SIG, CALL)                                                                         \
+  if (sh.vec == 4) {                                                                                 \
+    if (sh.nj <= 1) { CALL(T, 4, 1, SIG); } else if (sh.nj <= 2) { CALL(T, 4, 2, SIG); }             \
+    else if (sh.nj <= 4) { CALL(T, 4, 4, SIG); } else { CALL(T, 4, 8, SIG); }                        \
+  } else {                                                                                           \
+    if (sh.nj <= 1) { CALL(T, 1, 1, SIG); } else if (sh.nj <= 4) { CALL(T, 1, 4, SIG); }             \
+    else if (sh.nj <= 16) { CALL(T, 1, 16, SIG); } else { CALL(T, 1, 32, SIG); }                     \
+  }
+#define BAL_DISPATCH(CALL)                                                                           \
+  MSB_DISPATCH_FLOAT(dtype, T, if (sigmoid) { BAL_NJ(T, true, CALL) } else { BAL_NJ(T, false, CALL) })
+
+int bal_check(int S, int B, int E) {
+  MSB_REQUIRE(S > 0 && B > 0 && E > 0 && E <= 1024, "balance_loss: %d x %d tokens, %d experts (at most 1024)", S, B, E);
+  MSB_REQUIRE(B <= 65535 && (long long)S * B <= (1 << 24), "balance_loss: %d sequences of %d tokens (at most 2^24 tokens, counted in fp32)", B, S);
+  return 0;
+}
+
+}  // namespace
+
+// Blocks a sequence that both directions launch, and that the forward's scratch is sized by ([B, blocks, E] floats and ints).
+MSB_API int msb_balance_blocks(int S, int B, int E) {
+  const int units = E % 4 == 0 ? E / 4 : E;
+  int lanes = 32;
+  while (lanes > 1 && lanes / 2 >= units) lanes /= 2;
+  const long long rows_per_block = WARPS * (32 / lanes);
+  const long long want = (S + rows_per_block - 1) / rows_per_block;
+  const long long cap = std::max<long long>(1, (long long)msb::num_sms() * 4 / B);
+  return (int)std::min(want, cap);
+}
+
+MSB_API int msb_balance_forward(const void* logits, const unsigned char* map, int S, int B, int E, int sigmoid, float scale, int dtype,
+                                float* psum, int* csum, int blocks, float* load, float* lpart, unsigned int* ticket, float* loss,
+                                long long* counts, cudaStream_t s) {
+  if (int rc = bal_check(S, B, E)) return rc;
+  const Shape sh = shape_of(E, ((uintptr_t)logits & 15) == 0 && ((uintptr_t)map & 3) == 0);
+  const dim3 grid(blocks, B);
+#define BAL_CALL(T, V, NJ, SIG)                                                                                                        \
+  balance_sums_kernel<T, V, NJ, SIG><<<grid, WARPS * 32, WARPS * E * 4, s>>>((const T*)logits, map, S, B, E, sh.lanes, psum, csum, ticket)
+  BAL_DISPATCH(BAL_CALL)
+#undef BAL_CALL
+  MSB_CHECK_LAUNCH("balance_sums");
+  balance_join_kernel<<<dim3((E + 31) / 32, B), 1024, 0, s>>>(psum, csum, blocks, B, E, scale, load, lpart, ticket, loss, counts);
+  MSB_CHECK_LAUNCH("balance_join");
+  return 0;
+}
+
+MSB_API int msb_balance_backward(const void* logits, const float* load, int S, int B, int E, int sigmoid, float scale, const float* g, int dtype,
+                                 void* grad, cudaStream_t s) {
+  if (int rc = bal_check(S, B, E)) return rc;
+  const Shape sh = shape_of(E, (((uintptr_t)logits | (uintptr_t)grad) & 15) == 0);
+  const dim3 grid(msb_balance_blocks(S, B, E), B);
+#define BAL_CALL(T, V, NJ, SIG) \
+  balance_grad_kernel<T, V, NJ, SIG><<<grid, WARPS * 32, 0, s>>>((const T*)logits, load, S, B, E, sh.lanes, scale, g, (T*)grad)
+  BAL_DISPATCH(BAL_CALL)
+#undef BAL_CALL
+  MSB_CHECK_LAUNCH("balance_grad");
+  return 0;
+}

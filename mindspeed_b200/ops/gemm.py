@@ -18,11 +18,13 @@ _status = {}
 
 
 #: codes of the status word that are not expired waits
-_MEANING = {0x702: "a routing map with another number of entries than stated"}
+_MEANING = {0x702: "a routing map with another number of entries than stated",
+            0x703: "a label or teacher index outside the vocabulary"}
 
 
 def status_word(device) -> torch.Tensor:
-    """Per-device error word written by a kernel whose bounded wait expired (0 = healthy)."""
+    """Per-device error words (0 = healthy): [0] written by a kernel whose bounded wait expired (kernels that find it set stop waiting),
+    [1] by kernels that met input they leave out and go on."""
     t = _status.get(device)
     if t is None:
         t = torch.zeros(4, dtype=torch.int32, device=device)
@@ -35,7 +37,7 @@ def check_status(device=None):
     for dev, t in _status.items():
         if device is not None and dev != device:
             continue
-        v = int(t[0].item())
+        v = next((w for w in t[:2].tolist() if w != 0), 0)
         if v != 0:
             t.zero_()
             raise RuntimeError(f"sm_100a kernel reported {_MEANING.get(v, 'a bounded-wait time-out')}, code 0x{v:x} on {dev}")

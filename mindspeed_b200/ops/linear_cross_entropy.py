@@ -1,0 +1,332 @@
+"""Output projection and its loss in one operator, without the [tokens, vocab] matrix of logits
+(csrc/kernels/linear_ce_sm100.cu).
+
+  linear_cross_entropy(hidden, weight, labels)                                  per-token cross entropy of softmax(hidden weight^T)
+  linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices)     per-token tau^2 KL(teacher's top words || student)
+
+Both take ``hidden`` [..., H] and ``weight`` [V, H] in bf16 or fp16 (H a multiple of 8) and return the loss in fp32 with the leading shape
+of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token, the backward makes the logits again, a
+piece of the vocabulary at a time.  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
+teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
+
+A label or teacher index beyond the vocabulary gives its token loss NaN and no gradient, and makes ``ops.gemm.check_status`` raise.
+
+With ``group`` the weight holds this rank's slice of the vocabulary (rank r has words [r V, (r + 1) V)), ``hidden`` and the targets are the
+same on every rank, the loss is that of the whole vocabulary, and the gradient of ``hidden`` is this rank's part: the caller sums it
+over the group (``mappings.copy_to_tensor_model_parallel_region`` or the sequence-parallel gather in front of the operator does).
+
+``accumulate_main_grad`` adds the weight's gradient straight to the fp32 ``weight.main_grad``, as the parallel linears do under gradient
+accumulation fusion; autograd then gets none.
+
+On a CPU the same functions run as eager PyTorch.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+import torch.distributed as dist
+from torch.autograd.function import once_differentiable
+
+from . import gemm as G
+from . import loader
+from ._dtypes import code
+
+_P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+
+#: bytes of the 16-bit logit gradients that the backward holds at a time
+PIECE_BYTES = 512 << 20
+MAX_LIST = 1024
+
+
+class _Args(ctypes.Structure):
+    _fields_ = [("hidden", _P), ("weight", _P), ("idx", _P), ("teacher", _P), ("ldh", _LL), ("ldw", _LL), ("vocab_start", _LL), ("vocab", _LL),
+                ("ignore_index", _LL), ("T", _I), ("H", _I), ("V", _I), ("K", _I), ("dtype", _I), ("tau", _F), ("pos", _P), ("rowmap", _P),
+                ("count", _P), ("kind", _P), ("packed", _P), ("z", _P), ("q", _P), ("dot", _P), ("ent", _P), ("lse", _P), ("loss", _P),
+                ("part", _P), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
+                ("splits", _I), ("slab_rows", _I), ("dhidden", _P), ("dweight", _P), ("dweight_fp32_add", _I), ("scale", _P), ("status", _P)]
+
+
+class _on_device:
+    """Makes ``dev`` the current device for the launches inside; nothing where it is already."""
+
+    def __init__(self, dev):
+        self.dev = dev.index
+        self.prev = None
+
+    def __enter__(self):
+        cur = torch._C._cuda_getDevice()
+        if cur != self.dev:
+            self.prev = cur
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _status(dev):
+    if dev not in G._status and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call of a process on a device sets up its error words and cannot be captured; run the operator once before")
+    return G.status_word(dev)
+
+
+def _rows(t):
+    """``t`` [rows, H] as the kernels read it: unit inner stride, rows on 16-byte boundaries that do not overlap."""
+    ld = t.shape[1] if t.shape[0] == 1 else t.stride(0)
+    if t.stride(1) != 1 or ld % 8 or ld < t.shape[1] or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        ld = t.shape[1]
+    return t, ld
+
+
+def _piece_columns(T, V):
+    cols = max(256, PIECE_BYTES // (2 * T) // 256 * 256)
+    return min(cols, (V + 255) // 256 * 256)
+
+
+def _splits(T, H, V, piece):
+    """K splits of the hidden gradient.  Its tiles (256 rows x 256 of H) are few where there are few rows, and the 74 SM pairs would wait
+    for as many tiles; split along the vocabulary each pair takes a part of it, at the price of writing and adding ``s`` results.  Times
+    in us: a block of 64 words takes a tile 0.37, its read-out 2; the slabs move at 6 TB/s."""
+    if piece < V:
+        return 1
+    tiles, blocks = -(-T // 256) * -(-H // 256), -(-V // 64)
+    best, best_t = 1, None
+    for s in range(1, min(64, blocks) + 1):
+        t = -(-tiles * s // 74) * (-(-blocks // s) * 0.37 + 2.0) + s * T * H * 8 / 6e6
+        if best_t is None or t < best_t * 0.98:
+            best, best_t = s, t
+    return best
+
+
+class _LinearLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, idx, teacher, tau, ignore_index, group, main_grad):
+        L = loader.require_lib()
+        dev = hidden.device
+        lead = hidden.shape[:-1]
+        h, ldh = _rows(hidden.reshape(-1, hidden.shape[-1]))
+        w, ldw = _rows(weight)
+        (T, H), V = h.shape, w.shape[0]
+        K = 1 if teacher is None else idx.shape[-1]
+        world = 1 if group is None else dist.get_world_size(group)
+        rank = 0 if group is None else dist.get_rank(group)
+        with _on_device(dev):
+            f32 = dict(dtype=torch.float32, device=dev)
+            ints = torch.empty(2 * T + 1, dtype=torch.int32, device=dev)          # pos, rowmap, count
+            kept = torch.empty(2 * T * K + T, **f32)                              # z, q, lse: for the backward
+            packed = torch.empty(T, H, dtype=h.dtype, device=dev)
+            tiles = (V + 255) // 256
+            scratch = torch.empty(4 * T + 2 * tiles * T + (T if teacher is not None else 0), **f32)
+            loss = torch.empty(T, **f32)
+            ip, kp, sp = ints.data_ptr(), kept.data_ptr(), scratch.data_ptr()
+            a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
+                      ldh=ldh, ldw=ldw, vocab_start=rank * V, vocab=world * V, ignore_index=ignore_index, T=T, H=H, V=V, K=K,
+                      dtype=code(h.dtype), tau=tau, pos=ip, rowmap=ip + 4 * T, count=ip + 8 * T, packed=packed.data_ptr(), z=kp,
+                      q=kp + 4 * T * K, lse=kp + 8 * T * K, loss=loss.data_ptr(), part=sp, dot=sp + 8 * tiles * T,
+                      ent=sp + 8 * tiles * T + 4 * T, kind=sp + 8 * tiles * T + 16 * T, status=_status(dev).data_ptr())
+            st = ctypes.c_void_p(loader.stream_ptr())
+            if world > 1:
+                at = 2 * tiles * T
+                dot, ent, mx, sm = (scratch[at + i * T:at + (i + 1) * T] for i in range(4))
+                a.mx, a.sum = mx.data_ptr(), sm.data_ptr()
+            loader.check(L.msb_lce_forward(ctypes.byref(a), st), "linear_ce_forward")
+            if world > 1:
+                gmx = mx.clone()
+                dist.all_reduce(gmx, op=dist.ReduceOp.MAX, group=group)
+                loader.check(L.msb_lce_rescale(loader.p(sm), loader.p(mx), loader.p(gmx), _F(tau), _P(a.count), T, st), "linear_ce_rescale")
+                dist.all_reduce(sm, group=group)
+                dist.all_reduce(dot, group=group)
+                loader.check(L.msb_lce_loss(loader.p(gmx), loader.p(sm), loader.p(dot), loader.p(ent), _P(a.rowmap), _P(a.count), _F(tau), T,
+                                            _P(a.lse), loader.p(loss), st), "linear_ce_loss")
+        ctx.save_for_backward(h, w, idx, teacher, ints, kept, packed)
+        ctx.meta = (tau, rank, hidden.shape, weight if main_grad else None)
+        return loss.reshape(lead)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        L = loader.require_lib()
+        h, w, idx, teacher, ints, kept, packed = ctx.saved_tensors
+        tau, rank, shape, param = ctx.meta
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dev = h.device
+        h, ldh = _rows(h)
+        w, ldw = _rows(w)
+        (T, H), V = h.shape, w.shape[0]
+        K = 1 if teacher is None else idx.shape[-1]
+        with _on_device(dev):
+            g = g.float()
+            one = all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape))      # an expanded scalar, as a sum's backward gives
+            g = g if one else g.reshape(-1).contiguous()
+            piece = _piece_columns(T, V)
+            ldz = min(piece, (V + 7) // 8 * 8)
+            dz = torch.empty(T, ldz, dtype=h.dtype, device=dev)
+            ip, kp = ints.data_ptr(), kept.data_ptr()
+            a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
+                      ldh=ldh, ldw=ldw, vocab_start=rank * V, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=tau, pos=ip, rowmap=ip + 4 * T,
+                      count=ip + 8 * T, packed=packed.data_ptr(), z=kp, q=kp + 4 * T * K, lse=kp + 8 * T * K, g=g.data_ptr(),
+                      g_stride=0 if one else 1, dz=dz.data_ptr(), ldz=ldz, piece=piece, status=_status(dev).data_ptr())
+            dh = dw = scale = acc = None
+            if h.dtype == torch.float16:
+                scale = torch.empty(2, dtype=torch.float32, device=dev)
+                a.scale = scale.data_ptr()
+            if need_h:
+                dh = torch.empty(shape, dtype=h.dtype, device=dev)
+                a.splits, a.slab_rows = _splits(T, H, V, piece), (T + 31) // 32 * 32
+                acc = torch.empty(a.splits * a.slab_rows, H, dtype=torch.float32, device=dev)
+                a.acc, a.dhidden = acc.data_ptr(), dh.data_ptr()
+            if need_w:
+                if param is not None:
+                    a.dweight, a.dweight_fp32_add = param.main_grad.data_ptr(), 1
+                else:
+                    dw = torch.empty(V, H, dtype=h.dtype, device=dev)
+                    a.dweight = dw.data_ptr()
+            loader.check(L.msb_lce_backward(ctypes.byref(a), ctypes.c_void_p(loader.stream_ptr())), "linear_ce_backward")
+        if need_w and param is not None:
+            param.grad_added_to_main_grad = True
+            cb = getattr(param, "_main_grad_ready_cb", None)
+            if cb is not None:
+                cb(param)
+        return dh, dw, None, None, None, None, None, None
+
+
+class _SumOverGroup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, group):
+        x = x.clone()
+        dist.all_reduce(x, group=group)
+        return x
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, None
+
+
+def _linear_loss_ref(hidden, weight, idx, q, ent, tau, group):
+    """Eager form: ``idx``, ``q`` [T, K] with q = 0 in unused places, ``ent`` [T] = sum q log q; rows whose q are all 0 are left out."""
+    world = 1 if group is None else dist.get_world_size(group)
+    rank = 0 if group is None else dist.get_rank(group)
+    V = weight.shape[0]
+    keep = (q.sum(1) > 0).nonzero().squeeze(1)
+    x = hidden.reshape(-1, hidden.shape[-1]).index_select(0, keep)
+    idx, q, ent_k = idx.index_select(0, keep), q.index_select(0, keep), ent.index_select(0, keep)
+    z = (x.float() @ weight.float().t()) / tau
+    with torch.no_grad():
+        m = z.amax(1, keepdim=True)
+        if world > 1:
+            dist.all_reduce(m, op=dist.ReduceOp.MAX, group=group)
+    s = torch.exp(z - m).sum(1)
+    local = idx - rank * V
+    here = (local >= 0) & (local < V) & (q > 0)
+    picked = torch.where(here, z.gather(1, local.clamp(0, V - 1)), torch.zeros_like(q))
+    dot = (q * picked).sum(1)
+    if world > 1:
+        s, dot = _SumOverGroup.apply(s, group), _SumOverGroup.apply(dot, group)
+    loss = (ent_k + (m.squeeze(1) - dot) + torch.log(s)) * (tau * tau)
+    out = torch.zeros(ent.shape[0], dtype=torch.float32, device=hidden.device).index_put((keep,), loss)
+    return out.reshape(hidden.shape[:-1])
+
+
+def _check(name, hidden, weight, target, accumulate_main_grad):
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{name}: hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not fit")
+    if weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"{name}: empty weight {tuple(weight.shape)}")
+    if hidden.dtype != weight.dtype or not hidden.dtype.is_floating_point:
+        raise TypeError(f"{name}: hidden is {hidden.dtype}, weight {weight.dtype}")
+    if target.dtype.is_floating_point or target.dtype.is_complex or target.dtype == torch.bool:
+        raise TypeError(f"{name}: labels and indices are integers, not {target.dtype}")
+    if not (hidden.device == weight.device == target.device):
+        raise ValueError(f"{name}: hidden on {hidden.device}, weight on {weight.device}, targets on {target.device}")
+    if accumulate_main_grad:
+        mg = getattr(weight, "main_grad", None)
+        if mg is None or mg.dtype != torch.float32 or mg.shape != weight.shape or not mg.is_contiguous() or mg.device != weight.device:
+            raise ValueError(f"{name}: accumulate_main_grad needs a contiguous fp32 main_grad of the weight's shape")
+    if hidden.is_cuda:
+        if hidden.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"{name}: the sm_100a kernels take bf16 or fp16, not {hidden.dtype}")
+        if hidden.shape[-1] % 8:
+            raise ValueError(f"{name}: the hidden size {hidden.shape[-1]} is not a multiple of 8")
+        if accumulate_main_grad and weight.main_grad.data_ptr() % 16:
+            raise ValueError(f"{name}: main_grad is not on a 16-byte boundary")
+        if hidden.numel() // hidden.shape[-1] >= 2 ** 31 - 256 or weight.shape[0] >= 2 ** 31 - 256:
+            raise ValueError(f"{name}: more than 2^31 tokens or words")
+
+
+def _none(hidden, weight):
+    """Loss of no tokens: shape [..., 0], zero gradients."""
+    return hidden.float().sum(-1) + weight[:0].float().sum()
+
+
+def _main_grad_hook(weight):
+    """The eager form's weight for ``accumulate_main_grad``: its gradient goes to main_grad instead of autograd."""
+    w = weight.detach().requires_grad_(weight.requires_grad)
+    if weight.requires_grad:
+        def add(grad):
+            weight.main_grad.add_(grad)
+            weight.grad_added_to_main_grad = True
+            cb = getattr(weight, "_main_grad_ready_cb", None)
+            if cb is not None:
+                cb(weight)
+            return grad
+        w.register_hook(add)
+    return w
+
+
+def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, accumulate_main_grad=False):
+    """Cross entropy of ``softmax(hidden @ weight.T)`` against ``labels`` [...], per token, fp32."""
+    _check("linear_cross_entropy", hidden, weight, labels, accumulate_main_grad)
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
+    if labels.numel() == 0:
+        return _none(hidden, weight)
+    idx = labels.reshape(-1).long().contiguous()
+    if loader.use_kernels(hidden):
+        return _LinearLoss.apply(hidden, weight, idx, None, 1.0, int(ignore_index), group, bool(accumulate_main_grad))
+    world = 1 if group is None else dist.get_world_size(group)
+    kept = idx != ignore_index
+    if bool(((idx < 0) | (idx >= world * weight.shape[0]))[kept].any()):
+        raise IndexError("linear_cross_entropy: a label outside the vocabulary")
+    w = _main_grad_hook(weight) if accumulate_main_grad else weight
+    q = kept.float().unsqueeze(1)
+    return _linear_loss_ref(hidden, w, idx.unsqueeze(1), q, torch.zeros_like(q[:, 0]), 1.0, group)
+
+
+def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, temperature=1.0, group=None, accumulate_main_grad=False):
+    """``temperature^2 KL(q || p)`` per token, fp32: q is the softmax of ``teacher_logits`` [..., K] at the temperature over the listed words
+    ``teacher_indices`` [..., K] (negative: unused place; a word may be listed more than once), p the student's softmax over the whole
+    vocabulary.  The teacher gets no gradient."""
+    name = "linear_topk_distillation"
+    _check(name, hidden, weight, teacher_indices, accumulate_main_grad)
+    K = teacher_indices.shape[-1] if teacher_indices.dim() else 0
+    if teacher_logits.shape != teacher_indices.shape or teacher_indices.shape[:-1] != hidden.shape[:-1]:
+        raise ValueError(f"{name}: teacher logits {tuple(teacher_logits.shape)} and indices {tuple(teacher_indices.shape)} "
+                         f"for hidden {tuple(hidden.shape)}")
+    if not 1 <= K <= MAX_LIST:
+        raise ValueError(f"{name}: {K} listed words a token (1 to {MAX_LIST})")
+    if not teacher_logits.dtype.is_floating_point or teacher_logits.device != hidden.device:
+        raise ValueError(f"{name}: teacher logits are {teacher_logits.dtype} on {teacher_logits.device}")
+    tau = float(temperature)
+    if not 0.0 < tau < float("inf"):
+        raise ValueError(f"{name}: the temperature must be positive, got {temperature}")
+    if teacher_indices.numel() == 0:
+        return _none(hidden, weight)
+    idx = teacher_indices.reshape(-1, K).long().contiguous()
+    a = teacher_logits.detach().reshape(-1, K).float().contiguous()
+    if loader.use_kernels(hidden):
+        return _LinearLoss.apply(hidden, weight, idx, a, tau, 0, group, bool(accumulate_main_grad))
+    world = 1 if group is None else dist.get_world_size(group)
+    if bool((idx >= world * weight.shape[0]).any()):
+        raise IndexError(f"{name}: a teacher index outside the vocabulary")
+    used = (idx >= 0) & (a != float("-inf"))
+    logq = torch.where(used, a / tau, torch.full_like(a, float("-inf")))
+    logq = logq - torch.logsumexp(logq, 1, keepdim=True)
+    q = torch.where(used, torch.exp(logq), torch.zeros_like(a))
+    ent = torch.where(q > 0, q * logq, torch.zeros_like(a)).sum(1)
+    w = _main_grad_hook(weight) if accumulate_main_grad else weight
+    return _linear_loss_ref(hidden, w, idx, q, ent, tau, group)

@@ -1,0 +1,410 @@
+"""Output projection with cross entropy / distillation loss on the sm_100a kernels, against the formulas in 64 bits.
+
+Tolerances.  A logit is an fp32 sum of H products of 16-bit values, however the tensor cores order and cut it off by at most H 2^-23 of
+the sum of the products' magnitudes (``dz`` below, over the temperature).  The loss moves by at most twice that, and by 2^-20 of itself
+for the exponentials, sums of up to V of them and the logarithm.  A gradient entry d = g tau (p - sum q) is rounded to the 16-bit type
+(half a step u = eps / 2 of it), and p is off by p (exp(2 dz) - 1 + 2^-20); the products sum these with fp32 sums and round once more.
+fp16 entries are scaled so that the largest |g| tau lies in [2^14, 2^15): below the normal numbers they are off by 2^-25 of that scale.
+"""
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _inputs(T, V, H, dtype, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed + T * 131 + V * 7 + H)
+    w = (torch.randn(V, H, generator=gen, device="cuda") * 0.5 / H ** 0.5 * 3).to(dtype)
+    fav = torch.randint(0, V, (T,), generator=gen, device="cuda")
+    h = (torch.randn(T, H, generator=gen, device="cuda") + w[fav].float() * 3).to(dtype)
+    g = torch.randn(T, generator=gen, device="cuda") / T
+    return h, w, fav, g, gen
+
+
+def _reference(h, w, idx, q, ent, tau, g):
+    """Values and error bounds in 64 bits.  idx, q [T, K]; rows with q = 0 throughout are left out."""
+    keep = q.sum(1) > 0
+    hd, wd = torch.where(keep[:, None], h.double(), 0.0), w.double()
+    z = hd @ wd.t() / tau
+    lse = torch.logsumexp(z, 1)
+    dot = (q * z.gather(1, idx.clamp(min=0))).sum(1)
+    loss = torch.where(keep, tau * tau * (ent + lse - dot), 0.0)
+    p = torch.exp(z - lse[:, None])
+    s = torch.zeros_like(p).scatter_add_(1, idx.clamp(min=0), q)
+    gt = torch.where(keep, g.double(), 0.0) * tau
+    d = gt[:, None] * (p - s)
+    H, V, T = h.shape[1], w.shape[0], h.shape[0]
+    dz = (H * 2.0 ** -23 * (hd.abs() @ wd.abs().t()) / tau).amax(1)
+    u = torch.finfo(h.dtype).eps / 2
+    err_loss = tau * tau * (2 * dz + 2.0 ** -20 * (1 + ent.abs() + lse.abs() + dot.abs()))
+    ed = u * d.abs() + gt.abs()[:, None] * p * (torch.expm1(2 * dz)[:, None] + 2.0 ** -20) * (1 + u)
+    sub = 0.0
+    if h.dtype == FP16:
+        ed = ed + gt.abs().max() * 2.0 ** -39
+        sub = 2.0 ** -25
+    gh, gw = d @ wd, d.t() @ hd
+    eh = ed @ wd.abs() * (1 + u) + V * 2.0 ** -23 * (d.abs() @ wd.abs()) + u * gh.abs() * 1.01 + sub
+    ew = ed.t() @ hd.abs() * (1 + u) + T * 2.0 ** -23 * (d.abs().t() @ hd.abs()) + u * gw.abs() * 1.01 + sub
+    return (loss, gh, gw), (err_loss, eh, ew)
+
+
+def _within(got, want, tol, what):
+    bad = (got.double() - want).abs() > tol
+    assert torch.isfinite(got).all(), what
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()}, worst {float(((got.double() - want).abs() / tol.clamp(min=1e-300)).max())} of the tolerance"
+
+
+def _ce_target(labels, ignore=-100):
+    idx = labels.long().unsqueeze(1)
+    q = (idx != ignore).double()
+    return torch.where(idx == ignore, 0, idx), q, torch.zeros_like(q[:, 0])
+
+
+def _kd_target(idx, a, tau):
+    used = (idx >= 0) & (a != float("-inf"))
+    logq = torch.where(used, a.double() / tau, float("-inf"))
+    logq = logq - torch.logsumexp(logq, 1, keepdim=True)
+    q = torch.where(used, torch.exp(logq), 0.0)
+    return idx.clamp(min=0), q, torch.where(q > 0, q * logq, 0.0).sum(1)
+
+
+def _ce(h, w, labels, g, **kw):
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(h, w, labels, **kw)
+    gh, gw = torch.autograd.grad(loss, (h, w), g.reshape(loss.shape))
+    return loss.detach(), gh, gw
+
+
+def _kd(h, w, a, idx, tau, g, **kw):
+    from mindspeed_b200.ops.linear_cross_entropy import linear_topk_distillation
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_topk_distillation(h, w, a, idx, temperature=tau, **kw)
+    gh, gw = torch.autograd.grad(loss, (h, w), g.reshape(loss.shape))
+    return loss.detach(), gh, gw
+
+
+def _compare(got, h, w, target, tau, g):
+    want, tol = _reference(h, w, *target, tau, g)
+    for x, y, t, what in zip(got, want, tol, ("loss", "d hidden", "d weight")):
+        _within(x.reshape(y.shape), y, t, what)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,V,H", [(1, 1, 8), (1, 257, 64), (2, 256, 72), (31, 255, 136), (64, 1000, 128), (65, 4099, 64), (257, 513, 512),
+                                   (300, 7, 264), (513, 2050, 200), (3, 20011, 256)])
+@pytest.mark.parametrize("ignored", ["none", "some", "most", "all"])
+def test_cross_entropy(T, V, H, dtype, ignored):
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    labels = torch.where(torch.rand(T, generator=gen, device="cuda") < 0.6, fav, torch.randint(0, V, (T,), generator=gen, device="cuda"))
+    part = {"none": 0.0, "some": 0.3, "most": 0.9, "all": 2.0}[ignored]
+    labels = torch.where(torch.rand(T, generator=gen, device="cuda") < part, -100, labels)
+    _compare(_ce(h, w, labels, g), h, w, _ce_target(labels), 1.0, g)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,V,H,K,tau", [(1, 5, 8, 1, 1.0), (3, 1000, 64, 8, 2.0), (130, 4099, 136, 33, 4.0), (257, 513, 256, 64, 0.5),
+                                         (40, 3000, 128, 200, 1.0), (9, 2500, 64, 1024, 2.0)])
+def test_distillation(T, V, H, K, tau, dtype):
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    idx = torch.randint(0, V, (T, K), generator=gen, device="cuda")          # words come up more than once
+    idx[:, 0] = fav
+    a = torch.randn(T, K, generator=gen, device="cuda") * 3
+    drop = torch.rand(T, K, generator=gen, device="cuda")
+    idx = torch.where(drop < 0.2, -1, idx)
+    a = torch.where(drop > 0.9, float("-inf"), a)
+    if T > 2:
+        idx[1] = -1                                                          # no word listed
+        a[2] = float("-inf")
+    _compare(_kd(h, w, a, idx, tau, g), h, w, _kd_target(idx, a, tau), tau, g)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_pieces_and_splits(dtype, monkeypatch):
+    """The backward in several pieces of the vocabulary, the last one ragged; and the whole in one piece with K splits."""
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    T, V, H = 300, 3000, 136
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    idx = torch.randint(0, V, (T, 5), generator=gen, device="cuda")
+    a = torch.randn(T, 5, generator=gen, device="cuda")
+    assert M._splits(T, H, V, M._piece_columns(T, V)) > 1
+    for size in (M.PIECE_BYTES, 2 * T * 256, 2 * T * 1100):
+        monkeypatch.setattr(M, "PIECE_BYTES", size)
+        _compare(_ce(h, w, fav, g), h, w, _ce_target(fav), 1.0, g)
+        _compare(_kd(h, w, a, idx, 2.0, g), h, w, _kd_target(idx, a, 2.0), 2.0, g)
+
+
+def test_layouts():
+    """Leading axes, rows of a wider buffer, an unaligned view, 32-bit labels, a scalar's expanded gradient, another ignore index."""
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    T, V, H = 60, 999, 72
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    wide = torch.full((T, 2 * H), float("nan"), dtype=BF16, device="cuda")
+    wide[:, :H] = h
+    wwide = torch.full((V, H + 8), float("nan"), dtype=BF16, device="cuda")
+    wwide[:, 8:] = w
+    base = _ce(h, w, fav, g)
+    _compare(base, h, w, _ce_target(fav), 1.0, g)
+    for hh, ww in ((wide[:, :H], w), (h, wwide[:, 8:]), (h.t().contiguous().t(), w.t().contiguous().t())):
+        for x, y in zip(_ce(hh, ww, fav, g), base):
+            assert torch.equal(x, y)
+    odd = torch.empty(T * H + 1, dtype=BF16, device="cuda")[1:].view(T, H).copy_(h)          # 2 bytes off a 16-byte boundary
+    for x, y in zip(_ce(odd, w, fav.int(), g), base):
+        assert torch.equal(x, y)
+    got = _ce(h.view(6, 10, H), w, fav.view(6, 10), g)
+    assert got[0].shape == (6, 10) and got[1].shape == (6, 10, H)
+    for x, y in zip(got, base):
+        assert torch.equal(x.reshape(y.shape), y)
+    lab = torch.where(fav % 3 == 0, 7, fav)
+    got = _ce(h, w, lab, g, ignore_index=7)
+    _compare(got, h, w, _ce_target(lab, 7), 1.0, g)
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_cross_entropy(hg, wg, fav).sum().backward()
+    one = torch.ones(T, device="cuda")
+    _compare((base[0], hg.grad, wg.grad), h, w, _ce_target(fav), 1.0, one)
+    hg.grad = None                                                                            # only one of the gradients
+    linear_cross_entropy(hg, w, fav).sum().backward()
+    first = hg.grad
+    assert torch.equal(first, _ce(h, w, fav, one)[1])
+    wg.grad = None
+    linear_cross_entropy(h, wg, fav).sum().backward()
+    assert torch.equal(wg.grad, _ce(h, w, fav, one)[2])
+    one_row = h[5]
+    got = _ce(one_row, w, fav[5], g[5])
+    assert got[0].shape == () and got[1].shape == (H,)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_left_out_rows_hold_anything(bad):
+    T, V, H = 100, 700, 64
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    labels = torch.where(torch.arange(T, device="cuda") % 4 == 1, -100, fav)
+    clean = _ce(h, w, labels, g)
+    dirty = h.clone()
+    dirty[labels == -100] = bad
+    g2 = g.clone()
+    g2[labels == -100] = bad
+    for x, y in zip(_ce(dirty, w, labels, g2), clean):
+        assert torch.equal(x, y)
+    assert (clean[0][labels == -100] == 0).all() and (clean[1][labels == -100] == 0).all()
+
+
+def test_zero_gradient_rows_and_infinite_logits():
+    """A token whose loss gets gradient 0 adds nothing to the hidden gradient; a row of infinite logits gives NaN, as the formula does."""
+    T, V, H = 20, 300, 64
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    g[3] = 0
+    got = _ce(h, w, fav, g)
+    assert (got[1][3] == 0).all()
+    h2 = h.clone()
+    h2[7] = float("inf")
+    assert torch.isnan(_ce(h2, w, fav, g)[0][7])
+    big = h.clone()
+    big[5] = 3e4                                                # logits of some thousands: sums of exponentials stay in range
+    _compare(_ce(big, w, fav, g), big, w, _ce_target(fav), 1.0, g)
+
+
+def test_words_outside_the_vocabulary():
+    from mindspeed_b200.ops.gemm import check_status
+    T, V, H = 50, 300, 64
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    check_status()
+    for wrong in (V, -1, 2 ** 40):
+        labels = fav.clone()
+        labels[17] = wrong
+        got = _ce(h, w, labels, g)
+        with pytest.raises(RuntimeError, match="outside the vocabulary"):
+            check_status()
+        check_status()
+        assert torch.isnan(got[0][17])
+        left = labels.clone()
+        left[17] = -100
+        want = _ce(h, w, left, g)
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        assert torch.equal(got[0][18:], want[0][18:])
+    idx = torch.randint(0, V, (T, 4), generator=gen, device="cuda")
+    idx[9, 2] = V
+    got = _kd(h, w, torch.randn(T, 4, generator=gen, device="cuda"), idx, 1.0, g)
+    assert torch.isnan(got[0][9]) and (got[1][9] == 0).all() and torch.isfinite(got[2]).all()
+    with pytest.raises(RuntimeError, match="outside the vocabulary"):
+        check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_main_grad(dtype):
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    T, V, H = 200, 1500, 136
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    p = torch.nn.Parameter(w.clone())
+    start = torch.randn(V, H, generator=gen, device="cuda")
+    p.main_grad = start.clone()
+    called = []
+    p._main_grad_ready_cb = called.append
+    hg = h.clone().requires_grad_(True)
+    linear_cross_entropy(hg, p, fav, accumulate_main_grad=True).backward(g)
+    assert p.grad is None and p.grad_added_to_main_grad and called == [p]
+    (_, gh, gw), (_, eh, ew) = _reference(h, w, *_ce_target(fav), 1.0, g)
+    _within(hg.grad, gh, eh, "d hidden")
+    _within(p.main_grad, gw + start.double(), ew + (gw + start.double()).abs() * 2.0 ** -23, "main_grad")
+    empty = p.main_grad.clone()
+    linear_cross_entropy(hg, p, torch.full_like(fav, -100), accumulate_main_grad=True).backward(g)
+    assert torch.equal(p.main_grad, empty)
+
+
+def test_same_bits_every_time_and_on_a_side_stream():
+    T, V, H = 700, 5000, 256
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    first = _ce(h, w, fav, g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = _ce(h, w, fav, g)
+    third = _ce(h, w, fav, g)                       # at the same time as the one on the side stream
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y, z in zip(first, second, third):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_captured_step_follows_its_inputs():
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    T, V, H = 130, 1000, 64
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    _ce(h, w, fav, g)                               # the process's first call sets up its error words
+    hs, ws, ls = h.clone().requires_grad_(True), w.clone().requires_grad_(True), fav.clone()
+    graphs = []
+    for _ in range(2):                              # two graphs of the same call do not share their workspaces
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(graph, stream=side):
+                loss = linear_cross_entropy(hs, ws, ls)
+                gh, gw = torch.autograd.grad(loss, (hs, ws), g)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append((graph, loss, gh, gw))
+    for seed in (1, 2):
+        h2, w2, fav2, _, gen2 = _inputs(T, V, H, BF16, seed)
+        keep = torch.rand(T, generator=gen2, device="cuda") < 0.5 * seed
+        fav2 = torch.where(keep, fav2, -100)        # another number of rows than when captured
+        with torch.no_grad():
+            hs.copy_(h2)
+            ws.copy_(w2)
+            ls.copy_(fav2)
+        want = _ce(h2, w2, fav2, g)
+        for graph, *outs in graphs:
+            graph.replay()
+        for _, *outs in graphs:
+            for x, y in zip(outs, want):
+                assert torch.equal(x.detach(), y)
+
+
+class _ThreadGroup:
+    """Two ranks as host threads of one process: the reductions meet at a host barrier, no kernel waits for another."""
+
+    class ReduceOp:
+        MAX, SUM = "max", "sum"
+
+    def __init__(self, world):
+        self.world, self.barrier, self.slots, self.local = world, threading.Barrier(world, timeout=60), [None] * world, threading.local()
+
+    def get_world_size(self, group):
+        return self.world
+
+    def get_rank(self, group):
+        return self.local.rank
+
+    def all_reduce(self, t, op="sum", group=None):
+        torch.cuda.synchronize()
+        self.slots[self.local.rank] = t.clone()
+        torch.cuda.synchronize()
+        self.barrier.wait()
+        both = torch.stack(self.slots)
+        t.copy_(both.amax(0) if op == "max" else both.sum(0))
+        torch.cuda.synchronize()
+        self.barrier.wait()
+
+
+@pytest.mark.parametrize("kind", ["ce", "kd"])
+def test_vocabulary_parallel(kind, monkeypatch):
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    T, V, H, tau = 90, 1400, 64, 2.0
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    idx = torch.randint(0, V, (T, 6), generator=gen, device="cuda")
+    idx[3] = -1
+    a = torch.randn(T, 6, generator=gen, device="cuda")
+    labels = torch.where(torch.arange(T, device="cuda") % 5 == 0, -100, fav)
+    group = _ThreadGroup(2)
+    monkeypatch.setattr(M, "dist", group)
+    out, errors = [None, None], []
+
+    def rank(r):
+        try:
+            group.local.rank = r
+            ws = w[r * V // 2:(r + 1) * V // 2]
+            out[r] = _ce(h, ws, labels, g, group="tp") if kind == "ce" else _kd(h, ws, a, idx, tau, g, group="tp")
+            torch.cuda.synchronize()
+        except BaseException as e:           # noqa: BLE001 - reported below, and the other rank is let go
+            errors.append(e)
+            group.barrier.abort()
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    assert torch.equal(out[0][0], out[1][0])
+    t = 1.0 if kind == "ce" else tau
+    want, tol = _reference(h, w, *(_ce_target(labels) if kind == "ce" else _kd_target(idx, a, tau)), t, g)
+    _within(out[0][0], want[0], tol[0], "loss")
+    _within(torch.cat((out[0][2], out[1][2])), want[2], tol[2], "d weight")
+    u = torch.finfo(BF16).eps / 2            # each rank rounds its part
+    parts = out[0][1].double().abs() + out[1][1].double().abs()
+    _within((out[0][1].double() + out[1][1].double()), want[1], tol[1] + u * parts * 1.01, "d hidden")
+
+
+def test_gradient_follows_differences():
+    """Central differences of the kernel's own loss along a direction of the inputs that bf16 holds exactly."""
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    T, V, H = 16, 200, 64
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    w = (torch.randint(-8, 9, (V, H), generator=gen, device="cuda") / 64).to(BF16)
+    h = (torch.randint(-16, 17, (T, H), generator=gen, device="cuda") / 16).to(BF16)
+    lab = torch.randint(0, V, (T,), generator=gen, device="cuda")
+    dirh = torch.randint(-1, 2, (T, H), generator=gen, device="cuda") / 16
+    dirw = torch.randint(-1, 2, (V, H), generator=gen, device="cuda") / 64
+    one = torch.ones(T, device="cuda")
+    _, gh, gw = _ce(h, w, lab, one)
+
+    def along(e, dh, dw):
+        hh, ww = (h.float() + e * dh).to(BF16), (w.float() + e * dw).to(BF16)
+        assert torch.equal(hh.float(), h.float() + e * dh) and torch.equal(ww.float(), w.float() + e * dw)
+        return linear_cross_entropy(hh, ww, lab).double().sum()
+
+    for dh, dw, slope in ((dirh, 0 * dirw, (gh.double() * dirh).sum()), (0 * dirh, dirw, (gw.double() * dirw).sum())):
+        diff = (along(1, dh, dw) - along(-1, dh, dw)) / 2
+        # third derivative of log-sum-exp along dz is at most 2 max|dz|^3: sum |dz| <= 64 / 16 / 8 and 64 / 64 x |h| = 1; u on each gradient entry
+        step = (dh.double().abs() @ w.double().abs().t() + h.double().abs() @ dw.double().abs().t()).amax(1)
+        tol = (step ** 3 / 3).sum() + 2.0 ** -8 * ((gh.double().abs() * dh.abs()).sum() + (gw.double().abs() * dw.abs()).sum()) * 3
+        assert abs(float(diff - slope)) <= float(tol)
+        assert float(tol) < 0.5 * max(1.0, abs(float(slope))) or float(step.max()) > 0.5
+
+
+def test_refusals_on_the_gpu():
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy, linear_topk_distillation
+    h, w = torch.zeros(4, 64, device="cuda"), torch.zeros(10, 64, device="cuda")
+    lab = torch.zeros(4, dtype=torch.long, device="cuda")
+    with pytest.raises(TypeError, match="bf16 or fp16"):
+        linear_cross_entropy(h, w, lab)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        linear_cross_entropy(h[:, :60].to(BF16), w[:, :60].to(BF16), lab)
+    with pytest.raises(ValueError, match="labels"):
+        linear_cross_entropy(h.to(BF16), w.to(BF16), lab[:3])
+    with pytest.raises(ValueError, match="on cpu"):
+        linear_cross_entropy(h.to(BF16), w.to(BF16), lab.cpu())
+    with pytest.raises(ValueError, match="temperature"):
+        linear_topk_distillation(h.to(BF16), w.to(BF16), torch.zeros(4, 2, device="cuda"), torch.zeros(4, 2, dtype=torch.long, device="cuda"), 0.0)
+    none = linear_cross_entropy(h[:0].to(BF16).requires_grad_(True), w.to(BF16).requires_grad_(True), lab[:0])
+    assert none.shape == (0,)
+    none.sum().backward()
