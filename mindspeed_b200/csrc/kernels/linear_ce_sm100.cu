@@ -9,13 +9,16 @@
 // Rows without a listed word (ignored labels) leave the products: a scan numbers the rows that stay, and every product runs over their
 // count, which only the device knows.  When all rows stay, the products read the caller's hidden states directly, else a packed copy.
 //
-// Forward:  scan -> rows (packed copy, the K listed logits as dot products, q) -> GEMM whose epilogue keeps a (max, sum of exponentials)
-//           pair per row and 256 columns -> join of the pairs.
-// Backward: per piece of the vocabulary: the GEMM again, its epilogue now writing the 16-bit dz of the piece -> the listed words' entries
-//           -> d hidden += dz W -> dW rows of the piece = dz^T hidden.  dz is rounded to the 16-bit type of the operands (the tensor cores
-//           take nothing wider next to them): half a step on each term, as much as the rounding of the result itself.
-//           With fp16, dz is scaled by a power of two that puts the largest |g| at 2^14 or above, so that probabilities down to 2^-28 keep
-//           all their bits; the products' epilogues take the power out again in fp32.
+// Forward:  scan (part of the rows kernel for short inputs) -> rows (packed copy, the K listed logits as dot products, q) -> GEMM whose
+//           epilogue keeps (max, where, sum of exponentials) per row and 128 columns -> join, which computes the largest logit again as a
+//           dot product: the tensor cores cut sums off, 4e-6 of a logit over 5120 products, and the largest one is what the loss follows.
+// Backward: per piece of the vocabulary: the GEMM again, its epilogue now writing the 16-bit dz of the piece (with the label's -1; a
+//           list's q are subtracted by a kernel of its own) -> d hidden += dz W -> dW rows of the piece = dz^T hidden.  dz is rounded to
+//           the 16-bit type of the operands (the tensor cores take nothing wider next to them): half a step on each term, as much as the
+//           rounding of the result itself.  With fp16, dz is scaled by a power of two that puts the largest |g| at 2^14 or above, so that
+//           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
+// Few rows: where the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them (transposed, [V, rows]: rows are
+//           the lanes of the epilogue), and an elementwise pass makes dz of them: one reading of W less, a quarter of all traffic.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
 #include "msb_common.cuh"
@@ -31,7 +34,11 @@ constexpr int BM = 128;          // rows per CTA; the pair covers 256
 constexpr int BN = 256;
 constexpr int BK = 64;           // 64 16-bit values = one 128-byte swizzle row
 constexpr int UMMA_K = 16;
+constexpr int GROUP_M = 16;      // tile rows that share W panels in L2: forward of 8192 x 128256 x 4096 in 6.7 ms, 7.5 with 8, 6.7 with 32 (backward 20.3 / 20.4 / 21.7)
 constexpr float LOG2E = 1.4426950408889634f;
+
+constexpr int EPI_WARPS = 8;       // two a quarter of the 128 accumulator lanes, each half of the columns
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 
 enum Epi : int { EPI_STATS = 0, EPI_DLOGITS = 1, EPI_OUT16 = 2, EPI_OUT32 = 3 };
 
@@ -39,32 +46,40 @@ struct LceGemm {
   CUtensorMap tmA, tmB, tmD;
   CUtensorMap tmPacked;        // the packed copy of the hidden states, read in place of A (forward) / B (weight gradient) when rows left
   int M, N, K;                 // upper bounds; the dimension that counts rows is cut to *rows
-  const int* rows;             // rows that stay
+  const int* rows;             // [0] rows that stay, [1] K splits of the hidden gradient
   int all_rows;                // rows there are: the packed copy is unused when *rows equals it
   int group_m;
-  int splits, slab_rows;       // K splits; rows between the slabs of their fp32 results
+  int rows_on_k;               // the rows are summed over (weight gradient), else they are output rows
+  int split;                   // take rows[1] K splits, their fp32 results in slabs of slab_rows rows
+  int slab_rows;
   int accumulate;              // OUT32: add to what is there
   int half;                    // operands are fp16 (else bf16)
-  float2* part;                // STATS: [column tile][part_ld] (max, sum)
+  float2* part;                // STATS: [128 columns][part_ld] (max, sum)
+  unsigned char* part_at;      // STATS: column of the max
   long long part_ld;
+  float* zt;                   // STATS: keep the logits, [N][ldt], or null
+  int ldt;
   const float* lse;            // DLOGITS: per packed row, in units of z / tau
   const int* rowmap;           // DLOGITS: packed row -> token
   const float* g;              // DLOGITS: gradient of the token's loss
   int g_stride;
   float g_factor;              // DLOGITS: tau
   float inv_tau;
+  const long long* label;      // DLOGITS: the token's word (cross entropy), or null
+  const float* z;              // DLOGITS: its logit, per packed row
+  long long piece_start;       // DLOGITS: word of column 0
   const float* scale;          // fp16: scale[0] multiplies dz, scale[1] takes it out of the products
   unsigned int* status;
 };
 
 template <int EPI>
 struct Cfg {
-  static constexpr int NSTAGE = EPI == EPI_STATS ? 7 : EPI == EPI_OUT32 ? 5 : 6;
+  static constexpr int NSTAGE = EPI == EPI_STATS ? 7 : EPI == EPI_OUT32 ? 5 : 6;   // what the staging leaves of 227 KB
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + (BN / 2) * BK * 2;
   static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_OUT32 ? 8192 : 4096;   // 32 rows x 64 columns of the output type
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
-  static constexpr int BAR_OFFSET = EPI_OFFSET + 4 * 2 * EPI_BUF;
+  static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
   static_assert(TOTAL <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
 };
@@ -108,10 +123,10 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, int half) {
   return pack_bf16(lo, hi);
 }
 
-// EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K], rows on M.     EPI_OUT32, A_MN = false: A = dz [M, K], B = W [K, N], rows on M.
-// A_MN = true: A = dz [K, M], B = hidden [K, N], rows on K.
+// EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K].      Hidden gradient: A = dz [M, K], B = W [K, N].
+// Weight gradient: A = dz [K, M], B = hidden [K, N], rows on K.  A_MN tells how dz lies in memory ([tokens, words] or transposed).
 template <int EPI, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   using L = Cfg<EPI>;
   constexpr int NSTAGE = L::NSTAGE;
   extern __shared__ uint8_t smem_raw[];
@@ -127,14 +142,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();                 // 0 = leader
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int rows = *p.rows;
-  const int M = A_MN ? p.M : rows, K = A_MN ? rows : p.K;
+  const int rows = p.rows[0], splits = p.split ? p.rows[1] : 1;
+  const int M = p.rows_on_k ? p.M : rows, K = p.rows_on_k ? rows : p.K;
   const bool packed = rows != p.all_rows;
   constexpr uint32_t TMEM_COLS = 512u;                    // two accumulators of 256 columns
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NSTAGE; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
+    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 2 * EPI_WARPS); }
     mbar_fence_init();
   }
   if (warp == 1) { tmem_alloc_pair(tmem_slot, TMEM_COLS); tmem_relinquish_pair(); }
@@ -149,11 +164,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
     // ===================== TMA producer (both CTAs) =====================
     if (lane == 0) {
       const CUtensorMap* mapA = (EPI <= EPI_DLOGITS && packed) ? &p.tmPacked : &p.tmA;
-      const CUtensorMap* mapB = (A_MN && packed) ? &p.tmPacked : &p.tmB;
+      const CUtensorMap* mapB = (p.rows_on_k && packed) ? &p.tmPacked : &p.tmB;
       tma_prefetch_desc(mapA);
       tma_prefetch_desc(mapB);
       int stage = 0; uint32_t phase = 0;
-      Work w(M, p.N, K, p.group_m, p.splits, pair, npairs);
+      Work w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         const int m0 = w.m * (2 * BM) + (int)cta * BM;
         const int n0 = w.n * BN + (int)cta * (BN / 2);
@@ -193,7 +208,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
       const uint32_t idesc = make_idesc_f16(2 * BM, BN, p.half ? 0 : 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
       int stage = 0; uint32_t phase = 0;
       int acc = 0; uint32_t acc_phase = 0;
-      Work w(M, p.N, K, p.group_m, p.splits, pair, npairs);
+      Work w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.status, 0x20u)) { alive = false; break; }
         tc_fence_after();
@@ -221,33 +236,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
       }
     }
   } else {
-    // ===================== epilogue (warps 2..5, both CTAs) =====================
-    const int q = warp & 3;                          // TMEM lane quarter this warp may access
-    const uint32_t buf_base = smem_base + L::EPI_OFFSET + (uint32_t)q * 2u * L::EPI_BUF;
+    // ===================== epilogue (warps 2..9, both CTAs) =====================
+    const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which 128 columns it takes
+    const uint32_t buf = smem_base + L::EPI_OFFSET + (uint32_t)(warp - 2) * L::EPI_BUF;
     const uint32_t lead_tempty[2] = {mapa_u32(tempty_bar(0), 0), mapa_u32(tempty_bar(1), 0)};
     const float unscale = (EPI >= EPI_OUT16 && p.scale) ? p.scale[1] : 1.f;
     const float ctau = p.inv_tau * LOG2E;
     int acc = 0; uint32_t acc_phase = 0;
-    uint32_t chunk = 0;
-    Work w(M, p.N, K, p.group_m, p.splits, pair, npairs);
+    Work w(M, p.N, K, p.group_m, splits, pair, npairs);
     while (alive && w.next()) {
       const int row0 = w.m * (2 * BM) + (int)cta * BM + q * 32, row = row0 + lane;
-      float coef = 0.f, lse = 0.f;
+      float coef = 0.f, lse = 0.f, at_label = 0.f;
+      long long label = -1;
       if (EPI == EPI_DLOGITS && row < rows) {
-        coef = p.g[(long long)p.rowmap[row] * p.g_stride] * p.g_factor;
+        const int t = p.rowmap[row];
+        coef = p.g[(long long)t * p.g_stride] * p.g_factor;
         if (p.scale) coef *= p.scale[0];
         lse = p.lse[row];
+        if (p.label) {
+          label = p.label[t] - p.piece_start;
+          at_label = coef == 0.f ? 0.f : (ex2((p.z[row] * p.inv_tau - lse) * LOG2E) - 1.f) * coef;
+        }
       }
       if (!mbar_wait_warp(tfull_bar(acc), acc_phase, p.status, 0x30u)) { alive = false; break; }
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
       if (EPI == EPI_STATS) {
-        // online softmax over the 256 columns of this row; differences are taken before the scaling so that the terms that weigh
+        // online softmax over this warp's columns of the row; differences are taken before the scaling so that the terms that weigh
         // most (z near the maximum) keep their bits
         float m = -INFINITY, s = 0.f;
+        int at = 0;
 #pragma unroll 1
-        for (int c2 = 0; c2 < BN; c2 += 64) {
-          const int left = p.N - (w.n * BN + c2);
+        for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
+          const int col0 = w.n * BN + c2, left = p.N - col0;
           if (left <= 0) break;
           uint32_t rr[64];
           tmem_ld_32x32(t_row + (uint32_t)c2, rr);
@@ -258,12 +279,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
             for (int j = 0; j < 64; ++j)
               if (j >= left) rr[j] = 0xff800000u;          // -inf: columns past the vocabulary
           }
+          if (p.zt && row < rows) {
+            float* z = p.zt + (long long)col0 * p.ldt + row;
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j < left) z[(long long)j * p.ldt] = __uint_as_float(rr[j]);
+          }
           float mx[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) mx[u] = __uint_as_float(rr[u]);
 #pragma unroll
           for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(rr[j]));
-          const float mn = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (cm > m) {
+#pragma unroll
+            for (int j = 63; j >= 0; --j) at = __uint_as_float(rr[j]) == cm ? (c2 & 64) + j : at;
+          }
+          const float mn = fmaxf(m, cm);
           const float base = mn == -INFINITY ? 0.f : mn;
           float sm[4] = {s * ex2((m - base) * ctau), 0.f, 0.f, 0.f};
 #pragma unroll
@@ -271,12 +303,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
           s = (sm[0] + sm[1]) + (sm[2] + sm[3]);
           m = mn;
         }
-        if (row < rows) p.part[(long long)w.n * p.part_ld + row] = make_float2(m, s);
+        if (row < rows) {
+          const long long o = (long long)(2 * w.n + half) * p.part_ld + row;
+          p.part[o] = make_float2(m, s);
+          p.part_at[o] = (unsigned char)at;
+        }
       } else {
         const uint32_t sw = (uint32_t)(lane & 7);
-        const bool empty = A_MN && w.kb1 == w.kb0;          // no row at all: the weight gradient is zero
+        const bool empty = w.kb1 == w.kb0;                // nothing to sum: no rows, or more splits than blocks of a short last piece
 #pragma unroll 1
-        for (int c2 = 0; c2 < BN; c2 += 64, ++chunk) {
+        for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
           const int col0 = w.n * BN + c2;
           if (col0 >= p.N) break;                       // the rest of this tile is beyond the last column
           uint32_t rr[64];
@@ -290,12 +326,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
               const float e = ex2(fmaf(__uint_as_float(rr[j]), p.inv_tau, -lse) * LOG2E) * coef;
               rr[j] = __float_as_uint(coef == 0.f ? 0.f : e);
             }
+            const long long j0 = label - col0;
+            if (__any_sync(0xffffffffu, j0 >= 0 && j0 < 64)) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) rr[j] = j0 == j ? __float_as_uint(at_label) : rr[j];
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < 64; ++j) rr[j] = empty ? 0u : __float_as_uint(__uint_as_float(rr[j]) * unscale);
           }
-          const uint32_t buf = buf_base + (chunk & 1u) * L::EPI_BUF;
-          if (lane == 0) tma_store_wait_read<1>();      // the store that last read this buffer (two chunks ago) is done with it
+          if (lane == 0) tma_store_wait_read<0>();      // the last store of this warp has read its buffer
           __syncwarp();
           const uint32_t row_addr = buf + (uint32_t)lane * 128u;
           if (EPI != EPI_OUT32) {
@@ -320,10 +360,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
           fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
           __syncwarp();
           if (lane == 0) {
-            // OUT32 of the hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box
-            const int y = (EPI == EPI_OUT32 && !A_MN) ? w.split * p.slab_rows + row0 : row0;
-            const bool inside = (EPI == EPI_OUT32 && !A_MN) ? row0 < p.slab_rows : row0 < p.M;
-            if (inside) {
+            // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box
+            const int y = p.split ? w.split * p.slab_rows + row0 : row0;
+            if (row0 < (p.split ? p.slab_rows : p.M)) {
               if (EPI != EPI_OUT32) {
                 tma_store_2d(&p.tmD, buf, col0, y);
               } else if (!p.accumulate) {
@@ -334,13 +373,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) lce_gemm_ker
                 if (col0 + 32 < p.N) tma_reduce_add_2d(&p.tmD, buf + 4096u, col0 + 32, y);
               }
             }
-            tma_store_commit();                           // one group per chunk, empty or not: the wait above counts groups
+            tma_store_commit();
           }
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(lead_tempty[acc]);   // this warp has read its lanes of the accumulator
+      if (lane == 0) mbar_arrive_remote(lead_tempty[acc]);   // this warp has read its part of the accumulator
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) tma_store_wait<0>();                 // staging buffers are read and the stores are complete before exit
@@ -366,6 +405,37 @@ __device__ __forceinline__ int label_kind(long long y, long long vocab, long lon
 }
 __device__ __forceinline__ bool place_used(long long i, float a, long long vocab) { return i >= 0 && i < vocab && !(a == -INFINITY); }
 
+__device__ __forceinline__ int list_kind(const long long* idx, const float* teacher, int K, long long vocab, long long ignore_index) {
+  if (!teacher) return label_kind(*idx, vocab, ignore_index);
+  bool used = false, bad = false;
+  for (int k = 0; k < K; ++k) {
+    used |= place_used(idx[k], teacher[k], vocab);
+    bad |= idx[k] >= vocab;
+  }
+  return bad ? 2 : used ? 1 : 0;
+}
+
+// K splits of the hidden gradient, for `n` rows.  Its tiles (256 rows x 256 of H) are few where there are few rows, or fill the last round of
+// the SM pairs badly; split along the vocabulary every pair gets a part, at the price of writing and adding more results.  Times in us: a
+// block of 64 words takes a tile 0.37, its read-out 2; the slabs move at 6 TB/s.  One warp; all lanes get the result.
+__device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs, int most, int lane) {
+  const int tiles = max(1, (n + 255) / 256 * ((H + 255) / 256));
+  float best_t = INFINITY;
+  int best = 1;
+  for (int s = lane + 1; s <= most; s += 32) {
+    const float t = (float)((tiles * s + pairs - 1) / pairs) * ((float)((blocks + s - 1) / s) * 0.37f + 2.f) + (float)s * n * H * (8.f / 6e6f);
+    if (t < best_t) { best_t = t; best = s; }
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t = __shfl_xor_sync(0xffffffffu, best_t, o);
+    const int s = __shfl_xor_sync(0xffffffffu, best, o);
+    if (t < best_t || (t == best_t && s < best)) { best_t = t; best = s; }
+  }
+  return best;
+}
+
+struct Splits { int blocks, pairs, most; };
+
 // One warp a token.
 __global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restrict__ idx, const float* __restrict__ teacher, int T, int K,
                                                        long long vocab, unsigned char* __restrict__ kind) {
@@ -383,53 +453,55 @@ __global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restri
 }
 
 // Numbers the rows that stay, in the order of the tokens: pos[t] = packed row, -1 ignored, -2 a word outside the vocabulary (also noted
-// in `error`); rowmap is the inverse.  One block: 8 tokens a thread and round, so up to 8192 tokens take one round.
-__global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restrict__ labels, const unsigned char* __restrict__ kind, int T,
-                                                        long long vocab, long long ignore_index, int* __restrict__ pos,
+// in `error`); rowmap is the inverse.  One block; a warp takes 256 neighbouring tokens a round (8192 tokens a round of the block), their
+// kinds as eight ballots.
+__global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restrict__ labels, const unsigned char* __restrict__ kind, int T, int H,
+                                                        long long vocab, long long ignore_index, Splits sp, int* __restrict__ pos,
                                                         int* __restrict__ rowmap, int* __restrict__ count, unsigned int* error) {
-  __shared__ int warp_sum_s[32];
+  __shared__ int warp_n[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
   for (long long t0 = 0; t0 < T; t0 += 8192) {
-    int kd[8], mine = 0;
-    const long long first = t0 + (long long)threadIdx.x * 8;
+    const long long first = t0 + warp * 256 + lane;
+    int kd[8];
+    unsigned int keep[8];
+    int mine = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const long long t = first + j;
+      const long long t = first + 32 * j;
       kd[j] = t >= T ? 0 : labels ? label_kind(labels[t], vocab, ignore_index) : kind[t];
-      mine += kd[j] == 1;
     }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    __syncthreads();                      // the sums of the last round have been read
-    if (lane == 31) warp_sum_s[warp] = incl;
-    __syncthreads();
-    int before = 0, total = 0;
-    for (int w = 0; w < 32; ++w) {
-      const int v = warp_sum_s[w];
-      before += w < warp ? v : 0;
-      total += v;
-    }
-    int at = base + before + incl - mine;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const long long t = first + j;
-      if (t >= T) break;
-      if (kd[j] == 1) {
-        pos[t] = at;
-        rowmap[at++] = (int)t;
-      } else {
-        pos[t] = kd[j] == 2 ? -2 : -1;
-        if (kd[j] == 2) atomicCAS(error, 0u, 0x703u);
-      }
+      keep[j] = __ballot_sync(0xffffffffu, kd[j] == 1);
+      mine += __popc(keep[j]);
     }
-    base += total;
+    __syncthreads();                      // the numbers of the last round have been read
+    if (lane == 0) warp_n[warp] = mine;
+    __syncthreads();
+    const int v = warp_n[lane];
+    int at = base + __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+    base += __reduce_add_sync(0xffffffffu, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long long t = first + 32 * j;
+      if (t < T) {
+        if (kd[j] == 1) {
+          const int i = at + __popc(keep[j] & ((1u << lane) - 1u));
+          pos[t] = i;
+          rowmap[i] = (int)t;
+        } else {
+          pos[t] = kd[j] == 2 ? -2 : -1;
+          if (kd[j] == 2) atomicCAS(error, 0u, 0x703u);
+        }
+      }
+      at += __popc(keep[j]);
+    }
   }
-  if (threadIdx.x == 0) *count = base;
+  if (warp == 0) {
+    const int s = choose_splits(base, H, sp.blocks, sp.pairs, sp.most, lane);
+    if (lane == 0) { count[0] = base; count[1] = s; }
+  }
 }
 
 // Dot product of two rows of H 16-bit values by one warp (H a multiple of 8, rows 16-byte aligned): fp32 sums, same value in all lanes.
@@ -454,18 +526,69 @@ __device__ __forceinline__ float warp_dot(const T* __restrict__ a, const T* __re
 // weights q, and  dot = sum q z / tau,  ent = sum q log q.  Tokens that left get loss 0 (NaN where a word is outside the vocabulary).
 // WPT warps a token: one for a single listed word, eight for lists.  Blocks past the tokens zero the packed rows up to the next
 // multiple of 64: the weight gradient reads whole blocks of 64 rows.
-template <typename T, int WPT>
+// SCAN (up to SCAN_MOST tokens with short lists): every block numbers the rows itself, which saves the launches of the scan; the first
+// block writes the numbers out.
+constexpr int SCAN_MOST = 2048, SCAN_LIST = 16;
+template <typename T, int WPT, bool SCAN>
 __global__ void __launch_bounds__(256) lce_rows_kernel(const T* __restrict__ hidden, long long ldh, const T* __restrict__ weight, long long ldw,
                                                        const long long* __restrict__ idx, const float* __restrict__ teacher, int Tn, int H,
-                                                       int K, int vocab_local, long long vocab_start, long long vocab, float inv_tau,
-                                                       const int* __restrict__ pos, const int* __restrict__ count, T* __restrict__ packed,
+                                                       int K, int vocab_local, long long vocab_start, long long vocab, long long ignore_index,
+                                                       float inv_tau, Splits sp, int* __restrict__ pos, int* __restrict__ rowmap,
+                                                       int* __restrict__ count, unsigned int* error, T* __restrict__ packed,
                                                        float* __restrict__ z, float* __restrict__ qout, float* __restrict__ dot,
                                                        float* __restrict__ ent, float* __restrict__ loss) {
   constexpr int PER_BLOCK = 8 / WPT;
   extern __shared__ float zs[];            // WPT = 8: the token's K logits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = *count;
   const int token_blocks = (Tn + PER_BLOCK - 1) / PER_BLOCK;
+  const int t = (int)blockIdx.x * PER_BLOCK + (WPT == 1 ? warp : 0);
+  int n, at = -1;
+  if (SCAN) {
+    __shared__ unsigned int keep[SCAN_MOST / 32], wrong[SCAN_MOST / 32];
+    const int words = (Tn + 31) / 32;
+    for (int w = warp; w < words; w += 8) {
+      const int u = w * 32 + lane;
+      const int kd = u < Tn ? list_kind(idx + (long long)u * K, teacher ? teacher + (long long)u * K : nullptr, K, vocab, ignore_index) : 0;
+      const unsigned int k = __ballot_sync(0xffffffffu, kd == 1), b = __ballot_sync(0xffffffffu, kd == 2);
+      if (lane == 0) { keep[w] = k; wrong[w] = b; }
+    }
+    __syncthreads();
+    // rows kept in words below `w`, over all of them for the last
+    auto below = [&](int w) {
+      int c = 0;
+      for (int i = lane; i < w; i += 32) c += __popc(keep[i]);
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    n = below(words);
+    if (t < Tn) {
+      const unsigned int bit = 1u << (t & 31);
+      const int b = below(t >> 5);
+      at = keep[t >> 5] & bit ? b + __popc(keep[t >> 5] & (bit - 1u)) : wrong[t >> 5] & bit ? -2 : -1;
+    }
+    if (blockIdx.x == 0) {
+      for (int w = warp; w < words; w += 8) {
+        const int u = w * 32 + lane, b = below(w);
+        const unsigned int bit = 1u << lane;
+        if (u < Tn) {
+          if (keep[w] & bit) {
+            const int i = b + __popc(keep[w] & (bit - 1u));
+            pos[u] = i;
+            rowmap[i] = u;
+          } else {
+            pos[u] = wrong[w] & bit ? -2 : -1;
+            if (wrong[w] & bit) atomicCAS(error, 0u, 0x703u);
+          }
+        }
+      }
+      if (warp == 0) {
+        const int s = choose_splits(n, H, sp.blocks, sp.pairs, sp.most, lane);
+        if (lane == 0) { count[0] = n; count[1] = s; }
+      }
+    }
+  } else {
+    n = *count;
+    if (t < Tn) at = pos[t];
+  }
   if ((int)blockIdx.x >= token_blocks) {
     const int r = n + ((int)blockIdx.x - token_blocks);
     if (n == Tn || r >= min(Tn, (n + 63) / 64 * 64)) return;
@@ -473,9 +596,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const T* __restrict__ hid
     for (int c = threadIdx.x * 8; c < H; c += 2048) *reinterpret_cast<uint4*>(packed + (long long)r * H + c) = zero;
     return;
   }
-  const int t = (int)blockIdx.x * PER_BLOCK + (WPT == 1 ? warp : 0);
   if (t >= Tn) return;
-  const int at = pos[t];
   if (at < 0) {
     if (lane == 0 && (WPT == 1 || warp == 0)) loss[t] = at == -2 ? NAN : 0.f;
     return;
@@ -536,40 +657,61 @@ __device__ __forceinline__ void lce_finish(float m, float s, float dot, float en
   *loss = tau2 * (ent + (m * inv_tau - dot) + ls);       // the two large numbers are subtracted first
 }
 
-// 32 rows a block (coalesced over the rows), 32 threads a row over the column tiles; the order of the sums is fixed.
-__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, long long part_ld, int tiles, float inv_tau, float tau2,
+// 32 rows a block (coalesced over the rows), 32 threads a row over the 128-column parts; the order of the sums is fixed.  Then one warp a
+// row computes the largest logit again in fp32 and rebases the sum on it: s = 1 + (s - 1) exp((m - m') / tau), m' the new value.
+template <typename T>
+__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, const unsigned char* __restrict__ part_at,
+                                                        long long part_ld, int parts, const T* __restrict__ hidden, long long ldh,
+                                                        const T* __restrict__ weight, long long ldw, int H, float inv_tau, float tau2,
                                                         const int* __restrict__ count, const int* __restrict__ rowmap,
                                                         const float* __restrict__ dot, const float* __restrict__ ent, float* __restrict__ mo,
                                                         float* __restrict__ so, float* __restrict__ lse, float* __restrict__ loss) {
   __shared__ float ms[32][33], ss[32][33];
+  __shared__ int as[32][33];
   const int r = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int n = *count, row = blockIdx.x * 32 + r;
+  const int n = *count;
   if ((int)blockIdx.x * 32 >= n) return;
   const float c = inv_tau * LOG2E;
-  float m = -INFINITY, s = 0.f;
-  if (row < n)
-    for (int i = y; i < tiles; i += 32) {
-      const float2 v = part[(long long)i * part_ld + row];
-      const float mn = fmaxf(m, v.x), base = mn == -INFINITY ? 0.f : mn;
-      s = s * ex2((m - base) * c) + v.y * ex2((v.x - base) * c);
-      m = mn;
+  {
+    const int row = blockIdx.x * 32 + r;
+    float m = -INFINITY, s = 0.f;
+    int at = 0;
+    if (row < n) {
+#pragma unroll 4
+      for (int i = y; i < parts; i += 32) {
+        const float2 v = part[(long long)i * part_ld + row];
+        const float mn = fmaxf(m, v.x), base = mn == -INFINITY ? 0.f : mn;
+        s = s * ex2((m - base) * c) + v.y * ex2((v.x - base) * c);
+        if (v.x > m) at = i;
+        m = mn;
+      }
+      at = at * 128 + part_at[(long long)at * part_ld + row];
     }
-  ms[y][r] = m;
-  ss[y][r] = s;
+    ms[y][r] = m;
+    ss[y][r] = s;
+    as[y][r] = at;
+  }
   __syncthreads();
-  if (y == 0 && row < n) {
-    float mm = -INFINITY;
-    for (int i = 0; i < 32; ++i) mm = fmaxf(mm, ms[i][r]);
-    float t = 0.f;
-    for (int i = 0; i < 32; ++i) t += ss[i][r] * ex2((ms[i][r] - (ms[i][r] == -INFINITY && mm != -INFINITY ? 0.f : mm)) * c);
+  const int row = blockIdx.x * 32 + y, lane = r;
+  if (row >= n) return;
+  const float m = ms[lane][y];
+  const float mm = warp_max(m);
+  const float s = warp_sum(ss[lane][y] * ex2((m - (m == -INFINITY && mm != -INFINITY ? 0.f : mm)) * c));
+  const unsigned int who = __ballot_sync(0xffffffffu, m == mm);
+  const int word = who ? as[__ffs(who) - 1][y] : 0;
+  const int t = rowmap[row];
+  const float again = warp_dot(hidden + (long long)t * ldh, weight + (long long)word * ldw, H, lane);
+  if (lane == 0) {
+    const float m2 = mm == -INFINITY ? mm : again;         // nothing but -inf: NaN, as the formula
+    const float s2 = 1.f + (s - 1.f) * ex2((mm - m2) * c);
     if (mo) {
-      mo[row] = mm;
-      so[row] = t;
+      mo[row] = m2;
+      so[row] = s2;
     } else {
       float l, o;
-      lce_finish(mm, t, dot[row], ent[row], inv_tau, tau2, &l, &o);
+      lce_finish(m2, s2, dot[row], ent[row], inv_tau, tau2, &l, &o);
       lse[row] = l;
-      loss[rowmap[row]] = o;
+      loss[t] = o;
     }
   }
 }
@@ -614,7 +756,7 @@ __global__ void __launch_bounds__(1024) lce_scale_kernel(const float* __restrict
 // The listed words' entries of the piece: dz[i, v] = (exp(z / tau - lse) - sum of the q of all places that list v) * coefficient.  Places
 // that list a word twice write the same value.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, long long ldz, const long long* __restrict__ idx,
+__global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, long long ld_row, long long ld_word, const long long* __restrict__ idx,
                                                          const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lse,
                                                          const int* __restrict__ rowmap, const int* __restrict__ count, int K,
                                                          long long piece_start, int piece_cols, const float* __restrict__ g, int g_stride,
@@ -637,14 +779,63 @@ __global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, lon
   float coef = g[(long long)t * g_stride] * g_factor;
   if (scale) coef *= scale[0];
   const float p = ex2((z[(long long)i * K + k] * inv_tau - lse[i]) * LOG2E);
-  dz[(long long)i * ldz + v] = from_f<T>(coef == 0.f ? 0.f : (p - sum) * coef);
+  dz[i * ld_row + v * ld_word] = from_f<T>(coef == 0.f ? 0.f : (p - sum) * coef);
+}
+
+// dz of kept logits, both [V, ldt] with the rows innermost: eight rows of one word a thread.  Rows past the last are zero.
+template <typename T>
+__global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int V, const float* __restrict__ lse,
+                                                     const long long* __restrict__ label, const float* __restrict__ z,
+                                                     const int* __restrict__ rowmap, const int* __restrict__ count, long long vocab_start,
+                                                     const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
+                                                     const float* __restrict__ scale) {
+  const int groups = ldt / 8, n = *count;
+  // the block's threads take (256 / groups) words a round, always the same rows
+  const int per = max(1, 256 / groups), grp = threadIdx.x % groups, sub = threadIdx.x / groups;
+  if (sub >= per) return;
+  for (int g0 = grp; g0 < groups; g0 += 256) {
+    float coef[8], ls[8], atl[8];
+    long long lab[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = g0 * 8 + j;
+      coef[j] = ls[j] = atl[j] = 0.f;
+      lab[j] = -1;
+      if (i < n) {
+        const int t = rowmap[i];
+        coef[j] = g[(long long)t * g_stride] * g_factor;
+        if (scale) coef[j] *= scale[0];
+        ls[j] = lse[i];
+        if (label) {
+          lab[j] = label[t] - vocab_start;
+          atl[j] = (ex2((z[i] * inv_tau - ls[j]) * LOG2E) - 1.f) * coef[j];
+        }
+      }
+    }
+#pragma unroll 2
+    for (int v = blockIdx.x * per + sub; v < V; v += gridDim.x * per) {
+      const long long o = (long long)v * ldt + g0 * 8;
+      Vec8<float> x;
+      x.load(zt + o);
+      float f[8];
+      x.to_float(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], inv_tau, -ls[j]) * LOG2E) * coef[j];
+        f[j] = coef[j] == 0.f ? 0.f : e;
+      }
+      Vec8<T> w;
+      w.from_float(f);
+      w.store(dz + o);
+    }
+  }
 }
 
 // d hidden: the fp32 slabs of the K splits, added in order, back in the order of the tokens; zero rows for tokens that left.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restrict__ acc, int splits, long long slab, const int* __restrict__ pos,
+__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restrict__ acc, const int* __restrict__ count, long long slab, const int* __restrict__ pos,
                                                           T* __restrict__ out, int Tn, int H) {
-  const int per_row = H / 8;
+  const int per_row = H / 8, splits = count[1];
   const long long total = (long long)Tn * per_row;
   for (long long f = (long long)blockIdx.x * 256 + threadIdx.x; f < total; f += (long long)gridDim.x * 256) {
     const int t = (int)(f / per_row), c = (int)(f - (long long)t * per_row) * 8;
@@ -668,14 +859,14 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restric
 // launchers
 // ---------------------------------------------------------------------------------------------------------
 template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(const LceGemm& p, cudaStream_t s) {
+int launch_gemm(const LceGemm& p, int most_splits, cudaStream_t s) {
   using L = Cfg<EPI>;
   auto kern = lce_gemm_kernel<EPI, A_MN, B_MN>;
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
-  const long long items = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN) * p.splits;
+  const long long items = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN) * most_splits;
   const int pairs = (int)std::min<long long>(items, msb::num_sms() / 2);
-  kern<<<2 * pairs, 192, L::TOTAL, s>>>(p);
+  kern<<<2 * pairs, THREADS, L::TOTAL, s>>>(p);
   MSB_CHECK_LAUNCH("lce_gemm");
   return 0;
 }
@@ -697,7 +888,7 @@ struct MsbLceArgs {
   float tau;
   int* pos;                    // [T]
   int* rowmap;                 // [T]
-  int* count;                  // [1]
+  int* count;                  // [2]: rows that stay, K splits
   unsigned char* kind;         // [T] scratch (lists)
   void* packed;                // [T, H]
   float* z;                    // [T, K]
@@ -706,17 +897,20 @@ struct MsbLceArgs {
   float* ent;                  // [T]
   float* lse;                  // [T]
   float* loss;                 // [T]
-  float* part;                 // [column tiles, T] pairs, scratch
+  float* part;                 // [ceil(V / 256) * 2, T] pairs, scratch
+  unsigned char* part_at;      // [ceil(V / 256) * 2, T] scratch
+  float* zt;                   // [V, ldt] logits kept for the backward, or null
+  int ldt;                     // T rounded up to a multiple of 8
   float* mx;                   // [T], [T]: local statistics for the vocabulary-parallel form, else null
   float* sum;
   // backward
   const float* g;
   long long g_stride;          // 0: one value for all tokens
-  void* dz;                    // [T, piece] scratch, row pitch ldz
+  void* dz;                    // [T, piece] scratch, row pitch ldz; with zt [V, ldt]
   long long ldz;
   int piece;                   // columns of a piece (a multiple of 256)
   float* acc;                  // [splits, slab_rows, H] fp32 scratch, or null: no hidden gradient
-  int splits, slab_rows;
+  int splits, slab_rows;       // most K splits (both directions are given the same, and the same piece)
   void* dhidden;               // [T, H]
   void* dweight;               // [V, H], 16-bit or fp32; null: no weight gradient
   int dweight_fp32_add;        // dweight is fp32 and added to
@@ -731,49 +925,64 @@ static int lce_check(const MsbLceArgs* a) {
   MSB_REQUIRE(a->status != nullptr, "linear_ce: status words are required");
   MSB_REQUIRE(a->tau > 0.f, "linear_ce: the temperature must be positive");
   MSB_REQUIRE(a->K == 1 || a->teacher, "linear_ce: lists need teacher logits");
+  MSB_REQUIRE(!a->zt || (a->ldt % 8 == 0 && a->ldt >= a->T), "linear_ce: pitch %d of the kept logits", a->ldt);
+  MSB_REQUIRE(a->piece > 0 && a->piece % BN == 0 && a->splits >= 1, "linear_ce: piece of %d columns, %d splits", a->piece, a->splits);
   return 0;
 }
 
-// Scan, rows, GEMM with row statistics, join.  With `mx` the join stops at the local (max, sum).
-MSB_API int msb_lce_forward(const MsbLceArgs* a, cudaStream_t s) {
-  if (int rc = lce_check(a)) return rc;
+template <typename DT>
+static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const float inv_tau = 1.f / a->tau, tau2 = a->tau * a->tau;
-  if (a->teacher) {
-    lce_kind_kernel<<<(a->T + 7) / 8, 256, 0, s>>>(a->idx, a->teacher, a->T, a->K, a->vocab, a->kind);
-    MSB_CHECK_LAUNCH("lce_kind");
+  const DT* hidden = (const DT*)a->hidden;
+  const DT* weight = (const DT*)a->weight;
+  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, msb::num_sms() / 2, a->splits};
+  const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
+  if (!scan) {
+    if (a->teacher) {
+      lce_kind_kernel<<<(a->T + 7) / 8, 256, 0, s>>>(a->idx, a->teacher, a->T, a->K, a->vocab, a->kind);
+      MSB_CHECK_LAUNCH("lce_kind");
+    }
+    lce_scan_kernel<<<1, 1024, 0, s>>>(a->teacher ? nullptr : a->idx, a->kind, a->T, a->H, a->vocab, a->ignore_index, sp, a->pos, a->rowmap,
+                                       a->count, a->status + 1);
+    MSB_CHECK_LAUNCH("lce_scan");
   }
-  lce_scan_kernel<<<1, 1024, 0, s>>>(a->teacher ? nullptr : a->idx, a->kind, a->T, a->vocab, a->ignore_index, a->pos, a->rowmap, a->count,
-                                     a->status + 1);
-  MSB_CHECK_LAUNCH("lce_scan");
   const int per_block = a->teacher ? 1 : 8;
   const unsigned grid = (unsigned)((a->T + per_block - 1) / per_block + 63);
-#define LCE_ROWS(DT, WPT)                                                                                                                    \
-  lce_rows_kernel<DT, WPT><<<grid, 256, WPT == 8 ? a->K * 4 : 0, s>>>((const DT*)a->hidden, a->ldh, (const DT*)a->weight, a->ldw, a->idx,      \
-                                                                     a->teacher, a->T, a->H, a->K, a->V, a->vocab_start, a->vocab, inv_tau,   \
-                                                                     a->pos, a->count, (DT*)a->packed, a->z, a->q, a->dot, a->ent, a->loss)
-  if (a->dtype == MSB_F16) { if (a->teacher) LCE_ROWS(__half, 8); else LCE_ROWS(__half, 1); }
-  else { if (a->teacher) LCE_ROWS(__nv_bfloat16, 8); else LCE_ROWS(__nv_bfloat16, 1); }
+#define LCE_ROWS(WPT, SCAN)                                                                                                                  \
+  lce_rows_kernel<DT, WPT, SCAN><<<grid, 256, WPT == 8 ? a->K * 4 : 0, s>>>(hidden, a->ldh, weight, a->ldw, a->idx, a->teacher, a->T, a->H,    \
+                                                                           a->K, a->V, a->vocab_start, a->vocab, a->ignore_index, inv_tau,  \
+                                                                           sp, a->pos, a->rowmap, a->count, a->status + 1, (DT*)a->packed,  \
+                                                                           a->z, a->q, a->dot, a->ent, a->loss)
+  if (a->teacher) { if (scan) LCE_ROWS(8, true); else LCE_ROWS(8, false); }
+  else { if (scan) LCE_ROWS(1, true); else LCE_ROWS(1, false); }
 #undef LCE_ROWS
   MSB_CHECK_LAUNCH("lce_rows");
   LceGemm p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType dt = map_type(a->dtype);
   int rc;
-  if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
+  if ((rc = make_tmap_2d(&p.tmA, hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
   if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
-  if ((rc = make_tmap_2d(&p.tmB, a->weight, dt, 2, a->V, a->H, a->ldw, BN / 2, BK))) return rc;
+  if ((rc = make_tmap_2d(&p.tmB, weight, dt, 2, a->V, a->H, a->ldw, BN / 2, BK))) return rc;
   p.M = a->T; p.N = a->V; p.K = a->H;
   p.rows = a->count; p.all_rows = a->T;
-  p.group_m = 8; p.splits = 1;
+  p.group_m = GROUP_M;
   p.half = a->dtype == MSB_F16;
-  p.part = reinterpret_cast<float2*>(a->part); p.part_ld = a->T;
+  p.part = reinterpret_cast<float2*>(a->part); p.part_at = a->part_at; p.part_ld = a->T;
+  p.zt = a->zt; p.ldt = a->ldt;
   p.inv_tau = inv_tau;
   p.status = a->status;
-  if ((rc = launch_gemm<EPI_STATS, false, false>(p, s))) return rc;
-  lce_join_kernel<<<(a->T + 31) / 32, 1024, 0, s>>>(p.part, p.part_ld, (a->V + BN - 1) / BN, inv_tau, tau2, a->count, a->rowmap, a->dot, a->ent,
-                                                    a->mx, a->sum, a->lse, a->loss);
+  if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, s))) return rc;
+  lce_join_kernel<DT><<<(a->T + 31) / 32, 1024, 0, s>>>(p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden, a->ldh, weight, a->ldw, a->H,
+                                                        inv_tau, tau2, a->count, a->rowmap, a->dot, a->ent, a->mx, a->sum, a->lse, a->loss);
   MSB_CHECK_LAUNCH("lce_join");
   return 0;
+}
+
+// Scan, rows, GEMM with row statistics, join.  With `mx` the join stops at the local (max, sum).
+MSB_API int msb_lce_forward(const MsbLceArgs* a, cudaStream_t s) {
+  if (int rc = lce_check(a)) return rc;
+  return a->dtype == MSB_F16 ? lce_forward<__half>(a, s) : lce_forward<__nv_bfloat16>(a, s);
 }
 
 // Vocabulary-parallel form: sum *= exp((local max - global max) / tau), then (after the sums over the group) the loss.
@@ -789,16 +998,12 @@ MSB_API int msb_lce_loss(const float* gmx, const float* gsum, const float* dot, 
   return 0;
 }
 
-// Hidden and weight gradients, a piece of the vocabulary at a time.
-MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
-  if (int rc = lce_check(a)) return rc;
-  MSB_REQUIRE(a->piece > 0 && a->piece % BN == 0 && a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V), "linear_ce: piece of %d columns, pitch %lld", a->piece, a->ldz);
-  MSB_REQUIRE(!a->acc || (a->splits >= 1 && a->slab_rows >= a->T && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
-              "linear_ce: %d slabs of %d rows", a->splits, a->slab_rows);
-  MSB_REQUIRE(!a->acc || a->splits <= (a->V + BK - 1) / BK, "linear_ce: more K splits than blocks of %d words", BK);
-  MSB_REQUIRE(!a->acc || a->splits == 1 || a->piece >= a->V, "linear_ce: K splits need the vocabulary in one piece");
+template <typename DT>
+static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   const float inv_tau = 1.f / a->tau;
   const CUtensorMapDataType dt = map_type(a->dtype);
+  const long long* label = a->teacher ? nullptr : a->idx;
+  DT* dz = (DT*)a->dz;
   if (a->scale) {
     lce_scale_kernel<<<1, 1024, 0, s>>>(a->g, (int)a->g_stride, a->rowmap, a->count, a->tau, a->scale);
     MSB_CHECK_LAUNCH("lce_scale");
@@ -806,63 +1011,84 @@ MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   LceGemm p;
   memset(&p, 0, sizeof(p));
   p.rows = a->count; p.all_rows = a->T;
+  p.group_m = GROUP_M;
   p.half = a->dtype == MSB_F16;
   p.rowmap = a->rowmap; p.lse = a->lse;
   p.g = a->g; p.g_stride = (int)a->g_stride; p.g_factor = a->tau;
   p.inv_tau = inv_tau;
+  p.label = label; p.z = a->z;
   p.scale = a->scale;
   p.status = a->status;
+  const int piece = a->zt ? a->V : a->piece;       // kept logits are few
   int rc;
-  for (long long v0 = 0; v0 < a->V; v0 += a->piece) {
-    const int cols = (int)std::min<long long>(a->piece, a->V - v0);
-    const char* w = (const char*)a->weight + v0 * a->ldw * 2;
+  for (long long v0 = 0; v0 < a->V; v0 += piece) {
+    const int cols = (int)std::min<long long>(piece, a->V - v0);
+    const DT* w = (const DT*)a->weight + v0 * a->ldw;
     // dz of the piece
-    if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
-    if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
-    if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BN / 2, BK))) return rc;
-    if ((rc = make_tmap_2d(&p.tmD, a->dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
-    p.M = a->T; p.N = cols; p.K = a->H; p.group_m = 8; p.splits = 1; p.accumulate = 0;
-    if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, s))) return rc;
-    const long long places = (long long)a->T * a->K;
-    const unsigned grid = (unsigned)((places + 255) / 256);
-    if (a->dtype == MSB_F16)
-      lce_listed_kernel<__half><<<grid, 256, 0, s>>>((__half*)a->dz, a->ldz, a->idx, a->z, a->q, a->lse, a->rowmap, a->count, a->K,
-                                                     a->vocab_start + v0, cols, a->g, (int)a->g_stride, a->tau, inv_tau, a->scale);
-    else
-      lce_listed_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>((__nv_bfloat16*)a->dz, a->ldz, a->idx, a->z, a->q, a->lse, a->rowmap, a->count, a->K,
-                                                            a->vocab_start + v0, cols, a->g, (int)a->g_stride, a->tau, inv_tau, a->scale);
-    MSB_CHECK_LAUNCH("lce_listed");
+    if (a->zt) {
+      const int per = std::max(1, 256 / (a->ldt / 8));
+      const int grid = (int)std::min<long long>((a->V + per - 1) / per, (long long)msb::num_sms() * 8);
+      lce_dz_kernel<DT><<<grid, 256, 0, s>>>(a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start, a->g,
+                                             (int)a->g_stride, a->tau, inv_tau, a->scale);
+      MSB_CHECK_LAUNCH("lce_dz");
+    } else {
+      if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
+      if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
+      if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BN / 2, BK))) return rc;
+      if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
+      p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.piece_start = a->vocab_start + v0;
+      if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, s))) return rc;
+    }
+    if (a->teacher) {
+      const long long places = (long long)a->T * a->K;
+      lce_listed_kernel<DT><<<(unsigned)((places + 255) / 256), 256, 0, s>>>(dz, a->zt ? 1 : a->ldz, a->zt ? a->ldt : 1, a->idx, a->z, a->q, a->lse,
+                                                                            a->rowmap, a->count, a->K, a->vocab_start + v0, cols, a->g,
+                                                                            (int)a->g_stride, a->tau, inv_tau, a->scale);
+      MSB_CHECK_LAUNCH("lce_listed");
+    }
     if (a->acc) {
-      if ((rc = make_tmap_2d(&p.tmA, a->dz, dt, 2, a->T, cols, a->ldz, BM, BK))) return rc;
+      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, a->T, a->ldt, BK, 64);
+      else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BM, BK);
+      if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
-      p.M = a->T; p.N = a->H; p.K = cols; p.splits = a->splits; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
-      if ((rc = launch_gemm<EPI_OUT32, false, true>(p, s))) return rc;
+      p.M = a->T; p.N = a->H; p.K = cols; p.rows_on_k = 0; p.split = 1; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
+      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, s);
+      if (rc) return rc;
     }
     if (a->dweight) {
-      if ((rc = make_tmap_2d(&p.tmA, a->dz, dt, 2, a->T, cols, a->ldz, BK, 64))) return rc;
+      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, a->T, a->ldt, BM, BK);
+      else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BK, 64);
+      if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, a->hidden, dt, 2, a->T, a->H, a->ldh, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BK, 64))) return rc;
-      p.M = cols; p.N = a->H; p.K = a->T; p.splits = 1; p.slab_rows = 0;
+      p.M = cols; p.N = a->H; p.K = a->T; p.rows_on_k = 1; p.split = 0;
       if (a->dweight_fp32_add) {
-        float* d = (float*)a->dweight + v0 * a->H;
-        if ((rc = make_tmap_2d(&p.tmD, d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
+        if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
-        if ((rc = launch_gemm<EPI_OUT32, true, true>(p, s))) return rc;
+        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, 1, s) : launch_gemm<EPI_OUT32, true, true>(p, 1, s);
       } else {
-        if ((rc = make_tmap_2d(&p.tmD, (char*)a->dweight + v0 * a->H * 2, dt, 2, cols, a->H, a->H, 32, 64))) return rc;
+        if ((rc = make_tmap_2d(&p.tmD, (DT*)a->dweight + v0 * a->H, dt, 2, cols, a->H, a->H, 32, 64))) return rc;
         p.accumulate = 0;
-        if ((rc = launch_gemm<EPI_OUT16, true, true>(p, s))) return rc;
+        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, 1, s) : launch_gemm<EPI_OUT16, true, true>(p, 1, s);
       }
+      if (rc) return rc;
     }
   }
   if (a->acc) {
     const long long vecs = (long long)a->T * (a->H / 8);
     const unsigned grid = (unsigned)std::min<long long>((vecs + 255) / 256, (long long)msb::num_sms() * 16);
-    const long long slab = (long long)a->slab_rows * a->H;
-    if (a->dtype == MSB_F16) lce_dhidden_kernel<__half><<<grid, 256, 0, s>>>(a->acc, a->splits, slab, a->pos, (__half*)a->dhidden, a->T, a->H);
-    else lce_dhidden_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a->acc, a->splits, slab, a->pos, (__nv_bfloat16*)a->dhidden, a->T, a->H);
+    lce_dhidden_kernel<DT><<<grid, 256, 0, s>>>(a->acc, a->count, (long long)a->slab_rows * a->H, a->pos, (DT*)a->dhidden, a->T, a->H);
     MSB_CHECK_LAUNCH("lce_dhidden");
   }
   return 0;
+}
+
+// Hidden and weight gradients, a piece of the vocabulary at a time.
+MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
+  if (int rc = lce_check(a)) return rc;
+  MSB_REQUIRE(a->zt || (a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V)), "linear_ce: pitch %lld of a piece of %d columns", a->ldz, a->piece);
+  MSB_REQUIRE(!a->acc || (a->slab_rows >= a->T && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
+              "linear_ce: %d slabs of %d rows", a->splits, a->slab_rows);
+  return a->dtype == MSB_F16 ? lce_backward<__half>(a, s) : lce_backward<__nv_bfloat16>(a, s);
 }

@@ -9,20 +9,27 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import loader
 from ._dtypes import CODE, code
 from .linear_cross_entropy import _on_device
 
-_F = ctypes.c_float
 MAX_EXPERTS = 1024
+
+
+def _lib():
+    L = loader.require_lib()
+    if L.msb_balance_forward.argtypes is None:
+        P, I, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+        L.msb_balance_backward.argtypes = [P, P, I, I, I, I, F, P, I, P, P]
+        L.msb_balance_forward.argtypes = [P, P, I, I, I, I, F, I, P, P, I, P, P, P, P, P, P]
+    return L
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, routing_map, scale, sigmoid, B):
-        L = loader.require_lib()
+        L = _lib()
         dev = logits.device
         x, rmap = logits.contiguous(), routing_map.contiguous()
         T, E = x.shape
@@ -31,36 +38,35 @@ class _BalanceLoss(torch.autograd.Function):
             blocks = L.msb_balance_blocks(S, B, E)
             n = B * blocks * E
             parts = B * ((E + 31) // 32)
-            buf = torch.empty(2 * n + parts + 1, dtype=torch.float32, device=dev)     # sums of p, counts, joined products, ticket
-            load = torch.empty(B, E, dtype=torch.float32, device=dev)
+            buf = torch.empty(B * E + 2 * n + parts + 1, dtype=torch.float32, device=dev)   # loads; sums of p, counts, joined products, ticket
             loss = torch.empty((), dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int64, device=dev)
-            b = buf.data_ptr()
-            P = ctypes.c_void_p
-            loader.check(L.msb_balance_forward(loader.p(x), loader.p(rmap), S, B, E, int(sigmoid), _F(scale), code(x.dtype), P(b), P(b + 4 * n),
-                                               blocks, loader.p(load), P(b + 8 * n), P(b + 8 * n + 4 * parts), loader.p(loss),
-                                               loader.p(counts), P(loader.stream_ptr())), "balance_forward")
-        ctx.save_for_backward(x, load)
+            load = buf.data_ptr()
+            at = load + 4 * B * E
+            loader.check(L.msb_balance_forward(x.data_ptr(), rmap.data_ptr(), S, B, E, sigmoid, scale, code(x.dtype), at, at + 4 * n, blocks, load,
+                                               at + 8 * n, at + 8 * n + 4 * parts, loss.data_ptr(), counts.data_ptr(), loader.stream_ptr()),
+                         "balance_forward")
+        ctx.save_for_backward(x, buf)
         ctx.meta = (scale, sigmoid, B)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, _):
         if g is None:
             return None, None, None, None, None
-        L = loader.require_lib()
-        x, load = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            raise RuntimeError("router_balance_loss has no second derivative (create_graph)")
+        L = _lib()
+        x, buf = ctx.saved_tensors
         x = x.contiguous()
         scale, sigmoid, B = ctx.meta
         T, E = x.shape
         with _on_device(x.device):
-            g = g.float()
             grad = torch.empty_like(x)
-            loader.check(L.msb_balance_backward(loader.p(x), loader.p(load), T // B, B, E, int(sigmoid), _F(scale), loader.p(g), code(x.dtype),
-                                                loader.p(grad), ctypes.c_void_p(loader.stream_ptr())), "balance_backward")
+            loader.check(L.msb_balance_backward(x.data_ptr(), buf.data_ptr(), T // B, B, E, sigmoid, scale, g.data_ptr(), code(x.dtype),
+                                                grad.data_ptr(), loader.stream_ptr()), "balance_backward")
         return grad, None, None, None, None
 
 
@@ -102,5 +108,5 @@ def router_balance_loss(logits, routing_map, topk, coeff, score_function="softma
             raise TypeError(f"router_balance_loss: the sm_100a kernels take fp32, bf16 or fp16, not {logits.dtype}")
         if E > MAX_EXPERTS or T > 1 << 24:
             raise ValueError(f"router_balance_loss: {E} experts (at most {MAX_EXPERTS}), {T} tokens (at most 2^24)")
-        return _BalanceLoss.apply(logits, routing_map, scale, sigmoid, int(batch_size))
+        return _BalanceLoss.apply(logits, routing_map, scale, int(sigmoid), int(batch_size))
     return _balance_ref(logits, routing_map, scale, sigmoid, int(batch_size))

@@ -6,7 +6,8 @@
 
 Both take ``hidden`` [..., H] and ``weight`` [V, H] in bf16 or fp16 (H a multiple of 8) and return the loss in fp32 with the leading shape
 of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token, the backward makes the logits again, a
-piece of the vocabulary at a time.  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
+piece of the vocabulary at a time.  (For few tokens, at most a sixteenth of H, the fp32 logits take at most an eighth of the weight's bytes;
+then they are kept instead.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
 teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
 
 A label or teacher index beyond the vocabulary gives its token loss NaN and no gradient, and makes ``ops.gemm.check_status`` raise.
@@ -23,10 +24,10 @@ On a CPU the same functions run as eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.distributed as dist
-from torch.autograd.function import once_differentiable
 
 from . import gemm as G
 from . import loader
@@ -34,8 +35,9 @@ from ._dtypes import code
 
 _P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 
-#: bytes of the 16-bit logit gradients that the backward holds at a time
+#: bytes of the 16-bit logit gradients that the backward holds at a time, and of the fp32 partial results of the hidden gradient
 PIECE_BYTES = 512 << 20
+SLAB_BYTES = 256 << 20
 MAX_LIST = 1024
 
 
@@ -43,7 +45,7 @@ class _Args(ctypes.Structure):
     _fields_ = [("hidden", _P), ("weight", _P), ("idx", _P), ("teacher", _P), ("ldh", _LL), ("ldw", _LL), ("vocab_start", _LL), ("vocab", _LL),
                 ("ignore_index", _LL), ("T", _I), ("H", _I), ("V", _I), ("K", _I), ("dtype", _I), ("tau", _F), ("pos", _P), ("rowmap", _P),
                 ("count", _P), ("kind", _P), ("packed", _P), ("z", _P), ("q", _P), ("dot", _P), ("ent", _P), ("lse", _P), ("loss", _P),
-                ("part", _P), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
+                ("part", _P), ("part_at", _P), ("zt", _P), ("ldt", _I), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
                 ("splits", _I), ("slab_rows", _I), ("dhidden", _P), ("dweight", _P), ("dweight_fp32_add", _I), ("scale", _P), ("status", _P)]
 
 
@@ -83,76 +85,94 @@ def _rows(t):
     return t, ld
 
 
-def _piece_columns(T, V):
-    cols = max(256, PIECE_BYTES // (2 * T) // 256 * 256)
-    return min(cols, (V + 255) // 256 * 256)
+@functools.lru_cache(maxsize=64)
+def _plan(T, H, V, piece_bytes, slab_bytes):
+    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits or 0).
+
+    The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
+    four times are never better.  Logits are kept where they take, in fp32, at most an eighth of the weight's bytes."""
+    cols = min(max(256, piece_bytes // (2 * T) // 256 * 256), (V + 255) // 256 * 256)
+    tiles = -(-H // 256)
+    splits = max(1, min(64, -(-296 // tiles), slab_bytes // ((T + 31) // 32 * 32 * H * 4)))
+    return cols, splits, (T + 7) // 8 * 8 if 16 * T <= H else 0
 
 
-def _splits(T, H, V, piece):
-    """K splits of the hidden gradient.  Its tiles (256 rows x 256 of H) are few where there are few rows, and the 74 SM pairs would wait
-    for as many tiles; split along the vocabulary each pair takes a part of it, at the price of writing and adding ``s`` results.  Times
-    in us: a block of 64 words takes a tile 0.37, its read-out 2; the slabs move at 6 TB/s."""
-    if piece < V:
-        return 1
-    tiles, blocks = -(-T // 256) * -(-H // 256), -(-V // 64)
-    best, best_t = 1, None
-    for s in range(1, min(64, blocks) + 1):
-        t = -(-tiles * s // 74) * (-(-blocks // s) * 0.37 + 2.0) + s * T * H * 8 / 6e6
-        if best_t is None or t < best_t * 0.98:
-            best, best_t = s, t
-    return best
+def _lib():
+    L = loader.require_lib()
+    if L.msb_lce_forward.argtypes is None:
+        L.msb_lce_backward.argtypes = [ctypes.POINTER(_Args), _P]
+        L.msb_lce_rescale.argtypes = [_P, _P, _P, _F, _P, _I, _P]
+        L.msb_lce_loss.argtypes = [_P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P]
+        L.msb_lce_forward.argtypes = [ctypes.POINTER(_Args), _P]
+    return L
+
+
+def _point_at_kept(a, kept, T, H, V, K, ldt):
+    """Places of what both directions use in the one buffer that is kept between them (4-byte words)."""
+    at = kept.data_ptr()
+    a.packed = at
+    at += 2 * T * H
+    if ldt:
+        a.zt, a.ldt = at, ldt
+        at += 4 * V * ldt
+    a.z, a.q, a.lse = at, at + 4 * T * K, at + 8 * T * K
+    at += 8 * T * K + 4 * T
+    a.pos, a.rowmap, a.count = at, at + 4 * T, at + 8 * T
 
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, idx, teacher, tau, ignore_index, group, main_grad):
-        L = loader.require_lib()
+    def forward(ctx, hidden, weight, idx, teacher, tau, ignore_index, group, main_grad, train):
+        L = _lib()
         dev = hidden.device
         lead = hidden.shape[:-1]
-        h, ldh = _rows(hidden.reshape(-1, hidden.shape[-1]))
+        h, ldh = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
         w, ldw = _rows(weight)
         (T, H), V = h.shape, w.shape[0]
         K = 1 if teacher is None else idx.shape[-1]
-        world = 1 if group is None else dist.get_world_size(group)
-        rank = 0 if group is None else dist.get_rank(group)
+        world, rank = (1, 0) if group is None else (dist.get_world_size(group), dist.get_rank(group))
+        plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES)
+        piece, splits, ldt = plan
+        if not train:
+            ldt = 0
         with _on_device(dev):
-            f32 = dict(dtype=torch.float32, device=dev)
-            ints = torch.empty(2 * T + 1, dtype=torch.int32, device=dev)          # pos, rowmap, count
-            kept = torch.empty(2 * T * K + T, **f32)                              # z, q, lse: for the backward
-            packed = torch.empty(T, H, dtype=h.dtype, device=dev)
-            tiles = (V + 255) // 256
-            scratch = torch.empty(4 * T + 2 * tiles * T + (T if teacher is not None else 0), **f32)
-            loss = torch.empty(T, **f32)
-            ip, kp, sp = ints.data_ptr(), kept.data_ptr(), scratch.data_ptr()
+            kept = torch.empty(T * H // 2 + V * ldt + 2 * T * K + 3 * T + 2, dtype=torch.float32, device=dev)
+            parts = (V + 255) // 256 * 2
+            scratch = torch.empty(2 * parts * T + 4 * T + (parts * T + T + 3) // 4, dtype=torch.float32, device=dev)
+            loss = torch.empty(lead, dtype=torch.float32, device=dev)
+            sp = scratch.data_ptr()
+            after = sp + 8 * parts * T
             a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
                       ldh=ldh, ldw=ldw, vocab_start=rank * V, vocab=world * V, ignore_index=ignore_index, T=T, H=H, V=V, K=K,
-                      dtype=code(h.dtype), tau=tau, pos=ip, rowmap=ip + 4 * T, count=ip + 8 * T, packed=packed.data_ptr(), z=kp,
-                      q=kp + 4 * T * K, lse=kp + 8 * T * K, loss=loss.data_ptr(), part=sp, dot=sp + 8 * tiles * T,
-                      ent=sp + 8 * tiles * T + 4 * T, kind=sp + 8 * tiles * T + 16 * T, status=_status(dev).data_ptr())
-            st = ctypes.c_void_p(loader.stream_ptr())
+                      dtype=code(h.dtype), tau=tau, loss=loss.data_ptr(), part=sp, dot=after, ent=after + 4 * T,
+                      part_at=after + 16 * T, kind=after + 16 * T + parts * T, piece=piece, splits=splits, status=_status(dev).data_ptr())
+            _point_at_kept(a, kept, T, H, V, K, ldt)
+            st = loader.stream_ptr()
             if world > 1:
-                at = 2 * tiles * T
+                at = 2 * parts * T
                 dot, ent, mx, sm = (scratch[at + i * T:at + (i + 1) * T] for i in range(4))
                 a.mx, a.sum = mx.data_ptr(), sm.data_ptr()
-            loader.check(L.msb_lce_forward(ctypes.byref(a), st), "linear_ce_forward")
+            loader.check(L.msb_lce_forward(a, st), "linear_ce_forward")
             if world > 1:
                 gmx = mx.clone()
                 dist.all_reduce(gmx, op=dist.ReduceOp.MAX, group=group)
-                loader.check(L.msb_lce_rescale(loader.p(sm), loader.p(mx), loader.p(gmx), _F(tau), _P(a.count), T, st), "linear_ce_rescale")
+                loader.check(L.msb_lce_rescale(sm.data_ptr(), mx.data_ptr(), gmx.data_ptr(), tau, a.count, T, st), "linear_ce_rescale")
                 dist.all_reduce(sm, group=group)
                 dist.all_reduce(dot, group=group)
-                loader.check(L.msb_lce_loss(loader.p(gmx), loader.p(sm), loader.p(dot), loader.p(ent), _P(a.rowmap), _P(a.count), _F(tau), T,
-                                            _P(a.lse), loader.p(loss), st), "linear_ce_loss")
-        ctx.save_for_backward(h, w, idx, teacher, ints, kept, packed)
-        ctx.meta = (tau, rank, hidden.shape, weight if main_grad else None)
-        return loss.reshape(lead)
+                loader.check(L.msb_lce_loss(gmx.data_ptr(), sm.data_ptr(), dot.data_ptr(), ent.data_ptr(), a.rowmap, a.count, tau, T, a.lse,
+                                            loss.data_ptr(), st), "linear_ce_loss")
+        if train:
+            ctx.save_for_backward(h, w, idx, teacher, kept)
+            ctx.meta = (tau, rank, hidden.shape, plan, weight if main_grad else None)
+        return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        L = loader.require_lib()
-        h, w, idx, teacher, ints, kept, packed = ctx.saved_tensors
-        tau, rank, shape, param = ctx.meta
+        if torch.is_grad_enabled():
+            raise RuntimeError("linear loss operators have no second derivative (create_graph)")
+        L = _lib()
+        h, w, idx, teacher, kept = ctx.saved_tensors
+        tau, rank, shape, (piece, splits, ldt), param = ctx.meta
         need_h, need_w = ctx.needs_input_grad[:2]
         dev = h.device
         h, ldh = _rows(h)
@@ -160,39 +180,37 @@ class _LinearLoss(torch.autograd.Function):
         (T, H), V = h.shape, w.shape[0]
         K = 1 if teacher is None else idx.shape[-1]
         with _on_device(dev):
-            g = g.float()
             one = all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape))      # an expanded scalar, as a sum's backward gives
-            g = g if one else g.reshape(-1).contiguous()
-            piece = _piece_columns(T, V)
-            ldz = min(piece, (V + 7) // 8 * 8)
-            dz = torch.empty(T, ldz, dtype=h.dtype, device=dev)
-            ip, kp = ints.data_ptr(), kept.data_ptr()
+            if not one and not g.is_contiguous():
+                g = g.contiguous()
+            ldz = 0 if ldt else min(piece, (V + 7) // 8 * 8)
+            slab_rows = (T + 31) // 32 * 32
+            dz_words = (V * ldt if ldt else T * ldz) // 2
+            scratch = torch.empty(dz_words + (splits * slab_rows * H if need_h else 0) + 2, dtype=torch.float32, device=dev)
+            sp = scratch.data_ptr()
             a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
-                      ldh=ldh, ldw=ldw, vocab_start=rank * V, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=tau, pos=ip, rowmap=ip + 4 * T,
-                      count=ip + 8 * T, packed=packed.data_ptr(), z=kp, q=kp + 4 * T * K, lse=kp + 8 * T * K, g=g.data_ptr(),
-                      g_stride=0 if one else 1, dz=dz.data_ptr(), ldz=ldz, piece=piece, status=_status(dev).data_ptr())
-            dh = dw = scale = acc = None
+                      ldh=ldh, ldw=ldw, vocab_start=rank * V, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=tau, g=g.data_ptr(),
+                      g_stride=0 if one else 1, dz=sp, ldz=ldz, piece=piece, splits=splits, slab_rows=slab_rows, status=_status(dev).data_ptr())
+            _point_at_kept(a, kept, T, H, V, K, ldt)
+            dh = dw = None
             if h.dtype == torch.float16:
-                scale = torch.empty(2, dtype=torch.float32, device=dev)
-                a.scale = scale.data_ptr()
+                a.scale = sp + 4 * (scratch.numel() - 2)
             if need_h:
                 dh = torch.empty(shape, dtype=h.dtype, device=dev)
-                a.splits, a.slab_rows = _splits(T, H, V, piece), (T + 31) // 32 * 32
-                acc = torch.empty(a.splits * a.slab_rows, H, dtype=torch.float32, device=dev)
-                a.acc, a.dhidden = acc.data_ptr(), dh.data_ptr()
+                a.acc, a.dhidden = sp + 4 * dz_words, dh.data_ptr()
             if need_w:
                 if param is not None:
                     a.dweight, a.dweight_fp32_add = param.main_grad.data_ptr(), 1
                 else:
                     dw = torch.empty(V, H, dtype=h.dtype, device=dev)
                     a.dweight = dw.data_ptr()
-            loader.check(L.msb_lce_backward(ctypes.byref(a), ctypes.c_void_p(loader.stream_ptr())), "linear_ce_backward")
+            loader.check(L.msb_lce_backward(a, loader.stream_ptr()), "linear_ce_backward")
         if need_w and param is not None:
             param.grad_added_to_main_grad = True
             cb = getattr(param, "_main_grad_ready_cb", None)
             if cb is not None:
                 cb(param)
-        return dh, dw, None, None, None, None, None, None
+        return dh, dw, None, None, None, None, None, None, None
 
 
 class _SumOverGroup(torch.autograd.Function):
@@ -263,6 +281,10 @@ def _none(hidden, weight):
     return hidden.float().sum(-1) + weight[:0].float().sum()
 
 
+def _train(hidden, weight):
+    return torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+
+
 def _main_grad_hook(weight):
     """The eager form's weight for ``accumulate_main_grad``: its gradient goes to main_grad instead of autograd."""
     w = weight.detach().requires_grad_(weight.requires_grad)
@@ -287,7 +309,7 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, 
         return _none(hidden, weight)
     idx = labels.reshape(-1).long().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, idx, None, 1.0, int(ignore_index), group, bool(accumulate_main_grad))
+        return _LinearLoss.apply(hidden, weight, idx, None, 1.0, int(ignore_index), group, bool(accumulate_main_grad), _train(hidden, weight))
     world = 1 if group is None else dist.get_world_size(group)
     kept = idx != ignore_index
     if bool(((idx < 0) | (idx >= world * weight.shape[0]))[kept].any()):
@@ -319,7 +341,7 @@ def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, te
     idx = teacher_indices.reshape(-1, K).long().contiguous()
     a = teacher_logits.detach().reshape(-1, K).float().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, idx, a, tau, 0, group, bool(accumulate_main_grad))
+        return _LinearLoss.apply(hidden, weight, idx, a, tau, 0, group, bool(accumulate_main_grad), _train(hidden, weight))
     world = 1 if group is None else dist.get_world_size(group)
     if bool((idx >= world * weight.shape[0]).any()):
         raise IndexError(f"{name}: a teacher index outside the vocabulary")

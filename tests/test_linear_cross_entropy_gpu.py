@@ -95,7 +95,8 @@ def _compare(got, h, w, target, tau, g):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("T,V,H", [(1, 1, 8), (1, 257, 64), (2, 256, 72), (31, 255, 136), (64, 1000, 128), (65, 4099, 64), (257, 513, 512),
-                                   (300, 7, 264), (513, 2050, 200), (3, 20011, 256)])
+                                   (300, 7, 264), (513, 2050, 200), (3, 20011, 256), (16, 1300, 256), (130, 700, 2080),
+                                   (2100, 300, 64)])
 @pytest.mark.parametrize("ignored", ["none", "some", "most", "all"])
 def test_cross_entropy(T, V, H, dtype, ignored):
     h, w, fav, g, gen = _inputs(T, V, H, dtype)
@@ -107,7 +108,8 @@ def test_cross_entropy(T, V, H, dtype, ignored):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("T,V,H,K,tau", [(1, 5, 8, 1, 1.0), (3, 1000, 64, 8, 2.0), (130, 4099, 136, 33, 4.0), (257, 513, 256, 64, 0.5),
-                                         (40, 3000, 128, 200, 1.0), (9, 2500, 64, 1024, 2.0)])
+                                         (40, 3000, 128, 200, 1.0), (9, 2500, 64, 1024, 2.0), (13, 1111, 264, 12, 2.0),
+                                           (2050, 260, 64, 3, 1.0)])
 def test_distillation(T, V, H, K, tau, dtype):
     h, w, fav, g, gen = _inputs(T, V, H, dtype)
     idx = torch.randint(0, V, (T, K), generator=gen, device="cuda")          # words come up more than once
@@ -130,7 +132,7 @@ def test_pieces_and_splits(dtype, monkeypatch):
     h, w, fav, g, gen = _inputs(T, V, H, dtype)
     idx = torch.randint(0, V, (T, 5), generator=gen, device="cuda")
     a = torch.randn(T, 5, generator=gen, device="cuda")
-    assert M._splits(T, H, V, M._piece_columns(T, V)) > 1
+    assert M._plan(T, H, V, M.PIECE_BYTES, M.SLAB_BYTES)[1] > 1
     for size in (M.PIECE_BYTES, 2 * T * 256, 2 * T * 1100):
         monkeypatch.setattr(M, "PIECE_BYTES", size)
         _compare(_ce(h, w, fav, g), h, w, _ce_target(fav), 1.0, g)
