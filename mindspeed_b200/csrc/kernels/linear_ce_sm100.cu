@@ -9,16 +9,19 @@
 // Rows without a listed word (ignored labels) leave the products: a scan numbers the rows that stay, and every product runs over their
 // count, which only the device knows.  When all rows stay, the products read the caller's hidden states directly, else a packed copy.
 //
-// Forward:  scan (part of the rows kernel for short inputs) -> rows (packed copy, the K listed logits as dot products, q) -> GEMM whose
-//           epilogue keeps (max, where, sum of exponentials) per row and 128 columns -> join, which computes the largest logit again as a
-//           dot product: the tensor cores cut sums off, 4e-6 of a logit over 5120 products, and the largest one is what the loss follows.
+// Forward:  scan (part of the rows kernel for short inputs) -> rows (packed copy) -> GEMM whose epilogue keeps (max, where, sum of
+//           exponentials) per row and 128 columns, while four warps a CTA make the K listed logits as dot products -> join.
+//           The tensor cores cut every addition to their fp32 sums off: a logit comes out 0.26 (H / 16) 2^-24 of itself too small (0.258
+//           to 0.273 measured at H 1024 to 5120; half a unit in the last place for each of the H / 16 additions, of a sum that grows).
+//           The scale 1 / tau of such logits makes that good, and the join computes the largest logit of a row again as a dot product.
 // Backward: per piece of the vocabulary: the GEMM again, its epilogue now writing the 16-bit dz of the piece (with the label's -1; a
 //           list's q are subtracted by a kernel of its own) -> d hidden += dz W -> dW rows of the piece = dz^T hidden.  dz is rounded to
 //           the 16-bit type of the operands (the tensor cores take nothing wider next to them): half a step on each term, as much as the
 //           rounding of the result itself.  With fp16, dz is scaled by a power of two that puts the largest |g| at 2^14 or above, so that
 //           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
-// Few rows: where the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them (transposed, [V, rows]: rows are
+// Few rows: where there are at most 64 or the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them (transposed, [V, rows]: rows are
 //           the lanes of the epilogue), and an elementwise pass makes dz of them: one reading of W less, a quarter of all traffic.
+//           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
 #include "msb_common.cuh"
@@ -38,7 +41,8 @@ constexpr int GROUP_M = 16;      // tile rows that share W panels in L2: forward
 constexpr float LOG2E = 1.4426950408889634f;
 
 constexpr int EPI_WARPS = 8;       // two a quarter of the 128 accumulator lanes, each half of the columns
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int GATHER_WARPS = 4;    // of the forward: listed logits
+constexpr int TWO_ROWS = 64;       // up to so many rows dz has a second term (one block of K, half of a tile's rows)
 
 enum Epi : int { EPI_STATS = 0, EPI_DLOGITS = 1, EPI_OUT16 = 2, EPI_OUT32 = 3 };
 
@@ -50,6 +54,7 @@ struct LceGemm {
   int all_rows;                // rows there are: the packed copy is unused when *rows equals it
   int group_m;
   int rows_on_k;               // the rows are summed over (weight gradient), else they are output rows
+  int two;                     // dz in two terms, TWO_ROWS rows each: 2 TWO_ROWS rows whatever *rows says
   int split;                   // take rows[1] K splits, their fp32 results in slabs of slab_rows rows
   int slab_rows;
   int accumulate;              // OUT32: add to what is there
@@ -57,6 +62,14 @@ struct LceGemm {
   float2* part;                // STATS: [128 columns][part_ld] (max, sum)
   unsigned char* part_at;      // STATS: column of the max
   long long part_ld;
+  const long long* idx;        // STATS: listed words [T, list], their logits go to listed [rows, list]
+  const float* teacher;
+  float* listed;
+  int list;
+  const void* hidden;
+  const void* weight;
+  long long ldh, ldw, vocab_start, vocab;
+  int width, words;            // H, words of this rank
   float* zt;                   // STATS: keep the logits, [N][ldt], or null
   int ldt;
   const float* lse;            // DLOGITS: per packed row, in units of z / tau
@@ -64,7 +77,7 @@ struct LceGemm {
   const float* g;              // DLOGITS: gradient of the token's loss
   int g_stride;
   float g_factor;              // DLOGITS: tau
-  float inv_tau;
+  float inv_tau, tc_inv_tau;   // 1 / tau for exact logits and for those of the tensor cores
   const long long* label;      // DLOGITS: the token's word (cross entropy), or null
   const float* z;              // DLOGITS: its logit, per packed row
   long long piece_start;       // DLOGITS: word of column 0
@@ -74,10 +87,11 @@ struct LceGemm {
 
 template <int EPI>
 struct Cfg {
-  static constexpr int NSTAGE = EPI == EPI_STATS ? 7 : EPI == EPI_OUT32 ? 5 : 6;   // what the staging leaves of 227 KB
+  static constexpr int THREADS = 64 + 32 * (EPI_WARPS + (EPI == EPI_STATS ? GATHER_WARPS : 0));
+  static constexpr int NSTAGE = EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5;   // what the staging leaves of 227 KB
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + (BN / 2) * BK * 2;
-  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_OUT32 ? 8192 : 4096;   // 32 rows x 64 columns of the output type
+  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
   static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
@@ -123,10 +137,35 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, int half) {
   return pack_bf16(lo, hi);
 }
 
+// What a token's list says: 0 nothing (no listed word: the token is ignored), 1 at least one word, 2 a word outside the vocabulary.
+// Cross entropy: the label.  Distillation: negative indices and teacher logits of -inf are unused places.
+__device__ __forceinline__ int label_kind(long long y, long long vocab, long long ignore_index) {
+  return y == ignore_index ? 0 : (y >= 0 && y < vocab) ? 1 : 2;
+}
+__device__ __forceinline__ bool place_used(long long i, float a, long long vocab) { return i >= 0 && i < vocab && !(a == -INFINITY); }
+
+// Dot product of two rows of H 16-bit values by one warp (H a multiple of 8, rows 16-byte aligned): fp32 sums, same value in all lanes.
+template <typename T>
+__device__ __forceinline__ float warp_dot(const T* __restrict__ a, const T* __restrict__ b, int H, int lane) {
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+  for (int c = lane * 8; c < H; c += 256) {
+    Vec8<T> x, y;
+    x.load(a + c);
+    y.load(b + c);
+    float fx[8], fy[8];
+    x.to_float(fx);
+    y.to_float(fy);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) { s0 = fmaf(fx[j], fy[j], s0); s1 = fmaf(fx[j + 1], fy[j + 1], s1); }
+  }
+  return warp_sum(s0 + s1);
+}
+
 // EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K].      Hidden gradient: A = dz [M, K], B = W [K, N].
 // Weight gradient: A = dz [K, M], B = hidden [K, N], rows on K.  A_MN tells how dz lies in memory ([tokens, words] or transposed).
 template <int EPI, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   using L = Cfg<EPI>;
   constexpr int NSTAGE = L::NSTAGE;
   extern __shared__ uint8_t smem_raw[];
@@ -143,7 +182,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
   const uint32_t cta = cluster_ctarank();                 // 0 = leader
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int rows = p.rows[0], splits = p.split ? p.rows[1] : 1;
-  const int M = p.rows_on_k ? p.M : rows, K = p.rows_on_k ? rows : p.K;
+  const int padded = p.two && rows > 0 ? 2 * TWO_ROWS : rows;
+  const int M = p.rows_on_k ? p.M : padded, K = p.rows_on_k ? padded : p.K;
   const bool packed = rows != p.all_rows;
   constexpr uint32_t TMEM_COLS = 512u;                    // two accumulators of 256 columns
 
@@ -191,7 +231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
           } else {
 #pragma unroll
             for (int j = 0; j < BN / 128; ++j)                                         // boxes [64 k x 64 n]
-              tma_load_2d_pair(sb + j * (BK * 128), mapB, lead_full, n0 + j * 64, k0);
+              tma_load_2d_pair(sb + j * (BK * 128), mapB, lead_full, n0 + j * 64, p.rows_on_k && p.two ? 0 : k0);   // both terms times the same rows
           }
           if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
         }
@@ -235,13 +275,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
     }
+  } else if (EPI == EPI_STATS && warp >= 2 + EPI_WARPS) {
+    // ===================== listed logits (warps 10..13): a dot product each, up to eight neighbours at a time =====================
+    const long long total = (long long)rows * p.list, workers = (long long)gridDim.x * GATHER_WARPS;
+    const long long each = max(1ll, min(8ll, (total + workers - 1) / workers));
+    for (long long f0 = ((long long)blockIdx.x * GATHER_WARPS + warp - 2 - EPI_WARPS) * each; f0 < total; f0 += workers * each)
+      for (long long f = f0; f < min(total, f0 + each); ++f) {
+        const int i = (int)(f / p.list), k = (int)(f - (long long)i * p.list), t = p.rowmap[i];
+        const long long word = p.idx[(long long)t * p.list + k], v = word - p.vocab_start;
+        const bool here = v >= 0 && v < p.words && (!p.teacher || place_used(word, p.teacher[(long long)t * p.list + k], p.vocab));
+        float d = 0.f;
+        if (here)
+          d = p.half ? warp_dot((const __half*)p.hidden + t * p.ldh, (const __half*)p.weight + v * p.ldw, p.width, lane)
+                     : warp_dot((const __nv_bfloat16*)p.hidden + t * p.ldh, (const __nv_bfloat16*)p.weight + v * p.ldw, p.width, lane);
+        if (lane == 0) p.listed[f] = d;
+      }
   } else {
     // ===================== epilogue (warps 2..9, both CTAs) =====================
     const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which 128 columns it takes
-    const uint32_t buf = smem_base + L::EPI_OFFSET + (uint32_t)(warp - 2) * L::EPI_BUF;
+    const uint32_t buf_base = smem_base + L::EPI_OFFSET + (uint32_t)(warp - 2) * L::EPI_BUF;
     const uint32_t lead_tempty[2] = {mapa_u32(tempty_bar(0), 0), mapa_u32(tempty_bar(1), 0)};
     const float unscale = (EPI >= EPI_OUT16 && p.scale) ? p.scale[1] : 1.f;
-    const float ctau = p.inv_tau * LOG2E;
+    const float ctau = p.tc_inv_tau * LOG2E;
+    uint32_t chunk = 0;
     int acc = 0; uint32_t acc_phase = 0;
     Work w(M, p.N, K, p.group_m, splits, pair, npairs);
     while (alive && w.next()) {
@@ -323,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
             // a row with no gradient writes zeros even where its logits are not finite
 #pragma unroll
             for (int j = 0; j < 64; ++j) {
-              const float e = ex2(fmaf(__uint_as_float(rr[j]), p.inv_tau, -lse) * LOG2E) * coef;
+              const float e = ex2(fmaf(__uint_as_float(rr[j]), p.tc_inv_tau, -lse) * LOG2E) * coef;
               rr[j] = __float_as_uint(coef == 0.f ? 0.f : e);
             }
             const long long j0 = label - col0;
@@ -335,7 +391,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
 #pragma unroll
             for (int j = 0; j < 64; ++j) rr[j] = empty ? 0u : __float_as_uint(__uint_as_float(rr[j]) * unscale);
           }
-          if (lane == 0) tma_store_wait_read<0>();      // the last store of this warp has read its buffer
+          const uint32_t buf = buf_base + (EPI == EPI_OUT16 ? (chunk++ & 1u) * 4096u : 0u);
+          if (lane == 0) tma_store_wait_read<EPI == EPI_OUT16 ? 1 : 0>();   // the store that last read this buffer is done with it
           __syncwarp();
           const uint32_t row_addr = buf + (uint32_t)lane * 128u;
           if (EPI != EPI_OUT32) {
@@ -360,9 +417,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
           fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
           __syncwarp();
           if (lane == 0) {
-            // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box
+            // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box; rows past the last are never read
             const int y = p.split ? w.split * p.slab_rows + row0 : row0;
-            if (row0 < (p.split ? p.slab_rows : p.M)) {
+            if (p.split ? (p.two ? row0 < p.slab_rows && (row0 & (TWO_ROWS - 1)) < rows : row0 < rows) : row0 < p.M) {
               if (EPI != EPI_OUT32) {
                 tma_store_2d(&p.tmD, buf, col0, y);
               } else if (!p.accumulate) {
@@ -398,13 +455,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lce_gemm
 // ---------------------------------------------------------------------------------------------------------
 // rows
 // ---------------------------------------------------------------------------------------------------------
-// What a token's list says: 0 nothing (no listed word: the token is ignored), 1 at least one word, 2 a word outside the vocabulary.
-// Cross entropy: the label.  Distillation: negative indices and teacher logits of -inf are unused places.
-__device__ __forceinline__ int label_kind(long long y, long long vocab, long long ignore_index) {
-  return y == ignore_index ? 0 : (y >= 0 && y < vocab) ? 1 : 2;
-}
-__device__ __forceinline__ bool place_used(long long i, float a, long long vocab) { return i >= 0 && i < vocab && !(a == -INFINITY); }
-
 __device__ __forceinline__ int list_kind(const long long* idx, const float* teacher, int K, long long vocab, long long ignore_index) {
   if (!teacher) return label_kind(*idx, vocab, ignore_index);
   bool used = false, bad = false;
@@ -504,44 +554,19 @@ __global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restr
   }
 }
 
-// Dot product of two rows of H 16-bit values by one warp (H a multiple of 8, rows 16-byte aligned): fp32 sums, same value in all lanes.
-template <typename T>
-__device__ __forceinline__ float warp_dot(const T* __restrict__ a, const T* __restrict__ b, int H, int lane) {
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll 4
-  for (int c = lane * 8; c < H; c += 256) {
-    Vec8<T> x, y;
-    x.load(a + c);
-    y.load(b + c);
-    float fx[8], fy[8];
-    x.to_float(fx);
-    y.to_float(fy);
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) { s0 = fmaf(fx[j], fy[j], s0); s1 = fmaf(fx[j + 1], fy[j + 1], s1); }
-  }
-  return warp_sum(s0 + s1);
-}
-
-// Per token: the packed copy of its hidden state (when rows left), the listed logits z (raw; 0 where the word is another rank's), their
-// weights q, and  dot = sum q z / tau,  ent = sum q log q.  Tokens that left get loss 0 (NaN where a word is outside the vocabulary).
-// WPT warps a token: one for a single listed word, eight for lists.  Blocks past the tokens zero the packed rows up to the next
-// multiple of 64: the weight gradient reads whole blocks of 64 rows.
+// The packed copy of the hidden states (when rows left), a warp a token.  Tokens that left get loss 0 (NaN where a word is outside the
+// vocabulary).  Blocks past the tokens zero the packed rows up to the next multiple of 64: the weight gradient reads whole blocks of 64.
 // SCAN (up to SCAN_MOST tokens with short lists): every block numbers the rows itself, which saves the launches of the scan; the first
 // block writes the numbers out.
 constexpr int SCAN_MOST = 2048, SCAN_LIST = 16;
-template <typename T, int WPT, bool SCAN>
-__global__ void __launch_bounds__(256) lce_rows_kernel(const T* __restrict__ hidden, long long ldh, const T* __restrict__ weight, long long ldw,
-                                                       const long long* __restrict__ idx, const float* __restrict__ teacher, int Tn, int H,
-                                                       int K, int vocab_local, long long vocab_start, long long vocab, long long ignore_index,
-                                                       float inv_tau, Splits sp, int* __restrict__ pos, int* __restrict__ rowmap,
-                                                       int* __restrict__ count, unsigned int* error, T* __restrict__ packed,
-                                                       float* __restrict__ z, float* __restrict__ qout, float* __restrict__ dot,
-                                                       float* __restrict__ ent, float* __restrict__ loss) {
-  constexpr int PER_BLOCK = 8 / WPT;
-  extern __shared__ float zs[];            // WPT = 8: the token's K logits
+template <bool SCAN>
+__global__ void __launch_bounds__(256) lce_rows_kernel(const uint4* __restrict__ hidden, long long ldh, const long long* __restrict__ idx,
+                                                       const float* __restrict__ teacher, int Tn, int H, int K, long long vocab,
+                                                       long long ignore_index, Splits sp, int* __restrict__ pos, int* __restrict__ rowmap,
+                                                       int* __restrict__ count, unsigned int* error, uint4* __restrict__ packed,
+                                                       float* __restrict__ loss) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int token_blocks = (Tn + PER_BLOCK - 1) / PER_BLOCK;
-  const int t = (int)blockIdx.x * PER_BLOCK + (WPT == 1 ? warp : 0);
+  const int token_blocks = (Tn + 7) / 8, t = (int)blockIdx.x * 8 + warp, vecs = H / 8;
   int n, at = -1;
   if (SCAN) {
     __shared__ unsigned int keep[SCAN_MOST / 32], wrong[SCAN_MOST / 32];
@@ -590,62 +615,20 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const T* __restrict__ hid
     if (t < Tn) at = pos[t];
   }
   if ((int)blockIdx.x >= token_blocks) {
-    const int r = n + ((int)blockIdx.x - token_blocks);
+    const int r = n + ((int)blockIdx.x - token_blocks) * 8 + warp;
     if (n == Tn || r >= min(Tn, (n + 63) / 64 * 64)) return;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int c = threadIdx.x * 8; c < H; c += 2048) *reinterpret_cast<uint4*>(packed + (long long)r * H + c) = zero;
+    for (int c = lane; c < vecs; c += 32) packed[(long long)r * vecs + c] = make_uint4(0, 0, 0, 0);
     return;
   }
   if (t >= Tn) return;
   if (at < 0) {
-    if (lane == 0 && (WPT == 1 || warp == 0)) loss[t] = at == -2 ? NAN : 0.f;
+    if (lane == 0) loss[t] = at == -2 ? NAN : 0.f;
     return;
   }
-  const T* h = hidden + (long long)t * ldh;
-  if (n != Tn) {
-    const int step = WPT == 1 ? 256 : 2048;
-    for (int c = (WPT == 1 ? lane : (int)threadIdx.x) * 8; c < H; c += step)
-      *reinterpret_cast<uint4*>(packed + (long long)at * H + c) = *reinterpret_cast<const uint4*>(h + c);
-  }
-  if (WPT == 1) {
-    const long long v = idx[t] - vocab_start;
-    const bool here = v >= 0 && v < vocab_local;
-    const float d = here ? warp_dot(h, weight + v * ldw, H, lane) : 0.f;
-    if (lane == 0) { z[at] = d; qout[at] = 1.f; dot[at] = d * inv_tau; ent[at] = 0.f; }
-    return;
-  }
-  const long long first = (long long)t * K;
-  for (int k = warp; k < K; k += 8) {
-    const long long v = idx[first + k] - vocab_start;
-    const bool here = v >= 0 && v < vocab_local && place_used(idx[first + k], teacher[first + k], vocab);
-    const float d = here ? warp_dot(h, weight + v * ldw, H, lane) : 0.f;
-    if (lane == 0) { zs[k] = d; z[(long long)at * K + k] = d; }
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  float mx = -INFINITY;
-  for (int k = lane; k < K; k += 32)
-    if (place_used(idx[first + k], teacher[first + k], vocab)) mx = fmaxf(mx, teacher[first + k]);
-  mx = warp_max(mx);
-  float s = 0.f;
-  for (int k = lane; k < K; k += 32)
-    if (place_used(idx[first + k], teacher[first + k], vocab)) s += ex2((teacher[first + k] - mx) * (inv_tau * LOG2E));
-  s = warp_sum(s);
-  const float ls = (float)log((double)s);
-  float d = 0.f, e = 0.f;
-  for (int k = lane; k < K; k += 32) {
-    float q = 0.f;
-    if (place_used(idx[first + k], teacher[first + k], vocab)) {
-      const float a = (teacher[first + k] - mx) * inv_tau;
-      q = ex2(a * LOG2E) / s;
-      d = fmaf(q, zs[k] * inv_tau, d);
-      if (!(q == 0.f)) e = fmaf(q, a - ls, e);
-    }
-    qout[(long long)at * K + k] = q;
-  }
-  d = warp_sum(d);
-  e = warp_sum(e);
-  if (lane == 0) { dot[at] = d; ent[at] = e; }
+  if (n == Tn) return;
+  const uint4* h = hidden + t * (ldh / 8);
+#pragma unroll 4
+  for (int c = lane; c < vecs; c += 32) packed[(long long)at * vecs + c] = h[c];
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -657,28 +640,31 @@ __device__ __forceinline__ void lce_finish(float m, float s, float dot, float en
   *loss = tau2 * (ent + (m * inv_tau - dot) + ls);       // the two large numbers are subtracted first
 }
 
-// 32 rows a block (coalesced over the rows), 32 threads a row over the 128-column parts; the order of the sums is fixed.  Then one warp a
-// row computes the largest logit again in fp32 and rebases the sum on it: s = 1 + (s - 1) exp((m - m') / tau), m' the new value.
-template <typename T>
-__global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict__ part, const unsigned char* __restrict__ part_at,
+// R rows a block, S threads a row over the 128-column parts (neighbouring threads take neighbouring rows); the order of the sums is fixed.
+// Then one warp a row computes the largest logit again in fp32 and rebases the sum on it: s = 1 + (s - 1) exp((m - m') / tau), m' the new
+// value; for a list it makes the weights q, dot = sum q z / tau and ent = sum q log q.
+// 256 threads and 8 rows keep five blocks on an SM (8192 rows, 128256 words: 52 us with 32 rows a block); few rows take 128 threads each.
+template <typename T, int R, int S>
+__global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* __restrict__ part, const unsigned char* __restrict__ part_at,
                                                         long long part_ld, int parts, const T* __restrict__ hidden, long long ldh,
-                                                        const T* __restrict__ weight, long long ldw, int H, float inv_tau, float tau2,
-                                                        const int* __restrict__ count, const int* __restrict__ rowmap,
-                                                        const float* __restrict__ dot, const float* __restrict__ ent, float* __restrict__ mo,
+                                                        const T* __restrict__ weight, long long ldw, int H, float inv_tau, float tc_inv_tau,
+                                                        float tau2, const int* __restrict__ count, const int* __restrict__ rowmap,
+                                                        const long long* __restrict__ idx, const float* __restrict__ teacher, int K,
+                                                        long long vocab, const float* __restrict__ z, float* __restrict__ qout,
+                                                        float* __restrict__ dot, float* __restrict__ ent, float* __restrict__ mo,
                                                         float* __restrict__ so, float* __restrict__ lse, float* __restrict__ loss) {
-  __shared__ float ms[32][33], ss[32][33];
-  __shared__ int as[32][33];
-  const int r = threadIdx.x & 31, y = threadIdx.x >> 5;
+  __shared__ float ms[S][R + 1], ss[S][R + 1];
+  __shared__ int as[S][R + 1];
   const int n = *count;
-  if ((int)blockIdx.x * 32 >= n) return;
-  const float c = inv_tau * LOG2E;
+  if ((int)blockIdx.x * R >= n) return;
+  const float c = tc_inv_tau * LOG2E;
   {
-    const int row = blockIdx.x * 32 + r;
+    const int r = threadIdx.x % R, y = threadIdx.x / R, row = blockIdx.x * R + r;
     float m = -INFINITY, s = 0.f;
     int at = 0;
     if (row < n) {
 #pragma unroll 4
-      for (int i = y; i < parts; i += 32) {
+      for (int i = y; i < parts; i += S) {
         const float2 v = part[(long long)i * part_ld + row];
         const float mn = fmaxf(m, v.x), base = mn == -INFINITY ? 0.f : mn;
         s = s * ex2((m - base) * c) + v.y * ex2((v.x - base) * c);
@@ -692,24 +678,63 @@ __global__ void __launch_bounds__(1024) lce_join_kernel(const float2* __restrict
     as[y][r] = at;
   }
   __syncthreads();
-  const int row = blockIdx.x * 32 + y, lane = r;
-  if (row >= n) return;
-  const float m = ms[lane][y];
-  const float mm = warp_max(m);
-  const float s = warp_sum(ss[lane][y] * ex2((m - (m == -INFINITY && mm != -INFINITY ? 0.f : mm)) * c));
-  const unsigned int who = __ballot_sync(0xffffffffu, m == mm);
-  const int word = who ? as[__ffs(who) - 1][y] : 0;
+  const int r = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * R + r;
+  if (r >= R || row >= n) return;
+  float mm = -INFINITY;
+  int word = 0;
+#pragma unroll
+  for (int i = lane; i < S; i += 32)
+    if (ms[i][r] > mm) { mm = ms[i][r]; word = as[i][r]; }
+  const float mine = mm;
+  mm = warp_max(mm);
+  const unsigned int who = __ballot_sync(0xffffffffu, mine == mm);
+  word = __shfl_sync(0xffffffffu, word, who ? __ffs(who) - 1 : 0);
+  float s = 0.f;
+#pragma unroll
+  for (int i = lane; i < S; i += 32) s += ss[i][r] * ex2((ms[i][r] - (ms[i][r] == -INFINITY && mm != -INFINITY ? 0.f : mm)) * c);
+  s = warp_sum(s);
   const int t = rowmap[row];
-  const float again = warp_dot(hidden + (long long)t * ldh, weight + (long long)word * ldw, H, lane);
+  const float again = warp_dot(hidden + t * ldh, weight + word * ldw, H, lane);
+  float d, e = 0.f;
+  if (teacher) {
+    const long long* list = idx + (long long)t * K;
+    const float* a = teacher + (long long)t * K;
+    const float* zi = z + (long long)row * K;
+    float mx = -INFINITY, sum = 0.f;
+    for (int k = lane; k < K; k += 32)
+      if (place_used(list[k], a[k], vocab)) mx = fmaxf(mx, a[k]);
+    mx = warp_max(mx);
+    for (int k = lane; k < K; k += 32)
+      if (place_used(list[k], a[k], vocab)) sum += ex2((a[k] - mx) * (inv_tau * LOG2E));
+    sum = warp_sum(sum);
+    const float ls = (float)log((double)sum);
+    d = 0.f;
+    for (int k = lane; k < K; k += 32) {
+      float q = 0.f;
+      if (place_used(list[k], a[k], vocab)) {
+        const float b = (a[k] - mx) * inv_tau;
+        q = ex2(b * LOG2E) / sum;
+        d = fmaf(q, zi[k] * inv_tau, d);
+        if (!(q == 0.f)) e = fmaf(q, b - ls, e);
+      }
+      qout[(long long)row * K + k] = q;
+    }
+    d = warp_sum(d);
+    e = warp_sum(e);
+  } else {
+    d = z[row] * inv_tau;
+  }
   if (lane == 0) {
     const float m2 = mm == -INFINITY ? mm : again;         // nothing but -inf: NaN, as the formula
-    const float s2 = 1.f + (s - 1.f) * ex2((mm - m2) * c);
+    const float s2 = 1.f + (s - 1.f) * ex2(fmaf(mm, tc_inv_tau, -(m2 * inv_tau)) * LOG2E);
     if (mo) {
       mo[row] = m2;
       so[row] = s2;
+      dot[row] = d;
+      ent[row] = e;
     } else {
       float l, o;
-      lce_finish(m2, s2, dot[row], ent[row], inv_tau, tau2, &l, &o);
+      lce_finish(m2, s2, d, e, inv_tau, tau2, &l, &o);
       lse[row] = l;
       loss[t] = o;
     }
@@ -756,7 +781,7 @@ __global__ void __launch_bounds__(1024) lce_scale_kernel(const float* __restrict
 // The listed words' entries of the piece: dz[i, v] = (exp(z / tau - lse) - sum of the q of all places that list v) * coefficient.  Places
 // that list a word twice write the same value.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, long long ld_row, long long ld_word, const long long* __restrict__ idx,
+__global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, long long ld_row, long long ld_word, int two, const long long* __restrict__ idx,
                                                          const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lse,
                                                          const int* __restrict__ rowmap, const int* __restrict__ count, int K,
                                                          long long piece_start, int piece_cols, const float* __restrict__ g, int g_stride,
@@ -779,16 +804,20 @@ __global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, lon
   float coef = g[(long long)t * g_stride] * g_factor;
   if (scale) coef *= scale[0];
   const float p = ex2((z[(long long)i * K + k] * inv_tau - lse[i]) * LOG2E);
-  dz[i * ld_row + v * ld_word] = from_f<T>(coef == 0.f ? 0.f : (p - sum) * coef);
+  const float d = coef == 0.f ? 0.f : (p - sum) * coef;
+  const T hi = from_f<T>(d);
+  dz[i * ld_row + v * ld_word] = hi;
+  if (two) dz[(i + TWO_ROWS) * ld_row + v * ld_word] = from_f<T>(d - to_f(hi));
 }
 
-// dz of kept logits, both [V, ldt] with the rows innermost: eight rows of one word a thread.  Rows past the last are zero.
-template <typename T>
+// dz of kept logits, both [V, ldt] with the rows innermost: eight rows of one word a thread.  Rows past the last are zero.  TWO: dz is
+// [V, 2 ldt], the second half what the rounding of the first left.
+template <typename T, bool TWO>
 __global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int V, const float* __restrict__ lse,
                                                      const long long* __restrict__ label, const float* __restrict__ z,
                                                      const int* __restrict__ rowmap, const int* __restrict__ count, long long vocab_start,
                                                      const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
-                                                     const float* __restrict__ scale) {
+                                                     float tc_inv_tau, const float* __restrict__ scale) {
   const int groups = ldt / 8, n = *count;
   // the block's threads take (256 / groups) words a round, always the same rows
   const int per = max(1, 256 / groups), grp = threadIdx.x % groups, sub = threadIdx.x / groups;
@@ -821,19 +850,30 @@ __global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ z
       x.to_float(f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], inv_tau, -ls[j]) * LOG2E) * coef[j];
+        const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], tc_inv_tau, -ls[j]) * LOG2E) * coef[j];
         f[j] = coef[j] == 0.f ? 0.f : e;
       }
       Vec8<T> w;
       w.from_float(f);
-      w.store(dz + o);
+      if (TWO) {
+        T* at = dz + (long long)v * 2 * ldt + g0 * 8;
+        w.store(at);
+        float hi[8];
+        w.to_float(hi);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] -= hi[j];
+        w.from_float(f);
+        w.store(at + ldt);
+      } else {
+        w.store(dz + o);
+      }
     }
   }
 }
 
 // d hidden: the fp32 slabs of the K splits, added in order, back in the order of the tokens; zero rows for tokens that left.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restrict__ acc, const int* __restrict__ count, long long slab, const int* __restrict__ pos,
+__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restrict__ acc, const int* __restrict__ count, long long slab, int two, const int* __restrict__ pos,
                                                           T* __restrict__ out, int Tn, int H) {
   const int per_row = H / 8, splits = count[1];
   const long long total = (long long)Tn * per_row;
@@ -843,7 +883,7 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restric
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
       const float* a = acc + (long long)at * H + c;
-      for (int s = 0; s < splits; ++s, a += slab) {
+      for (int s = 0; s < splits * (two ? 2 : 1); ++s, a += two ? (s & 1 ? TWO_ROWS * (long long)H : slab - TWO_ROWS * (long long)H) : slab) {
         const float4 u = __ldcs(reinterpret_cast<const float4*>(a)), v = __ldcs(reinterpret_cast<const float4*>(a + 4));
         o[0] += u.x; o[1] += u.y; o[2] += u.z; o[3] += u.w;
         o[4] += v.x; o[5] += v.y; o[6] += v.z; o[7] += v.w;
@@ -866,10 +906,13 @@ int launch_gemm(const LceGemm& p, int most_splits, cudaStream_t s) {
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
   const long long items = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN) * most_splits;
   const int pairs = (int)std::min<long long>(items, msb::num_sms() / 2);
-  kern<<<2 * pairs, THREADS, L::TOTAL, s>>>(p);
+  kern<<<2 * pairs, L::THREADS, L::TOTAL, s>>>(p);
   MSB_CHECK_LAUNCH("lce_gemm");
   return 0;
 }
+
+// 1 / tau for logits that the tensor cores summed over H products (see the top of the file).
+float tc_scale(float inv_tau, int H) { return (float)((double)inv_tau * (1.0 + 0.26 * (H / 16) / 16777216.0)); }
 
 CUtensorMapDataType map_type(int dtype) { return dtype == MSB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
@@ -900,13 +943,13 @@ struct MsbLceArgs {
   float* part;                 // [ceil(V / 256) * 2, T] pairs, scratch
   unsigned char* part_at;      // [ceil(V / 256) * 2, T] scratch
   float* zt;                   // [V, ldt] logits kept for the backward, or null
-  int ldt;                     // T rounded up to a multiple of 8
+  int ldt;                     // T rounded up to a multiple of 8; TWO_ROWS for up to so many tokens
   float* mx;                   // [T], [T]: local statistics for the vocabulary-parallel form, else null
   float* sum;
   // backward
   const float* g;
   long long g_stride;          // 0: one value for all tokens
-  void* dz;                    // [T, piece] scratch, row pitch ldz; with zt [V, ldt]
+  void* dz;                    // [T, piece] scratch, row pitch ldz; with zt [V, ldt], or [V, 2 TWO_ROWS]
   long long ldz;
   int piece;                   // columns of a piece (a multiple of 256)
   float* acc;                  // [splits, slab_rows, H] fp32 scratch, or null: no hidden gradient
@@ -925,7 +968,7 @@ static int lce_check(const MsbLceArgs* a) {
   MSB_REQUIRE(a->status != nullptr, "linear_ce: status words are required");
   MSB_REQUIRE(a->tau > 0.f, "linear_ce: the temperature must be positive");
   MSB_REQUIRE(a->K == 1 || a->teacher, "linear_ce: lists need teacher logits");
-  MSB_REQUIRE(!a->zt || (a->ldt % 8 == 0 && a->ldt >= a->T), "linear_ce: pitch %d of the kept logits", a->ldt);
+  MSB_REQUIRE(!a->zt || (a->ldt % 8 == 0 && a->ldt >= a->T && (a->T > TWO_ROWS || a->ldt == TWO_ROWS)), "linear_ce: pitch %d of the kept logits", a->ldt);
   MSB_REQUIRE(a->piece > 0 && a->piece % BN == 0 && a->splits >= 1, "linear_ce: piece of %d columns, %d splits", a->piece, a->splits);
   return 0;
 }
@@ -946,15 +989,11 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
                                        a->count, a->status + 1);
     MSB_CHECK_LAUNCH("lce_scan");
   }
-  const int per_block = a->teacher ? 1 : 8;
-  const unsigned grid = (unsigned)((a->T + per_block - 1) / per_block + 63);
-#define LCE_ROWS(WPT, SCAN)                                                                                                                  \
-  lce_rows_kernel<DT, WPT, SCAN><<<grid, 256, WPT == 8 ? a->K * 4 : 0, s>>>(hidden, a->ldh, weight, a->ldw, a->idx, a->teacher, a->T, a->H,    \
-                                                                           a->K, a->V, a->vocab_start, a->vocab, a->ignore_index, inv_tau,  \
-                                                                           sp, a->pos, a->rowmap, a->count, a->status + 1, (DT*)a->packed,  \
-                                                                           a->z, a->q, a->dot, a->ent, a->loss)
-  if (a->teacher) { if (scan) LCE_ROWS(8, true); else LCE_ROWS(8, false); }
-  else { if (scan) LCE_ROWS(1, true); else LCE_ROWS(1, false); }
+  const unsigned grid = (unsigned)((a->T + 7) / 8 + 8);
+#define LCE_ROWS(SCAN)                                                                                                                       \
+  lce_rows_kernel<SCAN><<<grid, 256, 0, s>>>((const uint4*)hidden, a->ldh, a->idx, a->teacher, a->T, a->H, a->K, a->vocab, a->ignore_index,   \
+                                             sp, a->pos, a->rowmap, a->count, a->status + 1, (uint4*)a->packed, a->loss)
+  if (scan) LCE_ROWS(true); else LCE_ROWS(false);
 #undef LCE_ROWS
   MSB_CHECK_LAUNCH("lce_rows");
   LceGemm p;
@@ -970,11 +1009,20 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.half = a->dtype == MSB_F16;
   p.part = reinterpret_cast<float2*>(a->part); p.part_at = a->part_at; p.part_ld = a->T;
   p.zt = a->zt; p.ldt = a->ldt;
-  p.inv_tau = inv_tau;
+  p.idx = a->idx; p.teacher = a->teacher; p.listed = a->z; p.list = a->K;
+  p.hidden = hidden; p.weight = weight; p.ldh = a->ldh; p.ldw = a->ldw; p.vocab_start = a->vocab_start; p.vocab = a->vocab;
+  p.width = a->H; p.words = a->V;
+  p.rowmap = a->rowmap;
+  p.inv_tau = inv_tau; p.tc_inv_tau = tc_scale(inv_tau, a->H);
   p.status = a->status;
   if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, s))) return rc;
-  lce_join_kernel<DT><<<(a->T + 31) / 32, 1024, 0, s>>>(p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden, a->ldh, weight, a->ldw, a->H,
-                                                        inv_tau, tau2, a->count, a->rowmap, a->dot, a->ent, a->mx, a->sum, a->lse, a->loss);
+#define LCE_JOIN(R, S)                                                                                                                       \
+  lce_join_kernel<DT, R, S><<<(a->T + R - 1) / R, R * S, 0, s>>>(p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden, a->ldh, weight,     \
+                                                                a->ldw, a->H, inv_tau, p.tc_inv_tau, tau2, a->count, a->rowmap, a->idx,      \
+                                                                a->teacher, a->K, a->vocab, a->z, a->q, a->dot, a->ent, a->mx, a->sum,       \
+                                                                a->lse, a->loss)
+  if (a->T <= 1024) LCE_JOIN(4, 128); else LCE_JOIN(8, 32);
+#undef LCE_JOIN
   MSB_CHECK_LAUNCH("lce_join");
   return 0;
 }
@@ -1015,11 +1063,12 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   p.half = a->dtype == MSB_F16;
   p.rowmap = a->rowmap; p.lse = a->lse;
   p.g = a->g; p.g_stride = (int)a->g_stride; p.g_factor = a->tau;
-  p.inv_tau = inv_tau;
+  p.inv_tau = inv_tau; p.tc_inv_tau = tc_scale(inv_tau, a->H);
   p.label = label; p.z = a->z;
   p.scale = a->scale;
   p.status = a->status;
   const int piece = a->zt ? a->V : a->piece;       // kept logits are few
+  const int two = a->zt && a->T <= TWO_ROWS, dz_rows = two ? 2 * TWO_ROWS : a->T, dz_ld = two ? 2 * TWO_ROWS : a->ldt;
   int rc;
   for (long long v0 = 0; v0 < a->V; v0 += piece) {
     const int cols = (int)std::min<long long>(piece, a->V - v0);
@@ -1028,41 +1077,44 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
     if (a->zt) {
       const int per = std::max(1, 256 / (a->ldt / 8));
       const int grid = (int)std::min<long long>((a->V + per - 1) / per, (long long)msb::num_sms() * 8);
-      lce_dz_kernel<DT><<<grid, 256, 0, s>>>(a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start, a->g,
-                                             (int)a->g_stride, a->tau, inv_tau, a->scale);
+#define LCE_DZ(TWO)                                                                                                                          \
+  lce_dz_kernel<DT, TWO><<<grid, 256, 0, s>>>(a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start, a->g,        \
+                                              (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
+      if (two) LCE_DZ(true); else LCE_DZ(false);
+#undef LCE_DZ
       MSB_CHECK_LAUNCH("lce_dz");
     } else {
       if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BN / 2, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
-      p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.piece_start = a->vocab_start + v0;
+      p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
       if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, s))) return rc;
     }
     if (a->teacher) {
       const long long places = (long long)a->T * a->K;
-      lce_listed_kernel<DT><<<(unsigned)((places + 255) / 256), 256, 0, s>>>(dz, a->zt ? 1 : a->ldz, a->zt ? a->ldt : 1, a->idx, a->z, a->q, a->lse,
+      lce_listed_kernel<DT><<<(unsigned)((places + 255) / 256), 256, 0, s>>>(dz, a->zt ? 1 : a->ldz, a->zt ? dz_ld : 1, two, a->idx, a->z, a->q, a->lse,
                                                                             a->rowmap, a->count, a->K, a->vocab_start + v0, cols, a->g,
                                                                             (int)a->g_stride, a->tau, inv_tau, a->scale);
       MSB_CHECK_LAUNCH("lce_listed");
     }
     if (a->acc) {
-      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, a->T, a->ldt, BK, 64);
+      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BK, 64);
       else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BM, BK);
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
-      p.M = a->T; p.N = a->H; p.K = cols; p.rows_on_k = 0; p.split = 1; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
+      p.M = dz_rows; p.N = a->H; p.K = cols; p.rows_on_k = 0; p.split = 1; p.two = two; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
       rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, s);
       if (rc) return rc;
     }
     if (a->dweight) {
-      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, a->T, a->ldt, BM, BK);
+      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BM, BK);
       else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BK, 64);
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, a->hidden, dt, 2, a->T, a->H, a->ldh, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BK, 64))) return rc;
-      p.M = cols; p.N = a->H; p.K = a->T; p.rows_on_k = 1; p.split = 0;
+      p.M = cols; p.N = a->H; p.K = a->T; p.rows_on_k = 1; p.split = 0; p.two = two;
       if (a->dweight_fp32_add) {
         if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
@@ -1078,7 +1130,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   if (a->acc) {
     const long long vecs = (long long)a->T * (a->H / 8);
     const unsigned grid = (unsigned)std::min<long long>((vecs + 255) / 256, (long long)msb::num_sms() * 16);
-    lce_dhidden_kernel<DT><<<grid, 256, 0, s>>>(a->acc, a->count, (long long)a->slab_rows * a->H, a->pos, (DT*)a->dhidden, a->T, a->H);
+    lce_dhidden_kernel<DT><<<grid, 256, 0, s>>>(a->acc, a->count, (long long)a->slab_rows * a->H, two, a->pos, (DT*)a->dhidden, a->T, a->H);
     MSB_CHECK_LAUNCH("lce_dhidden");
   }
   return 0;
@@ -1088,7 +1140,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
 MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   if (int rc = lce_check(a)) return rc;
   MSB_REQUIRE(a->zt || (a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V)), "linear_ce: pitch %lld of a piece of %d columns", a->ldz, a->piece);
-  MSB_REQUIRE(!a->acc || (a->slab_rows >= a->T && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
+  MSB_REQUIRE(!a->acc || (a->slab_rows >= (a->zt && a->T <= TWO_ROWS ? 2 * TWO_ROWS : a->T) && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
               "linear_ce: %d slabs of %d rows", a->splits, a->slab_rows);
   return a->dtype == MSB_F16 ? lce_backward<__half>(a, s) : lce_backward<__nv_bfloat16>(a, s);
 }

@@ -6,8 +6,8 @@
 
 Both take ``hidden`` [..., H] and ``weight`` [V, H] in bf16 or fp16 (H a multiple of 8) and return the loss in fp32 with the leading shape
 of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token, the backward makes the logits again, a
-piece of the vocabulary at a time.  (For few tokens, at most a sixteenth of H, the fp32 logits take at most an eighth of the weight's bytes;
-then they are kept instead.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
+piece of the vocabulary at a time.  (For few tokens, at most 64 or a sixteenth of H, the fp32 logits are
+kept instead: at most an eighth of the weight's bytes, or 256 bytes a word.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
 teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
 
 A label or teacher index beyond the vocabulary gives its token loss NaN and no gradient, and makes ``ops.gemm.check_status`` raise.
@@ -39,6 +39,8 @@ _P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_flo
 PIECE_BYTES = 512 << 20
 SLAB_BYTES = 256 << 20
 MAX_LIST = 1024
+#: up to so many tokens the logits are kept whatever H is, and their gradients go into the products in two 16-bit terms
+TWO_ROWS = 64
 
 
 class _Args(ctypes.Structure):
@@ -90,11 +92,11 @@ def _plan(T, H, V, piece_bytes, slab_bytes):
     """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits or 0).
 
     The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
-    four times are never better.  Logits are kept where they take, in fp32, at most an eighth of the weight's bytes."""
+    four times are never better.  Logits are kept where they take, in fp32, at most an eighth of the weight's bytes, or 64 rows."""
     cols = min(max(256, piece_bytes // (2 * T) // 256 * 256), (V + 255) // 256 * 256)
     tiles = -(-H // 256)
     splits = max(1, min(64, -(-296 // tiles), slab_bytes // ((T + 31) // 32 * 32 * H * 4)))
-    return cols, splits, (T + 7) // 8 * 8 if 16 * T <= H else 0
+    return cols, splits, TWO_ROWS if T <= TWO_ROWS else (T + 7) // 8 * 8 if 16 * T <= H else 0
 
 
 def _lib():
@@ -184,8 +186,9 @@ class _LinearLoss(torch.autograd.Function):
             if not one and not g.is_contiguous():
                 g = g.contiguous()
             ldz = 0 if ldt else min(piece, (V + 7) // 8 * 8)
-            slab_rows = (T + 31) // 32 * 32
-            dz_words = (V * ldt if ldt else T * ldz) // 2
+            two = ldt and T <= TWO_ROWS
+            slab_rows = 2 * TWO_ROWS if two else (T + 31) // 32 * 32
+            dz_words = (V * (2 if two else 1) * ldt if ldt else T * ldz) // 2
             scratch = torch.empty(dz_words + (splits * slab_rows * H if need_h else 0) + 2, dtype=torch.float32, device=dev)
             sp = scratch.data_ptr()
             a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
