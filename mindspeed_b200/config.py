@@ -58,6 +58,7 @@ class ModelParallelConfig:
     tp_comm_overlap_ag: bool = True
     tp_comm_overlap_rs: bool = True
     cross_entropy_loss_fusion: bool = False
+    linear_cross_entropy_fusion: bool = False
 
     pipeline_dtype: Optional[torch.dtype] = None
     variable_seq_lengths: bool = False
@@ -195,6 +196,7 @@ class TransformerConfig(ModelParallelConfig):
     moe_grouped_gemm: bool = False
     moe_use_legacy_grouped_gemm: bool = False
     moe_aux_loss_coeff: float = 0.0
+    moe_balance_loss_fusion: bool = False
     moe_z_loss_coeff: Optional[float] = None
     moe_input_jitter_eps: Optional[float] = None
     moe_token_dropping: bool = False

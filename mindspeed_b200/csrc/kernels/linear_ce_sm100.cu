@@ -162,6 +162,43 @@ __device__ __forceinline__ float warp_dot(const T* __restrict__ a, const T* __re
   return warp_sum(s0 + s1);
 }
 
+// Logits of row i (token t) for up to four words: their rows of W are in flight together.
+template <typename T>
+__device__ __forceinline__ void dots_of_row(const LceGemm& p, int i, int k0, int t, long long mine, int lane) {
+  const T* h = (const T*)p.hidden + t * p.ldh;
+  const T* w[4];
+  bool here[4];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const long long v = __shfl_sync(0xffffffffu, mine, j);
+    here[j] = v >= 0;
+    w[j] = (const T*)p.weight + (here[j] ? v : 0) * p.ldw;
+  }
+#pragma unroll 2
+  for (int c = lane * 8; c < p.width; c += 256) {
+    Vec8<T> x, y[4];
+    x.load(h + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (here[j]) y[j].load(w[j] + c);
+    float fx[8], fy[8];
+    x.to_float(fx);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (here[j]) {
+        y[j].to_float(fy);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j] = fmaf(fx[e], fy[e], s[j]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    s[j] = warp_sum(s[j]);
+    if (lane == 0 && k0 + j < p.list) p.listed[(long long)i * p.list + k0 + j] = here[j] ? s[j] : 0.f;
+  }
+}
+
 // EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K].      Hidden gradient: A = dz [M, K], B = W [K, N].
 // Weight gradient: A = dz [K, M], B = hidden [K, N], rows on K.  A_MN tells how dz lies in memory ([tokens, words] or transposed).
 template <int EPI, bool A_MN, bool B_MN>
@@ -276,20 +313,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
       }
     }
   } else if (EPI == EPI_STATS && warp >= 2 + EPI_WARPS) {
-    // ===================== listed logits (warps 10..13): a dot product each, up to eight neighbours at a time =====================
-    const long long total = (long long)rows * p.list, workers = (long long)gridDim.x * GATHER_WARPS;
-    const long long each = max(1ll, min(8ll, (total + workers - 1) / workers));
-    for (long long f0 = ((long long)blockIdx.x * GATHER_WARPS + warp - 2 - EPI_WARPS) * each; f0 < total; f0 += workers * each)
-      for (long long f = f0; f < min(total, f0 + each); ++f) {
-        const int i = (int)(f / p.list), k = (int)(f - (long long)i * p.list), t = p.rowmap[i];
-        const long long word = p.idx[(long long)t * p.list + k], v = word - p.vocab_start;
-        const bool here = v >= 0 && v < p.words && (!p.teacher || place_used(word, p.teacher[(long long)t * p.list + k], p.vocab));
-        float d = 0.f;
-        if (here)
-          d = p.half ? warp_dot((const __half*)p.hidden + t * p.ldh, (const __half*)p.weight + v * p.ldw, p.width, lane)
-                     : warp_dot((const __nv_bfloat16*)p.hidden + t * p.ldh, (const __nv_bfloat16*)p.weight + v * p.ldw, p.width, lane);
-        if (lane == 0) p.listed[f] = d;
+    // ===================== listed logits (warps 10..13): four words of a row at a time =====================
+    const int groups = (p.list + 3) / 4;
+    const long long total = (long long)rows * groups, workers = (long long)gridDim.x * GATHER_WARPS;
+    for (long long f = (long long)blockIdx.x * GATHER_WARPS + warp - 2 - EPI_WARPS; f < total; f += workers) {
+      const int i = (int)(f / groups), k0 = (int)(f - (long long)i * groups) * 4, t = p.rowmap[i];
+      long long mine = -1;                              // lane j: place of word k0 + j among this rank's, or -1
+      if (lane < 4 && k0 + lane < p.list) {
+        const long long word = p.idx[(long long)t * p.list + k0 + lane], v = word - p.vocab_start;
+        if (v >= 0 && v < p.words && (!p.teacher || place_used(word, p.teacher[(long long)t * p.list + k0 + lane], p.vocab))) mine = v;
       }
+      if (p.half) dots_of_row<__half>(p, i, k0, t, mine, lane);
+      else dots_of_row<__nv_bfloat16>(p, i, k0, t, mine, lane);
+    }
   } else {
     // ===================== epilogue (warps 2..9, both CTAs) =====================
     const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which 128 columns it takes
@@ -883,6 +919,7 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restric
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
       const float* a = acc + (long long)at * H + c;
+#pragma unroll 4
       for (int s = 0; s < splits * (two ? 2 : 1); ++s, a += two ? (s & 1 ? TWO_ROWS * (long long)H : slab - TWO_ROWS * (long long)H) : slab) {
         const float4 u = __ldcs(reinterpret_cast<const float4*>(a)), v = __ldcs(reinterpret_cast<const float4*>(a + 4));
         o[0] += u.x; o[1] += u.y; o[2] += u.z; o[3] += u.w;

@@ -75,6 +75,8 @@ class TransformerEngineBasicFeature(Feature):
         add_arg(g, "--kl-temperature", type=float, default=1.0)
         add_arg(g, "--kl-loss-weight", type=float, default=1.0)
         add_arg(g, "--kl-loss-reduction", type=str, default="mean", choices=["mean", "sum"])
+        add_arg(g, "--kl-teacher-topk", type=int, default=0,
+                help="distil from the teacher's so many largest logits of each token instead of its whole vocabulary (0)")
 
     def validate_args(self, args):
         if args.fp8_format == "hif8":
@@ -99,6 +101,8 @@ class QADFeature(Feature):
             raise AssertionError(f"--kl-temperature must be positive, got {args.kl_temperature}")
         if args.kl_loss_weight < 0:
             raise AssertionError(f"--kl-loss-weight must not be negative, got {args.kl_loss_weight}")
+        if not 0 <= (args.kl_teacher_topk or 0) <= 1024:
+            raise AssertionError(f"--kl-teacher-topk is 0 (whole vocabulary) to 1024, got {args.kl_teacher_topk}")
         if getattr(args, "num_experts", None):
             raise AssertionError("--qad-enable covers dense models only (--num-experts is set)")
         if args.pipeline_model_parallel_size > 1:

@@ -1,7 +1,8 @@
 """GPT decoder language model (Megatron-core ``GPTModel`` surface).
 
 forward(input_ids, position_ids, attention_mask, labels) -> per-token loss [b, s] when labels are
-given on the last pipeline stage, else logits [b, s, V/tp] or hidden states for the next stage.
+given on the last pipeline stage, else logits [b, s, V/tp] or hidden states for the next stage.  With --linear-cross-entropy-fusion the
+loss comes straight from the hidden states (ops/linear_cross_entropy.py) and no logits are kept.
 """
 from __future__ import annotations
 
@@ -104,7 +105,8 @@ class GPTModel(nn.Module):
         return self.rotary_pos_emb.get_cos_sin(full, device)
 
     def forward(self, input_ids, position_ids=None, attention_mask=None, decoder_input=None, labels=None,
-                inference_params=None, packed_seq_params=None, extra_block_kwargs=None, loss_mask=None, **_):
+                inference_params=None, packed_seq_params=None, extra_block_kwargs=None, loss_mask=None, distill_targets=None,
+                distill_temperature=1.0, **_):
         if decoder_input is None and self.pre_process:
             decoder_input = self.embedding(input_ids, position_ids)
         if self.pre_process:
@@ -126,6 +128,8 @@ class GPTModel(nn.Module):
         if not self.post_process:
             return hidden
         weight = self.shared_embedding_or_output_weight() if self.share_embeddings_and_output_weights else None
+        if distill_targets is not None:
+            return self.distillation_loss(hidden, labels, distill_targets, distill_temperature, weight)
         mtp_loss = None
         if self.mtp is not None and labels is not None and self.training:
             mtp_loss = self.mtp(hidden, input_ids, position_ids, labels, loss_mask, self, rpe, attention_mask)
@@ -134,10 +138,12 @@ class GPTModel(nn.Module):
             # sample-major logits: the hidden states change places before the product, not the (vocabulary / hidden times larger) logits
             logits, _ = self.output_layer(hidden.transpose(0, 1).contiguous(), weight=weight)
             return logits
-        logits, _ = self.output_layer(hidden, weight=weight)  # [s, b, V/tp]
-        if labels is None:
-            return logits.transpose(0, 1).contiguous()
-        loss = self.compute_language_model_loss(labels, logits)
+        loss = self.linear_language_model_loss(hidden, labels, weight) if labels is not None else None
+        if loss is None:
+            logits, _ = self.output_layer(hidden, weight=weight)  # [s, b, V/tp]
+            if labels is None:
+                return logits.transpose(0, 1).contiguous()
+            loss = self.compute_language_model_loss(labels, logits)
         if mtp_loss is not None:
             loss = loss + mtp_loss
         return loss
@@ -150,6 +156,51 @@ class GPTModel(nn.Module):
             loss = vocab_parallel_cross_entropy(logits.float(), labels_sb)
         return loss.transpose(0, 1).contiguous()  # [b, s]
 
+    def _linear_loss_operands(self, hidden, weight):
+        """(hidden states [s, b, h] of all tokens, weight, vocabulary group, accumulate into main_grad) for the operators that make the loss
+        without the logits, or None where somebody watches or has replaced what they pass by, or the kernels take other types."""
+        out = self.output_layer
+        weight = out.weight if weight is None else weight
+        if (observed(out, ColumnParallelLinear) or out.bias is not None or type(self).compute_language_model_loss is not _OWN_LOSS
+                or "compute_language_model_loss" in self.__dict__ or hidden.dtype != weight.dtype):
+            return None
+        if hidden.is_cuda and (hidden.dtype not in (torch.bfloat16, torch.float16) or hidden.shape[-1] % 8):
+            return None
+        if out.sequence_parallel:
+            hidden = M.gather_from_sequence_parallel_region(hidden, tensor_parallel_output_grad=True)
+        elif out.allreduce_dgrad:
+            hidden = M.copy_to_tensor_model_parallel_region(hidden)
+        mg = getattr(weight, "main_grad", None)
+        into = (out.gradient_accumulation_fusion and mg is not None and mg.dtype == torch.float32 and mg.is_contiguous()
+                and mg.shape == weight.shape and mg.data_ptr() % 16 == 0)
+        return hidden, weight, out.tp_group if out.world > 1 else None, into
+
+    def linear_language_model_loss(self, hidden, labels, weight=None):
+        """Per-token loss [b, s] by the fused output projection and cross entropy (--linear-cross-entropy-fusion), or None."""
+        ops = self._linear_loss_operands(hidden, weight) if self.config.linear_cross_entropy_fusion else None
+        if ops is None:
+            return None
+        from ..ops.linear_cross_entropy import linear_cross_entropy
+        h, w, group, into = ops
+        return linear_cross_entropy(h, w, labels.transpose(0, 1), group=group, accumulate_main_grad=into).transpose(0, 1).contiguous()
+
+    def distillation_loss(self, hidden, labels, targets, temperature, weight=None):
+        """[2, b, s]: the divergence from a teacher's top words, ``targets`` = (logits, indices) [b, s, K], and next to it the cross entropy
+        against the labels without a graph."""
+        ops = self._linear_loss_operands(hidden, weight)
+        if ops is None:
+            raise RuntimeError("the distillation loss from top words takes a bf16 or fp16 model whose output layer and loss are not replaced")
+        from ..ops.linear_cross_entropy import linear_cross_entropy, linear_topk_distillation
+        h, w, group, into = ops
+        logits, indices = (t.transpose(0, 1) for t in targets)
+        kl = linear_topk_distillation(h, w, logits, indices, temperature, group=group, accumulate_main_grad=into)
+        with torch.no_grad():
+            ce = linear_cross_entropy(h, w, labels.transpose(0, 1), group=group)
+        return torch.stack((kl, ce)).transpose(1, 2).contiguous()
+
     def sharded_state_dict(self, prefix="", sharded_offsets=(), metadata=None):
         from ..checkpointing.sharded import model_sharded_state_dict
         return model_sharded_state_dict(self, prefix)
+
+
+_OWN_LOSS = GPTModel.compute_language_model_loss

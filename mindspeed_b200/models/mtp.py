@@ -61,8 +61,10 @@ class MultiTokenPredictionBlock(nn.Module):
                 raise NotImplementedError("MTP needs the embedding on the loss stage (DualPipeV places both on rank 0)")
             h = layer(h, emb, rotary_pos_emb, attention_mask)
             weight = model.shared_embedding_or_output_weight() if model.share_embeddings_and_output_weights else None
-            logits, _ = model.output_layer(h, weight=weight)
-            loss = vocab_parallel_cross_entropy(logits if logits.is_cuda else logits.float(), lab.transpose(0, 1).contiguous()).transpose(0, 1)
+            loss = model.linear_language_model_loss(h, lab, weight)
+            if loss is None:
+                logits, _ = model.output_layer(h, weight=weight)
+                loss = vocab_parallel_cross_entropy(logits if logits.is_cuda else logits.float(), lab.transpose(0, 1).contiguous()).transpose(0, 1)
             valid = torch.ones_like(loss)
             valid[:, loss.shape[1] - (k + 1):] = 0          # the last k+1 positions have no target
             loss = loss * valid

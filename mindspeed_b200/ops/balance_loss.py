@@ -7,6 +7,7 @@ map forward, one backward.  On a CPU it runs as eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -26,6 +27,11 @@ def _lib():
     return L
 
 
+@functools.lru_cache(maxsize=64)
+def _blocks(S, B, E):
+    return _lib().msb_balance_blocks(S, B, E)
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, routing_map, scale, sigmoid, B):
@@ -35,7 +41,7 @@ class _BalanceLoss(torch.autograd.Function):
         T, E = x.shape
         S = T // B
         with _on_device(dev):
-            blocks = L.msb_balance_blocks(S, B, E)
+            blocks = _blocks(S, B, E)
             n = B * blocks * E
             parts = B * ((E + 31) // 32)
             buf = torch.empty(B * E + 2 * n + parts + 1, dtype=torch.float32, device=dev)   # loads; sums of p, counts, joined products, ticket

@@ -57,13 +57,24 @@ class TopKRouter(nn.Module):
         dt = torch.float64 if getattr(self.config, "moe_router_dtype", None) == "fp64" else torch.float32
         return torch.nn.functional.linear(x.to(dt), self.weight.to(dt))
 
-    def _aux(self, probs_for_loss, routing_map, tokens_per_expert, activation, seq_shape):
+    def _wants_aux(self):
+        return self.config.moe_aux_loss_coeff > 0 and self.training and self.routing_type not in ("none", "sinkhorn")
+
+    def _fused_aux(self, logits):
+        """True where ops/balance_loss.py makes the balance loss and the counts (--moe-balance-loss-fusion)."""
+        return bool(self.config.moe_balance_loss_fusion and self._wants_aux() and (not logits.is_cuda or logits.dtype != torch.float64)
+                    and self.num_experts <= 1024)
+
+    def _aux(self, probs_for_loss, routing_map, tokens_per_expert, activation, seq_shape, aux_of=None):
+        """Attaches the balance loss to ``activation``; ``aux_of(coeff, sequences)`` gives it where it is made by one operator."""
         cfg = self.config
-        if cfg.moe_aux_loss_coeff <= 0 or not self.training or self.routing_type in ("none", "sinkhorn"):
+        if not self._wants_aux():
             return activation
         tp_cp = ps.get_tensor_and_context_parallel_world_size() if cfg.sequence_parallel or ps.get_context_parallel_world_size() > 1 else 1
         coeff = cfg.moe_aux_loss_coeff / max(tp_cp, 1)
-        if self.routing_type == "seq_aux_loss":
+        if aux_of is not None:
+            aux = aux_of(coeff, seq_shape[1] if self.routing_type == "seq_aux_loss" else 1)
+        elif self.routing_type == "seq_aux_loss":
             s, b = seq_shape
             aux = sequence_load_balancing_loss_func(probs_for_loss, routing_map, b, s, self.topk, coeff)
         else:
@@ -89,19 +100,31 @@ class TopKRouter(nn.Module):
             logits, self.topk, cfg.moe_expert_capacity_factor, cfg.moe_pad_expert_input_to_capacity, cfg.moe_token_drop_policy,
             cfg.moe_router_pre_softmax, cfg.moe_router_num_groups, cfg.moe_router_group_topk,
             cfg.moe_router_topk_scaling_factor, self.score_function, self.expert_bias)
+        if self._fused_aux(logits):
+            from ...ops.balance_loss import router_balance_loss
+            counts = []
+
+            def aux_of(coeff, sequences):
+                aux, n = router_balance_loss(logits, rmap, self.topk, coeff, self.score_function, sequences)
+                counts.append(n)
+                return aux
+            probs = self._aux(None, rmap, tpe, probs, seq_shape, aux_of)
+            per_expert = counts[0]
+        else:
+            per_expert = None
+            if self.score_function == "softmax":
+                scores_for_loss = torch.softmax(logits.float(), dim=-1)
+            else:
+                sg = torch.sigmoid(logits.float())
+                scores_for_loss = sg / (sg.sum(-1, keepdim=True) + 1e-20)
+            probs = self._aux(scores_for_loss, rmap, tpe, probs, seq_shape)
         if self.expert_bias is not None and self.training:
             with torch.no_grad():
-                self.local_tokens_per_expert += rmap.sum(0).float()
+                self.local_tokens_per_expert += (rmap.sum(0) if per_expert is None else per_expert).float()
         if self.track_load and self.training:
             # tokens routed to each expert since the last report (--print-expert-load / --enable-expert-placement)
             with torch.no_grad():
-                self.expert_load += rmap.sum(0).float()
-        if self.score_function == "softmax":
-            scores_for_loss = torch.softmax(logits.float(), dim=-1)
-        else:
-            sg = torch.sigmoid(logits.float())
-            scores_for_loss = sg / (sg.sum(-1, keepdim=True) + 1e-20)
-        probs = self._aux(scores_for_loss, rmap, tpe, probs, seq_shape)
+                self.expert_load += (rmap.sum(0) if per_expert is None else per_expert).float()
         if cfg.moe_expert_capacity_factor is None:
             mark_rows_per_token(rmap, self.topk)     # no token was dropped: the dispatcher knows its row count without asking the device
         return probs, rmap

@@ -5,7 +5,8 @@ kept in evaluation mode without fake quantisation; the student is the model bein
 linears run on fake-quantised weights).  Every micro-batch the teacher's logits are computed without a graph from the same
 tokens, and the student is trained on the KL divergence from the teacher's distribution alone: temperature
 ``--kl-temperature`` (loss scaled by T^2), weight ``--kl-loss-weight``, ``--kl-loss-reduction`` mean (over unmasked
-tokens) or sum.  The cross entropy against the labels is computed without a graph and reported next to it.  With
+tokens) or sum.  With ``--kl-teacher-topk`` K the teacher's K largest logits of each token, normalised among themselves, stand
+for its distribution; the student's logits are then not kept either (ops/linear_cross_entropy.py).  The cross entropy against the labels is computed without a graph and reported next to it.  With
 vocabulary-parallel logits the softmax normalisers are reduced over the tensor-parallel group, so the loss equals the
 single-rank one.  Dense models without pipeline parallelism only: the loss needs both models' logits for the same
 micro-batch on one rank.
@@ -107,9 +108,49 @@ def qad_loss_func(loss_mask, labels, teacher_logits, args, student_logits):
     return loss, {"lm loss": rep[:2].clone(), "kl loss": rep[2:].clone()}
 
 
+def teacher_top_logits(logits, k, tp_group=None):
+    """The ``k`` largest logits of each token and their words, from (vocabulary-parallel) logits ``[..., V / tp]``: a rank's own largest
+    first, then the largest of all ranks'."""
+    local = logits.shape[-1]
+    world = dist.get_world_size(tp_group) if tp_group is not None else 1
+    if k > local * world:
+        raise ValueError(f"--kl-teacher-topk {k} of a vocabulary of {local * world}")
+    v, i = logits.topk(min(k, local), dim=-1)
+    if world > 1:
+        i = i + dist.get_rank(tp_group) * local
+        vs, is_ = [torch.empty_like(v) for _ in range(world)], [torch.empty_like(i) for _ in range(world)]
+        dist.all_gather(vs, v.contiguous(), group=tp_group)
+        dist.all_gather(is_, i.contiguous(), group=tp_group)
+        v, sel = torch.cat(vs, -1).topk(k, dim=-1)
+        i = torch.cat(is_, -1).gather(-1, sel)
+    return v, i
+
+
+def qad_topk_loss_func(loss_mask, args, out):
+    """Loss function of one micro-batch with --kl-teacher-topk; ``out`` [2, b, s] is the student's divergence and cross entropy per token."""
+    from ..parallel import parallel_state as ps
+    m = loss_mask.reshape(out.shape[1:]).float()
+    kl, n = (out[0] * m).sum(), m.sum()
+    mean = args.kl_loss_reduction == "mean"
+    if mean:
+        kl = kl / n.clamp_min(1.0)
+    with torch.no_grad():
+        rep = torch.stack([(out[1] * m).sum(), n, kl.detach() * (n if mean else 1.0), n if mean else torch.ones_like(n)])
+        dist.all_reduce(rep, group=ps.get_data_parallel_group())
+    return args.kl_loss_weight * kl, {"lm loss": rep[:2].clone(), "kl loss": rep[2:].clone()}
+
+
 def qad_forward_step(tokens, labels, loss_mask, attention_mask, position_ids, packed, model, args):
     """Teacher (no graph) and student forward of one micro-batch; returns (student logits, loss function)."""
     from functools import partial
     teacher_logits = get_teacher().forward(tokens, position_ids, attention_mask, packed_seq_params=packed)
+    if getattr(args, "kl_teacher_topk", 0):
+        from ..parallel import parallel_state as ps
+        tp_group = ps.get_tensor_model_parallel_group() if ps.get_tensor_model_parallel_world_size() > 1 else None
+        with torch.no_grad():
+            targets = teacher_top_logits(teacher_logits, args.kl_teacher_topk, tp_group)
+        out = model(tokens, position_ids, attention_mask, packed_seq_params=packed, labels=labels, distill_targets=targets,
+                    distill_temperature=args.kl_temperature)
+        return out, partial(qad_topk_loss_func, loss_mask, args)
     out = model(tokens, position_ids, attention_mask, packed_seq_params=packed)
     return out, partial(qad_loss_func, loss_mask, labels, teacher_logits, args)

@@ -55,6 +55,8 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--apply-query-key-layer-scaling", action="store_true")
     g.add_argument("--attention-softmax-in-fp32", action="store_true")
     g.add_argument("--use-flash-attn", action="store_true")
+    g.add_argument("--linear-cross-entropy-fusion", action="store_true",
+                   help="output projection and cross entropy in one operator that keeps no logits (bf16 / fp16 on a GPU)")
     g.add_argument("--mtp-num-layers", type=int, default=None)
     g.add_argument("--mtp-loss-scaling-factor", type=float, default=0.1)
 
@@ -91,6 +93,8 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--moe-token-drop-policy", type=str, default="probs", choices=["probs", "position"])
     g.add_argument("--moe-layer-recompute", action="store_true")
     g.add_argument("--moe-permute-fusion", action="store_true")
+    g.add_argument("--moe-balance-loss-fusion", action="store_true",
+                   help="scores, counts, balance loss and its gradient in one pass over the router logits each way")
     g.add_argument("--moe-per-layer-logging", action="store_true")
     g.add_argument("--first-k-dense-replace", type=int, default=0)
 
