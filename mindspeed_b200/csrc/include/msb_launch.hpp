@@ -1,7 +1,7 @@
 // Host side of kernel launches.
 #pragma once
 #include <atomic>
-#include <cuda_runtime_api.h>
+#include <cuda_runtime.h>
 
 extern "C" void msb_set_error(const char* fmt, ...);
 
@@ -21,4 +21,25 @@ inline int allow_smem(const void* kern, int bytes, const char* what, std::atomic
   stated.fetch_or(bit, std::memory_order_relaxed);
   return 0;
 }
+
+#ifdef __CUDACC__
+// Launch of a kernel that begins while the one before it on the stream ends: its blocks are placed and set up early and wait in
+// `after_previous()`, which every thread of such a kernel calls before it touches memory that an earlier kernel writes or reads.  What
+// earlier kernels of the same chain wrote must not be read through `const __restrict__` pointers (the compiler may move such loads).
+// The first kernel of a chain is launched the ordinary way.
+template <typename... P, typename... A>
+inline cudaError_t launch_after(void (*kern)(P...), dim3 grid, unsigned block, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid; c.blockDim = dim3(block); c.dynamicSmemBytes = smem; c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at; c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kern, P(args)...);
+}
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+#endif
 }  // namespace msb

@@ -98,6 +98,7 @@ template <typename T, int VEC, int NJ, bool SIGMOID>
 __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S,
                                                                  int B, int E, int lanes, float* __restrict__ psum, int* __restrict__ csum,
                                                                  unsigned int* __restrict__ ticket) {
+  after_previous();
   extern __shared__ float sh[];                 // [WARPS][E]
   constexpr int N = NJ * VEC;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (lanes - 1), sub = lane / lanes, rows_per_warp = 32 / lanes;
@@ -165,9 +166,10 @@ __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __res
 
 // grid (ceil(E / 32), B), 32 experts x 32 slices of the blocks: loads f, the products' sum; the last block to end adds those in order and
 // the counts over the sequences.
-__global__ void __launch_bounds__(1024) balance_join_kernel(const float* __restrict__ psum, const int* __restrict__ csum, int blocks, int B, int E,
+__global__ void __launch_bounds__(1024) balance_join_kernel(const float* psum, const int* csum, int blocks, int B, int E,
                                                             float scale, float* __restrict__ load, float* __restrict__ lpart,
                                                             unsigned int* ticket, float* __restrict__ loss, long long* __restrict__ counts) {
+  after_previous();
   __shared__ float ps[32][33];
   __shared__ int cs[32][33];
   __shared__ bool last;
@@ -307,7 +309,7 @@ MSB_API int msb_balance_forward(const void* logits, const unsigned char* map, in
   BAL_DISPATCH(BAL_CALL)
 #undef BAL_CALL
   MSB_CHECK_LAUNCH("balance_sums");
-  balance_join_kernel<<<dim3((E + 31) / 32, B), 1024, 0, s>>>(psum, csum, blocks, B, E, scale, load, lpart, ticket, loss, counts);
+  msb::launch_after(balance_join_kernel, dim3((E + 31) / 32, B), 1024, 0, s, psum, csum, blocks, B, E, scale, load, lpart, ticket, loss, counts);
   MSB_CHECK_LAUNCH("balance_join");
   return 0;
 }

@@ -218,16 +218,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();                 // 0 = leader
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int rows = p.rows[0], splits = p.split ? p.rows[1] : 1;
-  const int padded = p.two && rows > 0 ? 2 * TWO_ROWS : rows;
-  const int M = p.rows_on_k ? p.M : padded, K = p.rows_on_k ? padded : p.K;
-  const bool packed = rows != p.all_rows;
   constexpr uint32_t TMEM_COLS = 512u;                    // two accumulators of 256 columns
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NSTAGE; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 2 * EPI_WARPS); }
     mbar_fence_init();
+    tma_prefetch_desc(&p.tmA);
+    tma_prefetch_desc(&p.tmB);
   }
   if (warp == 1) { tmem_alloc_pair(tmem_slot, TMEM_COLS); tmem_relinquish_pair(); }
   tc_fence_before();
@@ -235,6 +233,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
   cluster_sync_all();          // barriers of both CTAs are initialised before anyone signals across the pair
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_ptr;
+  after_previous();
+
+  const int rows = p.rows[0], splits = p.split ? p.rows[1] : 1;
+  const int padded = p.two && rows > 0 ? 2 * TWO_ROWS : rows;
+  const int M = p.rows_on_k ? p.M : padded, K = p.rows_on_k ? padded : p.K;
+  const bool packed = rows != p.all_rows;
 
   bool alive = true;
   if (warp == 0) {
@@ -242,8 +246,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
     if (lane == 0) {
       const CUtensorMap* mapA = (EPI <= EPI_DLOGITS && packed) ? &p.tmPacked : &p.tmA;
       const CUtensorMap* mapB = (p.rows_on_k && packed) ? &p.tmPacked : &p.tmB;
-      tma_prefetch_desc(mapA);
-      tma_prefetch_desc(mapB);
       int stage = 0; uint32_t phase = 0;
       Work w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
@@ -524,7 +526,8 @@ struct Splits { int blocks, pairs, most; };
 
 // One warp a token.
 __global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restrict__ idx, const float* __restrict__ teacher, int T, int K,
-                                                       long long vocab, unsigned char* __restrict__ kind) {
+                                                       long long vocab, unsigned char* kind) {
+  after_previous();
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t >= T) return;
   bool used = false, bad = false;
@@ -541,9 +544,10 @@ __global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restri
 // Numbers the rows that stay, in the order of the tokens: pos[t] = packed row, -1 ignored, -2 a word outside the vocabulary (also noted
 // in `error`); rowmap is the inverse.  One block; a warp takes 256 neighbouring tokens a round (8192 tokens a round of the block), their
 // kinds as eight ballots.
-__global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restrict__ labels, const unsigned char* __restrict__ kind, int T, int H,
-                                                        long long vocab, long long ignore_index, Splits sp, int* __restrict__ pos,
-                                                        int* __restrict__ rowmap, int* __restrict__ count, unsigned int* error) {
+__global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restrict__ labels, const unsigned char* kind, int T, int H,
+                                                        long long vocab, long long ignore_index, Splits sp, int* pos,
+                                                        int* rowmap, int* count, unsigned int* error) {
+  after_previous();
   __shared__ int warp_n[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int base = 0;
@@ -598,9 +602,10 @@ constexpr int SCAN_MOST = 2048, SCAN_LIST = 16;
 template <bool SCAN>
 __global__ void __launch_bounds__(256) lce_rows_kernel(const uint4* __restrict__ hidden, long long ldh, const long long* __restrict__ idx,
                                                        const float* __restrict__ teacher, int Tn, int H, int K, long long vocab,
-                                                       long long ignore_index, Splits sp, int* __restrict__ pos, int* __restrict__ rowmap,
-                                                       int* __restrict__ count, unsigned int* error, uint4* __restrict__ packed,
-                                                       float* __restrict__ loss) {
+                                                       long long ignore_index, Splits sp, int* pos, int* rowmap,
+                                                       int* count, unsigned int* error, uint4* packed,
+                                                       float* loss) {
+  after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int token_blocks = (Tn + 7) / 8, t = (int)blockIdx.x * 8 + warp, vecs = H / 8;
   int n, at = -1;
@@ -681,14 +686,15 @@ __device__ __forceinline__ void lce_finish(float m, float s, float dot, float en
 // value; for a list it makes the weights q, dot = sum q z / tau and ent = sum q log q.
 // 256 threads and 8 rows keep five blocks on an SM (8192 rows, 128256 words: 52 us with 32 rows a block); few rows take 128 threads each.
 template <typename T, int R, int S>
-__global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* __restrict__ part, const unsigned char* __restrict__ part_at,
+__global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* part, const unsigned char* part_at,
                                                         long long part_ld, int parts, const T* __restrict__ hidden, long long ldh,
                                                         const T* __restrict__ weight, long long ldw, int H, float inv_tau, float tc_inv_tau,
-                                                        float tau2, const int* __restrict__ count, const int* __restrict__ rowmap,
+                                                        float tau2, const int* count, const int* rowmap,
                                                         const long long* __restrict__ idx, const float* __restrict__ teacher, int K,
-                                                        long long vocab, const float* __restrict__ z, float* __restrict__ qout,
-                                                        float* __restrict__ dot, float* __restrict__ ent, float* __restrict__ mo,
-                                                        float* __restrict__ so, float* __restrict__ lse, float* __restrict__ loss) {
+                                                        long long vocab, const float* z, float* qout,
+                                                        float* dot, float* ent, float* mo,
+                                                        float* so, float* lse, float* loss) {
+  after_previous();
   __shared__ float ms[S][R + 1], ss[S][R + 1];
   __shared__ int as[S][R + 1];
   const int n = *count;
@@ -796,8 +802,9 @@ __global__ void lce_loss_kernel(const float* gm, const float* gs, const float* d
 // backward helpers
 // ---------------------------------------------------------------------------------------------------------
 // scale[0] = 2^e with max |g| * factor * 2^e in [2^14, 2^15), scale[1] = 2^-e (one block; 1 where there is no finite gradient but 0)
-__global__ void __launch_bounds__(1024) lce_scale_kernel(const float* __restrict__ g, int g_stride, const int* __restrict__ rowmap,
-                                                         const int* __restrict__ count, float factor, float* __restrict__ scale) {
+__global__ void __launch_bounds__(1024) lce_scale_kernel(const float* __restrict__ g, int g_stride, const int* rowmap,
+                                                         const int* count, float factor, float* scale) {
+  after_previous();
   __shared__ float red[32];
   const int n = *count;
   float m = 0.f;
@@ -817,11 +824,12 @@ __global__ void __launch_bounds__(1024) lce_scale_kernel(const float* __restrict
 // The listed words' entries of the piece: dz[i, v] = (exp(z / tau - lse) - sum of the q of all places that list v) * coefficient.  Places
 // that list a word twice write the same value.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, long long ld_row, long long ld_word, int two, const long long* __restrict__ idx,
-                                                         const float* __restrict__ z, const float* __restrict__ q, const float* __restrict__ lse,
-                                                         const int* __restrict__ rowmap, const int* __restrict__ count, int K,
+__global__ void __launch_bounds__(256) lce_listed_kernel(T* dz, long long ld_row, long long ld_word, int two, const long long* __restrict__ idx,
+                                                         const float* z, const float* q, const float* lse,
+                                                         const int* rowmap, const int* count, int K,
                                                          long long piece_start, int piece_cols, const float* __restrict__ g, int g_stride,
-                                                         float g_factor, float inv_tau, const float* __restrict__ scale) {
+                                                         float g_factor, float inv_tau, const float* scale) {
+  after_previous();
   const long long f = (long long)blockIdx.x * 256 + threadIdx.x;
   const int i = (int)(f / K), k = (int)(f - (long long)i * K);
   if (i >= *count) return;
@@ -849,11 +857,12 @@ __global__ void __launch_bounds__(256) lce_listed_kernel(T* __restrict__ dz, lon
 // dz of kept logits, both [V, ldt] with the rows innermost: eight rows of one word a thread.  Rows past the last are zero.  TWO: dz is
 // [V, 2 ldt], the second half what the rounding of the first left.
 template <typename T, bool TWO>
-__global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int V, const float* __restrict__ lse,
-                                                     const long long* __restrict__ label, const float* __restrict__ z,
-                                                     const int* __restrict__ rowmap, const int* __restrict__ count, long long vocab_start,
+__global__ void __launch_bounds__(256) lce_dz_kernel(const float* zt, T* dz, int ldt, int V, const float* lse,
+                                                     const long long* __restrict__ label, const float* z,
+                                                     const int* rowmap, const int* count, long long vocab_start,
                                                      const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
-                                                     float tc_inv_tau, const float* __restrict__ scale) {
+                                                     float tc_inv_tau, const float* scale) {
+  after_previous();
   const int groups = ldt / 8, n = *count;
   // the block's threads take (256 / groups) words a round, always the same rows
   const int per = max(1, 256 / groups), grp = threadIdx.x % groups, sub = threadIdx.x / groups;
@@ -909,8 +918,9 @@ __global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ z
 
 // d hidden: the fp32 slabs of the K splits, added in order, back in the order of the tokens; zero rows for tokens that left.
 template <typename T>
-__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restrict__ acc, const int* __restrict__ count, long long slab, int two, const int* __restrict__ pos,
+__global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* acc, const int* count, long long slab, int two, const int* pos,
                                                           T* __restrict__ out, int Tn, int H) {
+  after_previous();
   const int per_row = H / 8, splits = count[1];
   const long long total = (long long)Tn * per_row;
   for (long long f = (long long)blockIdx.x * 256 + threadIdx.x; f < total; f += (long long)gridDim.x * 256) {
@@ -935,15 +945,29 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* __restric
 // ---------------------------------------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------------------------------------
+#define LCE_FIRST(name, kern, grid, block, smem, ...)          \
+  do {                                                         \
+    auto k__ = kern;                                           \
+    k__<<<grid, block, smem, s>>>(__VA_ARGS__);                \
+    MSB_CHECK_LAUNCH(name);                                    \
+  } while (0)
+#define LCE_AFTER(name, kern, grid, block, smem, ...)          \
+  do {                                                         \
+    auto k__ = kern;                                           \
+    msb::launch_after(k__, dim3(grid), block, smem, s, __VA_ARGS__); \
+    MSB_CHECK_LAUNCH(name);                                    \
+  } while (0)
+
 template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(const LceGemm& p, int most_splits, cudaStream_t s) {
+int launch_gemm(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
   using L = Cfg<EPI>;
   auto kern = lce_gemm_kernel<EPI, A_MN, B_MN>;
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
   const long long items = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN) * most_splits;
   const int pairs = (int)std::min<long long>(items, msb::num_sms() / 2);
-  kern<<<2 * pairs, L::THREADS, L::TOTAL, s>>>(p);
+  if (first) kern<<<2 * pairs, L::THREADS, L::TOTAL, s>>>(p);
+  else msb::launch_after(kern, dim3(2 * pairs), L::THREADS, L::TOTAL, s, p);
   MSB_CHECK_LAUNCH("lce_gemm");
   return 0;
 }
@@ -1019,20 +1043,23 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
   if (!scan) {
     if (a->teacher) {
-      lce_kind_kernel<<<(a->T + 7) / 8, 256, 0, s>>>(a->idx, a->teacher, a->T, a->K, a->vocab, a->kind);
-      MSB_CHECK_LAUNCH("lce_kind");
+      LCE_FIRST("lce_kind", lce_kind_kernel, (a->T + 7) / 8, 256, 0, a->idx, a->teacher, a->T, a->K, a->vocab, a->kind);
     }
-    lce_scan_kernel<<<1, 1024, 0, s>>>(a->teacher ? nullptr : a->idx, a->kind, a->T, a->H, a->vocab, a->ignore_index, sp, a->pos, a->rowmap,
-                                       a->count, a->status + 1);
-    MSB_CHECK_LAUNCH("lce_scan");
+    const long long* labels = a->teacher ? nullptr : a->idx;
+    if (a->teacher)
+      LCE_AFTER("lce_scan", lce_scan_kernel, 1, 1024, 0, labels, a->kind, a->T, a->H, a->vocab, a->ignore_index, sp, a->pos, a->rowmap, a->count,
+                a->status + 1);
+    else
+      LCE_FIRST("lce_scan", lce_scan_kernel, 1, 1024, 0, labels, a->kind, a->T, a->H, a->vocab, a->ignore_index, sp, a->pos, a->rowmap, a->count,
+                a->status + 1);
   }
   const unsigned grid = (unsigned)((a->T + 7) / 8 + 8);
-#define LCE_ROWS(SCAN)                                                                                                                       \
-  lce_rows_kernel<SCAN><<<grid, 256, 0, s>>>((const uint4*)hidden, a->ldh, a->idx, a->teacher, a->T, a->H, a->K, a->vocab, a->ignore_index,   \
-                                             sp, a->pos, a->rowmap, a->count, a->status + 1, (uint4*)a->packed, a->loss)
-  if (scan) LCE_ROWS(true); else LCE_ROWS(false);
+#define LCE_ROWS(HOW, SCAN)                                                                                                                  \
+  HOW("lce_rows", lce_rows_kernel<SCAN>, grid, 256, 0, (const uint4*)hidden, a->ldh, a->idx, a->teacher, a->T, a->H, a->K, a->vocab,           \
+      a->ignore_index, sp, a->pos, a->rowmap, a->count, a->status + 1, (uint4*)a->packed, a->loss)
+  if (scan) LCE_ROWS(LCE_FIRST, true);
+  else LCE_ROWS(LCE_AFTER, false);
 #undef LCE_ROWS
-  MSB_CHECK_LAUNCH("lce_rows");
   LceGemm p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType dt = map_type(a->dtype);
@@ -1052,15 +1079,14 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.rowmap = a->rowmap;
   p.inv_tau = inv_tau; p.tc_inv_tau = tc_scale(inv_tau, a->H);
   p.status = a->status;
-  if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, s))) return rc;
+  if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, false, s))) return rc;
 #define LCE_JOIN(R, S)                                                                                                                       \
-  lce_join_kernel<DT, R, S><<<(a->T + R - 1) / R, R * S, 0, s>>>(p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden, a->ldh, weight,     \
-                                                                a->ldw, a->H, inv_tau, p.tc_inv_tau, tau2, a->count, a->rowmap, a->idx,      \
-                                                                a->teacher, a->K, a->vocab, a->z, a->q, a->dot, a->ent, a->mx, a->sum,       \
-                                                                a->lse, a->loss)
-  if (a->T <= 1024) LCE_JOIN(4, 128); else LCE_JOIN(8, 32);
+  LCE_AFTER("lce_join", (lce_join_kernel<DT, R, S>), (a->T + R - 1) / R, R * S, 0, p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden,    \
+            a->ldh, weight, a->ldw, a->H, inv_tau, p.tc_inv_tau, tau2, a->count, a->rowmap, a->idx, a->teacher, a->K, a->vocab, a->z, a->q,    \
+            a->dot, a->ent, a->mx, a->sum, a->lse, a->loss)
+  if (a->T <= 1024) LCE_JOIN(4, 128);
+  else LCE_JOIN(8, 32);
 #undef LCE_JOIN
-  MSB_CHECK_LAUNCH("lce_join");
   return 0;
 }
 
@@ -1090,8 +1116,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   const long long* label = a->teacher ? nullptr : a->idx;
   DT* dz = (DT*)a->dz;
   if (a->scale) {
-    lce_scale_kernel<<<1, 1024, 0, s>>>(a->g, (int)a->g_stride, a->rowmap, a->count, a->tau, a->scale);
-    MSB_CHECK_LAUNCH("lce_scale");
+    LCE_FIRST("lce_scale", lce_scale_kernel, 1, 1024, 0, a->g, (int)a->g_stride, a->rowmap, a->count, a->tau, a->scale);
   }
   LceGemm p;
   memset(&p, 0, sizeof(p));
@@ -1114,26 +1139,30 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
     if (a->zt) {
       const int per = std::max(1, 256 / (a->ldt / 8));
       const int grid = (int)std::min<long long>((a->V + per - 1) / per, (long long)msb::num_sms() * 8);
-#define LCE_DZ(TWO)                                                                                                                          \
-  lce_dz_kernel<DT, TWO><<<grid, 256, 0, s>>>(a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start, a->g,        \
-                                              (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
-      if (two) LCE_DZ(true); else LCE_DZ(false);
+#define LCE_DZ(HOW, TWO)                                                                                                                     \
+  HOW("lce_dz", (lce_dz_kernel<DT, TWO>), grid, 256, 0, a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start,      \
+      a->g, (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
+      if (a->scale) {
+        if (two) LCE_DZ(LCE_AFTER, true);
+        else LCE_DZ(LCE_AFTER, false);
+      } else {
+        if (two) LCE_DZ(LCE_FIRST, true);
+        else LCE_DZ(LCE_FIRST, false);
+      }
 #undef LCE_DZ
-      MSB_CHECK_LAUNCH("lce_dz");
     } else {
       if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BN / 2, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
       p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
-      if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, s))) return rc;
+      if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, v0 == 0 && !a->scale, s))) return rc;
     }
     if (a->teacher) {
       const long long places = (long long)a->T * a->K;
-      lce_listed_kernel<DT><<<(unsigned)((places + 255) / 256), 256, 0, s>>>(dz, a->zt ? 1 : a->ldz, a->zt ? dz_ld : 1, two, a->idx, a->z, a->q, a->lse,
-                                                                            a->rowmap, a->count, a->K, a->vocab_start + v0, cols, a->g,
-                                                                            (int)a->g_stride, a->tau, inv_tau, a->scale);
-      MSB_CHECK_LAUNCH("lce_listed");
+      LCE_AFTER("lce_listed", lce_listed_kernel<DT>, (unsigned)((places + 255) / 256), 256, 0, dz, a->zt ? 1 : a->ldz, a->zt ? dz_ld : 1, two,
+                a->idx, a->z, a->q, a->lse, a->rowmap, a->count, a->K, a->vocab_start + v0, cols, a->g, (int)a->g_stride, a->tau, inv_tau,
+                a->scale);
     }
     if (a->acc) {
       if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BK, 64);
@@ -1142,7 +1171,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
       p.M = dz_rows; p.N = a->H; p.K = cols; p.rows_on_k = 0; p.split = 1; p.two = two; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
-      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, s);
+      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, false, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, false, s);
       if (rc) return rc;
     }
     if (a->dweight) {
@@ -1155,11 +1184,11 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if (a->dweight_fp32_add) {
         if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
-        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, 1, s) : launch_gemm<EPI_OUT32, true, true>(p, 1, s);
+        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, 1, false, s) : launch_gemm<EPI_OUT32, true, true>(p, 1, false, s);
       } else {
         if ((rc = make_tmap_2d(&p.tmD, (DT*)a->dweight + v0 * a->H, dt, 2, cols, a->H, a->H, 32, 64))) return rc;
         p.accumulate = 0;
-        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, 1, s) : launch_gemm<EPI_OUT16, true, true>(p, 1, s);
+        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, 1, false, s) : launch_gemm<EPI_OUT16, true, true>(p, 1, false, s);
       }
       if (rc) return rc;
     }
@@ -1167,8 +1196,8 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   if (a->acc) {
     const long long vecs = (long long)a->T * (a->H / 8);
     const unsigned grid = (unsigned)std::min<long long>((vecs + 255) / 256, (long long)msb::num_sms() * 16);
-    lce_dhidden_kernel<DT><<<grid, 256, 0, s>>>(a->acc, a->count, (long long)a->slab_rows * a->H, two, a->pos, (DT*)a->dhidden, a->T, a->H);
-    MSB_CHECK_LAUNCH("lce_dhidden");
+    LCE_AFTER("lce_dhidden", lce_dhidden_kernel<DT>, grid, 256, 0, a->acc, a->count, (long long)a->slab_rows * a->H, two, a->pos,
+              (DT*)a->dhidden, a->T, a->H);
   }
   return 0;
 }
