@@ -34,7 +34,8 @@ def _blocks(S, B, E):
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, routing_map, scale, sigmoid, B):
+    def forward(ctx, logits, job):
+        routing_map, scale, sigmoid, B = job
         L = _lib()
         dev = logits.device
         x, rmap = logits.contiguous(), routing_map.contiguous()
@@ -61,7 +62,7 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g, _):
         if g is None:
-            return None, None, None, None, None
+            return None, None
         if torch.is_grad_enabled():
             raise RuntimeError("router_balance_loss has no second derivative (create_graph)")
         L = _lib()
@@ -73,7 +74,7 @@ class _BalanceLoss(torch.autograd.Function):
             grad = torch.empty_like(x)
             loader.check(L.msb_balance_backward(x.data_ptr(), buf.data_ptr(), T // B, B, E, sigmoid, scale, g.data_ptr(), code(x.dtype),
                                                 grad.data_ptr(), loader.stream_ptr()), "balance_backward")
-        return grad, None, None, None, None
+        return grad, None
 
 
 def _balance_ref(logits, routing_map, scale, sigmoid, B):
@@ -114,5 +115,5 @@ def router_balance_loss(logits, routing_map, topk, coeff, score_function="softma
             raise TypeError(f"router_balance_loss: the sm_100a kernels take fp32, bf16 or fp16, not {logits.dtype}")
         if E > MAX_EXPERTS or T > 1 << 24:
             raise ValueError(f"router_balance_loss: {E} experts (at most {MAX_EXPERTS}), {T} tokens (at most 2^24)")
-        return _BalanceLoss.apply(logits, routing_map, scale, int(sigmoid), int(batch_size))
+        return _BalanceLoss.apply(logits, (routing_map, scale, int(sigmoid), int(batch_size)))
     return _balance_ref(logits, routing_map, scale, sigmoid, int(batch_size))

@@ -23,6 +23,7 @@ On a CPU the same functions run as eager PyTorch.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -51,23 +52,12 @@ class _Args(ctypes.Structure):
                 ("splits", _I), ("slab_rows", _I), ("dhidden", _P), ("dweight", _P), ("dweight_fp32_add", _I), ("scale", _P), ("status", _P)]
 
 
-class _on_device:
+_STAY = contextlib.nullcontext()
+
+
+def _on_device(dev):
     """Makes ``dev`` the current device for the launches inside; nothing where it is already."""
-
-    def __init__(self, dev):
-        self.dev = dev.index
-        self.prev = None
-
-    def __enter__(self):
-        cur = torch._C._cuda_getDevice()
-        if cur != self.dev:
-            self.prev = cur
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-        return False
+    return _STAY if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _status(dev):
@@ -78,25 +68,26 @@ def _status(dev):
 
 def _rows(t):
     """``t`` [rows, H] as the kernels read it: unit inner stride, rows on 16-byte boundaries that do not overlap."""
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t
     ld = t.shape[1] if t.shape[0] == 1 else t.stride(0)
     if t.stride(1) != 1 or ld % 8 or ld < t.shape[1] or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        ld = t.shape[1]
-    return t, ld
+    return t
 
 
 @functools.lru_cache(maxsize=64)
-def _plan(T, H, V, piece_bytes, slab_bytes):
-    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits or 0).
+def _plan(T, H, V, piece_bytes, slab_bytes, train):
+    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits or 0 where none are).
 
     The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
     four times are never better.  Logits are kept where they take, in fp32, at most an eighth of the weight's bytes, or 64 rows."""
     cols = min(max(256, piece_bytes // (2 * T) // 256 * 256), (V + 255) // 256 * 256)
     tiles = -(-H // 256)
     splits = max(1, min(64, -(-296 // tiles), slab_bytes // ((T + 31) // 32 * 32 * H * 4)))
-    return cols, splits, TWO_ROWS if T <= TWO_ROWS else (T + 7) // 8 * 8 if 16 * T <= H else 0
+    return cols, splits, 0 if not train else TWO_ROWS if T <= TWO_ROWS else (T + 7) // 8 * 8 if 16 * T <= H else 0
 
 
 def _lib():
@@ -109,63 +100,74 @@ def _lib():
     return L
 
 
-def _point_at_kept(a, kept, T, H, V, K, ldt):
-    """Places of what both directions use in the one buffer that is kept between them (4-byte words)."""
-    at = kept.data_ptr()
-    a.packed = at
-    at += 2 * T * H
-    if ldt:
-        a.zt, a.ldt = at, ldt
-        at += 4 * V * ldt
-    a.z, a.q, a.lse = at, at + 4 * T * K, at + 8 * T * K
-    at += 8 * T * K + 4 * T
-    a.pos, a.rowmap, a.count = at, at + 4 * T, at + 8 * T
+class _Job:
+    """One call: its targets and what stays the same in both directions.  (Autograd passes it along as one argument; every argument of a
+    function costs host time, and short calls are bound by that.)"""
+    __slots__ = ("idx", "teacher", "K", "tau", "ignore_index", "group", "world", "rank", "main_grad", "train", "plan", "shape")
+
+    def __init__(self, hidden, weight, idx, teacher, K, tau, ignore_index, group, main_grad):
+        self.idx, self.teacher, self.K, self.tau, self.ignore_index, self.group = idx, teacher, K, tau, ignore_index, group
+        self.world, self.rank = (1, 0) if group is None else (dist.get_world_size(group), dist.get_rank(group))
+        self.main_grad = weight if main_grad else None
+        self.train = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+
+    def args(self, h, w, idx, teacher, kept):
+        """The argument block with what both directions need.  ``kept``: [packed rows | logits of few rows | z, q, lse | pos, rowmap, count],
+        4-byte words."""
+        (T, H), (V, _) = h.shape, w.shape
+        K = self.K
+        piece, splits, ldt = self.plan
+        at = kept.data_ptr()
+        z = at + 2 * T * H + 4 * V * ldt
+        pos = z + 8 * T * K + 4 * T
+        return _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
+                     ldh=h.stride(0) if T > 1 else H, ldw=w.stride(0) if V > 1 else H, vocab_start=self.rank * V, vocab=self.world * V,
+                     ignore_index=self.ignore_index, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=self.tau, packed=at,
+                     zt=at + 2 * T * H if ldt else None, ldt=ldt, z=z, q=z + 4 * T * K, lse=z + 8 * T * K, pos=pos, rowmap=pos + 4 * T,
+                     count=pos + 8 * T, piece=piece, splits=splits, status=_status(h.device).data_ptr())
 
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, idx, teacher, tau, ignore_index, group, main_grad, train):
+    def forward(ctx, hidden, weight, job):
         L = _lib()
         dev = hidden.device
-        lead = hidden.shape[:-1]
-        h, ldh = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1]))
-        w, ldw = _rows(weight)
-        (T, H), V = h.shape, w.shape[0]
-        K = 1 if teacher is None else idx.shape[-1]
-        world, rank = (1, 0) if group is None else (dist.get_world_size(group), dist.get_rank(group))
-        plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES)
-        piece, splits, ldt = plan
-        if not train:
-            ldt = 0
+        h, w = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
+        (T, H), V, K = h.shape, w.shape[0], job.K
+        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train)
+        job.shape = hidden.shape
+        ldt = job.plan[2]
         with _on_device(dev):
             kept = torch.empty(T * H // 2 + V * ldt + 2 * T * K + 3 * T + 2, dtype=torch.float32, device=dev)
             parts = (V + 255) // 256 * 2
             scratch = torch.empty(2 * parts * T + 4 * T + (parts * T + T + 3) // 4, dtype=torch.float32, device=dev)
-            loss = torch.empty(lead, dtype=torch.float32, device=dev)
-            sp = scratch.data_ptr()
-            after = sp + 8 * parts * T
-            a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
-                      ldh=ldh, ldw=ldw, vocab_start=rank * V, vocab=world * V, ignore_index=ignore_index, T=T, H=H, V=V, K=K,
-                      dtype=code(h.dtype), tau=tau, loss=loss.data_ptr(), part=sp, dot=after, ent=after + 4 * T,
-                      part_at=after + 16 * T, kind=after + 16 * T + parts * T, piece=piece, splits=splits, status=_status(dev).data_ptr())
-            _point_at_kept(a, kept, T, H, V, K, ldt)
+            loss = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
+            a = job.args(h, w, job.idx, job.teacher, kept)
+            a.loss = loss.data_ptr()
+            a.part = at = scratch.data_ptr()
+            a.dot = at = at + 8 * parts * T
+            a.ent = at + 4 * T
+            a.part_at = at + 16 * T
+            a.kind = at + 16 * T + parts * T
             st = loader.stream_ptr()
-            if world > 1:
+            if job.world > 1:
                 at = 2 * parts * T
                 dot, ent, mx, sm = (scratch[at + i * T:at + (i + 1) * T] for i in range(4))
                 a.mx, a.sum = mx.data_ptr(), sm.data_ptr()
             loader.check(L.msb_lce_forward(a, st), "linear_ce_forward")
-            if world > 1:
+            if job.world > 1:
                 gmx = mx.clone()
-                dist.all_reduce(gmx, op=dist.ReduceOp.MAX, group=group)
-                loader.check(L.msb_lce_rescale(sm.data_ptr(), mx.data_ptr(), gmx.data_ptr(), tau, a.count, T, st), "linear_ce_rescale")
-                dist.all_reduce(sm, group=group)
-                dist.all_reduce(dot, group=group)
-                loader.check(L.msb_lce_loss(gmx.data_ptr(), sm.data_ptr(), dot.data_ptr(), ent.data_ptr(), a.rowmap, a.count, tau, T, a.lse,
+                dist.all_reduce(gmx, op=dist.ReduceOp.MAX, group=job.group)
+                loader.check(L.msb_lce_rescale(sm.data_ptr(), mx.data_ptr(), gmx.data_ptr(), job.tau, a.count, T, st), "linear_ce_rescale")
+                dist.all_reduce(sm, group=job.group)
+                dist.all_reduce(dot, group=job.group)
+                loader.check(L.msb_lce_loss(gmx.data_ptr(), sm.data_ptr(), dot.data_ptr(), ent.data_ptr(), a.rowmap, a.count, job.tau, T, a.lse,
                                             loss.data_ptr(), st), "linear_ce_loss")
-        if train:
-            ctx.save_for_backward(h, w, idx, teacher, kept)
-            ctx.meta = (tau, rank, hidden.shape, plan, weight if main_grad else None)
+        if job.train:
+            # targets that come from inference mode cannot be kept as they are
+            ctx.save_for_backward(h, w, *(t.clone() if t is not None and t.is_inference() else t for t in (job.idx, job.teacher)), kept)
+            job.idx = job.teacher = None          # the saved ones count: hooks may have moved them
+            ctx.job = job
         return loss
 
     @staticmethod
@@ -174,33 +176,32 @@ class _LinearLoss(torch.autograd.Function):
             raise RuntimeError("linear loss operators have no second derivative (create_graph)")
         L = _lib()
         h, w, idx, teacher, kept = ctx.saved_tensors
-        tau, rank, shape, (piece, splits, ldt), param = ctx.meta
-        need_h, need_w = ctx.needs_input_grad[:2]
+        job = ctx.job
+        need_h, need_w, _ = ctx.needs_input_grad
         dev = h.device
-        h, ldh = _rows(h)
-        w, ldw = _rows(w)
+        h, w = _rows(h), _rows(w)
         (T, H), V = h.shape, w.shape[0]
-        K = 1 if teacher is None else idx.shape[-1]
+        piece, splits, ldt = job.plan
         with _on_device(dev):
-            one = all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape))      # an expanded scalar, as a sum's backward gives
+            one = not any(g.stride()) or g.numel() == 1      # an expanded scalar, as a sum's backward gives
             if not one and not g.is_contiguous():
                 g = g.contiguous()
-            ldz = 0 if ldt else min(piece, (V + 7) // 8 * 8)
             two = ldt and T <= TWO_ROWS
+            ldz = 0 if ldt else min(piece, (V + 7) // 8 * 8)
             slab_rows = 2 * TWO_ROWS if two else (T + 31) // 32 * 32
             dz_words = (V * (2 if two else 1) * ldt if ldt else T * ldz) // 2
             scratch = torch.empty(dz_words + (splits * slab_rows * H if need_h else 0) + 2, dtype=torch.float32, device=dev)
-            sp = scratch.data_ptr()
-            a = _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
-                      ldh=ldh, ldw=ldw, vocab_start=rank * V, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=tau, g=g.data_ptr(),
-                      g_stride=0 if one else 1, dz=sp, ldz=ldz, piece=piece, splits=splits, slab_rows=slab_rows, status=_status(dev).data_ptr())
-            _point_at_kept(a, kept, T, H, V, K, ldt)
+            a = job.args(h, w, idx, teacher, kept)
+            a.g, a.g_stride = g.data_ptr(), 0 if one else 1
+            a.dz = at = scratch.data_ptr()
+            a.ldz, a.slab_rows = ldz, slab_rows
             dh = dw = None
             if h.dtype == torch.float16:
-                a.scale = sp + 4 * (scratch.numel() - 2)
+                a.scale = at + 4 * (scratch.numel() - 2)
             if need_h:
-                dh = torch.empty(shape, dtype=h.dtype, device=dev)
-                a.acc, a.dhidden = sp + 4 * dz_words, dh.data_ptr()
+                dh = torch.empty(job.shape, dtype=h.dtype, device=dev)
+                a.acc, a.dhidden = at + 4 * dz_words, dh.data_ptr()
+            param = job.main_grad
             if need_w:
                 if param is not None:
                     a.dweight, a.dweight_fp32_add = param.main_grad.data_ptr(), 1
@@ -213,7 +214,7 @@ class _LinearLoss(torch.autograd.Function):
             cb = getattr(param, "_main_grad_ready_cb", None)
             if cb is not None:
                 cb(param)
-        return dh, dw, None, None, None, None, None, None, None
+        return dh, dw, None
 
 
 class _SumOverGroup(torch.autograd.Function):
@@ -284,10 +285,6 @@ def _none(hidden, weight):
     return hidden.float().sum(-1) + weight[:0].float().sum()
 
 
-def _train(hidden, weight):
-    return torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
-
-
 def _main_grad_hook(weight):
     """The eager form's weight for ``accumulate_main_grad``: its gradient goes to main_grad instead of autograd."""
     w = weight.detach().requires_grad_(weight.requires_grad)
@@ -310,9 +307,10 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, 
         raise ValueError(f"linear_cross_entropy: labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
     if labels.numel() == 0:
         return _none(hidden, weight)
-    idx = labels.reshape(-1).long().contiguous()
+    idx = labels if labels.dtype == torch.int64 and labels.is_contiguous() else labels.long().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, idx, None, 1.0, int(ignore_index), group, bool(accumulate_main_grad), _train(hidden, weight))
+        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, None, 1, 1.0, int(ignore_index), group, accumulate_main_grad))
+    idx = idx.reshape(-1)
     world = 1 if group is None else dist.get_world_size(group)
     kept = idx != ignore_index
     if bool(((idx < 0) | (idx >= world * weight.shape[0]))[kept].any()):
@@ -344,7 +342,7 @@ def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, te
     idx = teacher_indices.reshape(-1, K).long().contiguous()
     a = teacher_logits.detach().reshape(-1, K).float().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, idx, a, tau, 0, group, bool(accumulate_main_grad), _train(hidden, weight))
+        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, a, K, tau, 0, group, accumulate_main_grad))
     world = 1 if group is None else dist.get_world_size(group)
     if bool((idx >= world * weight.shape[0]).any()):
         raise IndexError(f"{name}: a teacher index outside the vocabulary")

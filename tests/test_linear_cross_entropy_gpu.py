@@ -132,7 +132,7 @@ def test_pieces_and_splits(dtype, monkeypatch):
     h, w, fav, g, gen = _inputs(T, V, H, dtype)
     idx = torch.randint(0, V, (T, 5), generator=gen, device="cuda")
     a = torch.randn(T, 5, generator=gen, device="cuda")
-    assert M._plan(T, H, V, M.PIECE_BYTES, M.SLAB_BYTES)[1] > 1
+    assert M._plan(T, H, V, M.PIECE_BYTES, M.SLAB_BYTES, True)[1] > 1
     for size in (M.PIECE_BYTES, 2 * T * 256, 2 * T * 1100):
         monkeypatch.setattr(M, "PIECE_BYTES", size)
         _compare(_ce(h, w, fav, g), h, w, _ce_target(fav), 1.0, g)
@@ -233,6 +233,21 @@ def test_words_outside_the_vocabulary():
     assert torch.isnan(got[0][9]) and (got[1][9] == 0).all() and torch.isfinite(got[2]).all()
     with pytest.raises(RuntimeError, match="outside the vocabulary"):
         check_status()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_targets_of_inference_mode_and_no_gradients(dtype):
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    T, V, H = 70, 500, 64
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    with torch.inference_mode():
+        idx, a, lab = torch.randint(0, V, (T, 4), generator=gen, device="cuda"), torch.randn(T, 4, generator=gen, device="cuda"), fav.clone()
+        scored = linear_cross_entropy(h, w, lab)
+    _compare(_kd(h, w, a, idx, 2.0, g), h, w, _kd_target(idx.clone(), a.clone(), 2.0), 2.0, g)
+    got = _ce(h, w, lab, g)
+    _compare(got, h, w, _ce_target(fav), 1.0, g)
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(h.clone().requires_grad_(True), w, fav), got[0]) and torch.equal(scored.clone(), got[0])
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
