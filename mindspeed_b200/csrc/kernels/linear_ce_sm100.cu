@@ -24,6 +24,9 @@
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
+// Up to 128 rows they run on single CTAs with tiles of 128 x 256: half of a pair's 256 rows would be padding, and although W's bytes bound
+// such calls, products of padding draw the power that the clocks then lack (96 x 128256 x 4096 forward: 215 us at first, 255 at the power
+// limit with pairs).
 #include "msb_common.cuh"
 #include "msb_sm100.cuh"
 #include <algorithm>
@@ -85,12 +88,13 @@ struct LceGemm {
   unsigned int* status;
 };
 
-template <int EPI>
+template <int EPI, bool PAIR>
 struct Cfg {
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + (EPI == EPI_STATS ? GATHER_WARPS : 0));
-  static constexpr int NSTAGE = EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5;   // what the staging leaves of 227 KB
+  // what the staging leaves of 227 KB
+  static constexpr int NSTAGE = PAIR ? (EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5) : EPI == EPI_OUT32 ? 3 : 4;
   static constexpr int A_BYTES = BM * BK * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + (BN / 2) * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? BN / 2 : BN) * BK * 2;
   static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
   static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
@@ -98,12 +102,13 @@ struct Cfg {
   static_assert(TOTAL <= 232448, "exceeds the 227 KB of shared memory a CTA may use");
 };
 
-// Work items of a pair: (tile, split of K).  Every role walks its own copy.  Tiles in groups of `group_m` tile rows share panels in L2.
+// Work items of a pair (or single CTA): (tile, split of K).  Every role walks its own copy.  Tiles in groups of `group_m` tile rows share panels in L2.
+template <int TILE_M>
 struct Work {
   int num_m, num_n, num_kb, group_m, splits, item, items, stride;
   int m, n, split, kb0, kb1;
   __device__ Work(int M, int N, int K, int group_m_, int splits_, int pair, int npairs)
-      : num_m((M + 2 * BM - 1) / (2 * BM)), num_n((N + BN - 1) / BN), num_kb((K + BK - 1) / BK), splits(splits_), item(pair),
+      : num_m((M + TILE_M - 1) / TILE_M), num_n((N + BN - 1) / BN), num_kb((K + BK - 1) / BK), splits(splits_), item(pair),
         stride(npairs), m(0), n(0), split(0), kb0(0), kb1(0) {
     group_m = min(group_m_, max(num_m, 1));
     items = num_m * num_n * splits;
@@ -201,9 +206,11 @@ __device__ __forceinline__ void dots_of_row(const LceGemm& p, int i, int k0, int
 
 // EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K].      Hidden gradient: A = dz [M, K], B = W [K, N].
 // Weight gradient: A = dz [K, M], B = hidden [K, N], rows on K.  A_MN tells how dz lies in memory ([tokens, words] or transposed).
-template <int EPI, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
-  using L = Cfg<EPI>;
+template <int EPI, bool A_MN, bool B_MN, bool PAIR>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, PAIR>::THREADS, 1)
+    lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+  using L = Cfg<EPI, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
   constexpr int NSTAGE = L::NSTAGE;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // identical in both CTAs of the pair
@@ -216,21 +223,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
   uint32_t* tmem_slot_ptr = reinterpret_cast<uint32_t*>(smem_raw + (tmem_slot - smem_u32(smem_raw)));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t cta = cluster_ctarank();                 // 0 = leader
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const uint32_t cta = PAIR ? cluster_ctarank() : 0;      // 0 = leader
+  const int pair = blockIdx.x / CTAS, npairs = gridDim.x / CTAS;
   constexpr uint32_t TMEM_COLS = 512u;                    // two accumulators of 256 columns
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NSTAGE; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 2 * EPI_WARPS); }
+    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), CTAS * EPI_WARPS); }
     mbar_fence_init();
     tma_prefetch_desc(&p.tmA);
     tma_prefetch_desc(&p.tmB);
   }
-  if (warp == 1) { tmem_alloc_pair(tmem_slot, TMEM_COLS); tmem_relinquish_pair(); }
+  if (warp == 1) {
+    if (PAIR) { tmem_alloc_pair(tmem_slot, TMEM_COLS); tmem_relinquish_pair(); }
+    else { tmem_alloc(tmem_slot, TMEM_COLS); tmem_relinquish(); }
+  }
   tc_fence_before();
   __syncwarp();
-  cluster_sync_all();          // barriers of both CTAs are initialised before anyone signals across the pair
+  if (PAIR) cluster_sync_all();   // barriers of both CTAs are initialised before anyone signals across the pair
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_ptr;
   after_previous();
@@ -247,30 +258,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
       const CUtensorMap* mapA = (EPI <= EPI_DLOGITS && packed) ? &p.tmPacked : &p.tmA;
       const CUtensorMap* mapB = (p.rows_on_k && packed) ? &p.tmPacked : &p.tmB;
       int stage = 0; uint32_t phase = 0;
-      Work w(M, p.N, K, p.group_m, splits, pair, npairs);
+      Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
-        const int m0 = w.m * (2 * BM) + (int)cta * BM;
+        const int m0 = (w.m * CTAS + (int)cta) * BM;
         const int n0 = w.n * BN + (int)cta * (BN / 2);
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.status, 0x10u)) { alive = false; break; }
           const uint32_t sa = smem_base + stage * L::STAGE_BYTES;
           const uint32_t sb = sa + L::A_BYTES;
-          if (cta == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * L::STAGE_BYTES);
-          const uint32_t lead_full = mapa_u32(full_bar(stage), 0);
+          if (cta == 0) mbar_arrive_expect_tx(full_bar(stage), CTAS * L::STAGE_BYTES);
+          const uint32_t lead_full = PAIR ? mapa_u32(full_bar(stage), 0) : full_bar(stage);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if (PAIR) tma_load_2d_pair(dst, map, lead_full, x, y);
+            else tma_load_2d(dst, map, lead_full, x, y);
+          };
           const int k0 = kb * BK;
           if (!A_MN) {
-            tma_load_2d_pair(sa, mapA, lead_full, k0, m0);                             // box [128 rows x 64 k]
+            load(sa, mapA, k0, m0);                                                    // box [128 rows x 64 k]
           } else {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j)                                          // boxes [64 k x 64 m]
-              tma_load_2d_pair(sa + j * (BK * 128), mapA, lead_full, m0 + j * 64, k0);
+            for (int j = 0; j < BM / 64; ++j) load(sa + j * (BK * 128), mapA, m0 + j * 64, k0);   // boxes [64 k x 64 m]
           }
           if (!B_MN) {
-            tma_load_2d_pair(sb, mapB, lead_full, k0, n0);                             // box [128 rows x 64 k]
+            load(sb, mapB, k0, n0);                                                    // box [128 rows x 64 k] (256 on a single CTA)
           } else {
 #pragma unroll
-            for (int j = 0; j < BN / 128; ++j)                                         // boxes [64 k x 64 n]
-              tma_load_2d_pair(sb + j * (BK * 128), mapB, lead_full, n0 + j * 64, p.rows_on_k && p.two ? 0 : k0);   // both terms times the same rows
+            for (int j = 0; j < BN / CTAS / 64; ++j)                                   // boxes [64 k x 64 n]; both terms times the same rows
+              load(sb + j * (BK * 128), mapB, n0 + j * 64, p.rows_on_k && p.two ? 0 : k0);
           }
           if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
         }
@@ -284,10 +298,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
   } else if (warp == 1) {
     // ===================== MMA issuer (leader CTA, one thread) =====================
     if (lane == 0 && cta == 0) {
-      const uint32_t idesc = make_idesc_f16(2 * BM, BN, p.half ? 0 : 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
+      const uint32_t idesc = make_idesc_f16(CTAS * BM, BN, p.half ? 0 : 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
       int stage = 0; uint32_t phase = 0;
       int acc = 0; uint32_t acc_phase = 0;
-      Work w(M, p.N, K, p.group_m, splits, pair, npairs);
+      Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.status, 0x20u)) { alive = false; break; }
         tc_fence_after();
@@ -304,13 +318,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
                                         : make_smem_desc(sa + k * (UMMA_K * 2), 0, 1024);
             const uint64_t bdesc = B_MN ? make_smem_desc(sb + k * (UMMA_K * 128), BK * 128, 1024)
                                         : make_smem_desc(sb + k * (UMMA_K * 2), 0, 1024);
-            umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            if (PAIR) umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            else umma_f16(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
           }
-          umma_commit_pair(empty_bar(stage), 3);      // both CTAs may refill this stage once these MMAs have read it
+          // both CTAs may refill this stage once these MMAs have read it
+          if (PAIR) umma_commit_pair(empty_bar(stage), 3);
+          else umma_commit(empty_bar(stage));
           if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
         }
         if (!alive) break;
-        umma_commit_pair(tfull_bar(acc), 3);          // accumulator complete in both CTAs
+        if (PAIR) umma_commit_pair(tfull_bar(acc), 3);          // accumulator complete in both CTAs
+        else umma_commit(tfull_bar(acc));
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
     }
@@ -332,14 +350,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
     // ===================== epilogue (warps 2..9, both CTAs) =====================
     const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which 128 columns it takes
     const uint32_t buf_base = smem_base + L::EPI_OFFSET + (uint32_t)(warp - 2) * L::EPI_BUF;
-    const uint32_t lead_tempty[2] = {mapa_u32(tempty_bar(0), 0), mapa_u32(tempty_bar(1), 0)};
+    const uint32_t lead_tempty[2] = {PAIR ? mapa_u32(tempty_bar(0), 0) : tempty_bar(0), PAIR ? mapa_u32(tempty_bar(1), 0) : tempty_bar(1)};
     const float unscale = (EPI >= EPI_OUT16 && p.scale) ? p.scale[1] : 1.f;
     const float ctau = p.tc_inv_tau * LOG2E;
     uint32_t chunk = 0;
     int acc = 0; uint32_t acc_phase = 0;
-    Work w(M, p.N, K, p.group_m, splits, pair, npairs);
+    Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
     while (alive && w.next()) {
-      const int row0 = w.m * (2 * BM) + (int)cta * BM + q * 32, row = row0 + lane;
+      const int row0 = (w.m * CTAS + (int)cta) * BM + q * 32, row = row0 + lane;
       float coef = 0.f, lse = 0.f, at_label = 0.f;
       long long label = -1;
       if (EPI == EPI_DLOGITS && row < rows) {
@@ -474,7 +492,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(lead_tempty[acc]);   // this warp has read its part of the accumulator
+      if (lane == 0) {                                       // this warp has read its part of the accumulator
+        if (PAIR) mbar_arrive_remote(lead_tempty[acc]);
+        else mbar_arrive(lead_tempty[acc]);
+      }
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) tma_store_wait<0>();                 // staging buffers are read and the stores are complete before exit
@@ -483,10 +504,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI>::THREADS, 1
   // ---- teardown: both CTAs meet, TMEM is returned ----
   tc_fence_before();
   __syncwarp();
-  cluster_sync_all();
+  if (PAIR) cluster_sync_all();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
@@ -522,7 +545,7 @@ __device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs
   return best;
 }
 
-struct Splits { int blocks, pairs, most; };
+struct Splits { int blocks, pairs, most; };        // blocks of 64 words, SM pairs (or SMs) that take the tiles, most splits
 
 // One warp a token.
 __global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restrict__ idx, const float* __restrict__ teacher, int T, int K,
@@ -958,19 +981,29 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* acc, cons
     MSB_CHECK_LAUNCH(name);                                    \
   } while (0)
 
-template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
-  using L = Cfg<EPI>;
-  auto kern = lce_gemm_kernel<EPI, A_MN, B_MN>;
+template <int EPI, bool A_MN, bool B_MN, bool PAIR>
+int launch_gemm_on(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
+  using L = Cfg<EPI, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
+  auto kern = lce_gemm_kernel<EPI, A_MN, B_MN, PAIR>;
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
-  const long long items = (long long)((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + BN - 1) / BN) * most_splits;
-  const int pairs = (int)std::min<long long>(items, msb::num_sms() / 2);
-  if (first) kern<<<2 * pairs, L::THREADS, L::TOTAL, s>>>(p);
-  else msb::launch_after(kern, dim3(2 * pairs), L::THREADS, L::TOTAL, s, p);
+  const long long items = (long long)((p.M + CTAS * BM - 1) / (CTAS * BM)) * ((p.N + BN - 1) / BN) * most_splits;
+  const unsigned grid = CTAS * (unsigned)std::min<long long>(items, msb::num_sms() / CTAS);
+  if (first) kern<<<grid, L::THREADS, L::TOTAL, s>>>(p);
+  else msb::launch_after(kern, dim3(grid), L::THREADS, L::TOTAL, s, p);
   MSB_CHECK_LAUNCH("lce_gemm");
   return 0;
 }
+// Single CTAs for up to 128 output rows (see the top of the file); the weight gradient's output rows are words.
+template <int EPI, bool A_MN, bool B_MN>
+int launch_gemm(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
+  if (EPI != EPI_OUT16 && !p.rows_on_k && p.M <= BM)
+    return launch_gemm_on<EPI, A_MN, B_MN, EPI == EPI_OUT16>(p, most_splits, first, s);
+  return launch_gemm_on<EPI, A_MN, B_MN, true>(p, most_splits, first, s);
+}
+// Rows of the box that loads B of such a product: [words, H] as it lies.
+uint32_t words_box(int rows) { return rows <= BM ? BN : BN / 2; }
 
 // 1 / tau for logits that the tensor cores summed over H products (see the top of the file).
 float tc_scale(float inv_tau, int H) { return (float)((double)inv_tau * (1.0 + 0.26 * (H / 16) / 16777216.0)); }
@@ -1039,7 +1072,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const float inv_tau = 1.f / a->tau, tau2 = a->tau * a->tau;
   const DT* hidden = (const DT*)a->hidden;
   const DT* weight = (const DT*)a->weight;
-  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, msb::num_sms() / 2, a->splits};
+  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, a->T <= BM ? msb::num_sms() : msb::num_sms() / 2, a->splits};
   const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
   if (!scan) {
     if (a->teacher) {
@@ -1066,7 +1099,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   int rc;
   if ((rc = make_tmap_2d(&p.tmA, hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
   if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
-  if ((rc = make_tmap_2d(&p.tmB, weight, dt, 2, a->V, a->H, a->ldw, BN / 2, BK))) return rc;
+  if ((rc = make_tmap_2d(&p.tmB, weight, dt, 2, a->V, a->H, a->ldw, words_box(a->T), BK))) return rc;
   p.M = a->T; p.N = a->V; p.K = a->H;
   p.rows = a->count; p.all_rows = a->T;
   p.group_m = GROUP_M;
@@ -1153,7 +1186,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
     } else {
       if ((rc = make_tmap_2d(&p.tmA, a->hidden, dt, 2, a->T, a->H, a->ldh, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
-      if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BN / 2, BK))) return rc;
+      if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, words_box(a->T), BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
       p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
       if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, v0 == 0 && !a->scale, s))) return rc;
