@@ -92,10 +92,10 @@ template <int EPI, bool PAIR>
 struct Cfg {
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + (EPI == EPI_STATS ? GATHER_WARPS : 0));
   // what the staging leaves of 227 KB
-  static constexpr int NSTAGE = PAIR ? (EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5) : EPI == EPI_OUT32 ? 3 : 4;
+  static constexpr int NSTAGE = PAIR ? (EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5) : 4;
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? BN / 2 : BN) * BK * 2;
-  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers
+  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS || !PAIR ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers, OUT32 on single CTAs half a one
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
   static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
@@ -447,46 +447,48 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
 #pragma unroll
             for (int j = 0; j < 64; ++j) rr[j] = empty ? 0u : __float_as_uint(__uint_as_float(rr[j]) * unscale);
           }
-          const uint32_t buf = buf_base + (EPI == EPI_OUT16 ? (chunk++ & 1u) * 4096u : 0u);
-          if (lane == 0) tma_store_wait_read<EPI == EPI_OUT16 ? 1 : 0>();   // the store that last read this buffer is done with it
-          __syncwarp();
-          const uint32_t row_addr = buf + (uint32_t)lane * 128u;
-          if (EPI != EPI_OUT32) {
+          const uint32_t sw_row = (uint32_t)lane * 128u;
+          // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box; rows past the last are never read
+          const int y = p.split ? w.split * p.slab_rows + row0 : row0;
+          const bool inside = p.split ? (p.two ? row0 < p.slab_rows && (row0 & (TWO_ROWS - 1)) < rows : row0 < rows) : row0 < p.M;
+          constexpr int BOXES = EPI == EPI_OUT32 ? 2 : 1, TOGETHER = EPI == EPI_OUT32 && PAIR ? 2 : 1;   // boxes of 128-byte rows; in one go
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {                 // 16-byte chunk j = columns 8j .. 8j+7
-              uint32_t pk[4];
+          for (int b0 = 0; b0 < BOXES; b0 += TOGETHER) {
+            const uint32_t buf = buf_base + (EPI == EPI_OUT16 ? (chunk++ & 1u) * 4096u : 0u);
+            if (lane == 0) tma_store_wait_read<EPI == EPI_OUT16 ? 1 : 0>();   // the store that last read this buffer is done with it
+            __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 4; ++e) pk[e] = pack16(__uint_as_float(rr[8 * j + 2 * e]), __uint_as_float(rr[8 * j + 2 * e + 1]), p.half);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + ((((uint32_t)j) ^ sw) << 4)), "r"(pk[0]), "r"(pk[1]),
-                           "r"(pk[2]), "r"(pk[3])
-                           : "memory");
-            }
-          } else {
+            for (int b = b0; b < b0 + TOGETHER; ++b) {
+              const uint32_t row_addr = buf + (uint32_t)(b - b0) * 4096u + sw_row;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)                   // two [32 x 32] fp32 boxes per 64 columns
+              for (int j = 0; j < 8; ++j) {                 // 16-byte chunk j of the row: eight 16-bit or four 32-bit columns
+                uint32_t v[4];
+                if (EPI == EPI_OUT32) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + (uint32_t)h * 4096u + ((((uint32_t)j) ^ sw) << 4)),
-                             "r"(rr[32 * h + 4 * j]), "r"(rr[32 * h + 4 * j + 1]), "r"(rr[32 * h + 4 * j + 2]), "r"(rr[32 * h + 4 * j + 3])
+                  for (int e = 0; e < 4; ++e) v[e] = rr[32 * b + 4 * j + e];
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) v[e] = pack16(__uint_as_float(rr[8 * j + 2 * e]), __uint_as_float(rr[8 * j + 2 * e + 1]), p.half);
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + ((((uint32_t)j) ^ sw) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                             "r"(v[3])
                              : "memory");
-          }
-          fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
-          __syncwarp();
-          if (lane == 0) {
-            // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box; rows past the last are never read
-            const int y = p.split ? w.split * p.slab_rows + row0 : row0;
-            if (p.split ? (p.two ? row0 < p.slab_rows && (row0 & (TWO_ROWS - 1)) < rows : row0 < rows) : row0 < p.M) {
-              if (EPI != EPI_OUT32) {
-                tma_store_2d(&p.tmD, buf, col0, y);
-              } else if (!p.accumulate) {
-                tma_store_2d(&p.tmD, buf, col0, y);
-                if (col0 + 32 < p.N) tma_store_2d(&p.tmD, buf + 4096u, col0 + 32, y);
-              } else {
-                tma_reduce_add_2d(&p.tmD, buf, col0, y);
-                if (col0 + 32 < p.N) tma_reduce_add_2d(&p.tmD, buf + 4096u, col0 + 32, y);
               }
             }
-            tma_store_commit();
+            fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+              for (int b = b0; b < b0 + TOGETHER; ++b) {
+                const int x = col0 + 32 * b;
+                const uint32_t src = buf + (uint32_t)(b - b0) * 4096u;
+                if (inside && x < p.N) {
+                  if (EPI == EPI_OUT32 && p.accumulate) tma_reduce_add_2d(&p.tmD, src, x, y);
+                  else tma_store_2d(&p.tmD, src, x, y);
+                }
+              }
+              tma_store_commit();
+            }
           }
         }
       }
@@ -939,29 +941,50 @@ __global__ void __launch_bounds__(256) lce_dz_kernel(const float* zt, T* dz, int
   }
 }
 
-// d hidden: the fp32 slabs of the K splits, added in order, back in the order of the tokens; zero rows for tokens that left.
-template <typename T>
+// d hidden: the fp32 slabs of the K splits, added in a fixed order, back in the order of the tokens; zero rows for tokens that left.
+// Y threads share the slabs of eight columns: one where there are few slabs, eight where there are many (few rows), which would
+// otherwise be a chain of loads (one token, 37 slabs: 13 us with one thread).
+template <typename T, int Y>
 __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* acc, const int* count, long long slab, int two, const int* pos,
                                                           T* __restrict__ out, int Tn, int H) {
   after_previous();
-  const int per_row = H / 8, splits = count[1];
+  constexpr int X = 256 / Y;
+  __shared__ float part[Y == 1 ? 1 : Y][X][9];
+  const int x = threadIdx.x % X, y = threadIdx.x / X;
+  const int per_row = H / 8, terms = count[1] * (two ? 2 : 1);
   const long long total = (long long)Tn * per_row;
-  for (long long f = (long long)blockIdx.x * 256 + threadIdx.x; f < total; f += (long long)gridDim.x * 256) {
-    const int t = (int)(f / per_row), c = (int)(f - (long long)t * per_row) * 8;
-    const int at = pos[t];
+  for (long long f0 = (long long)blockIdx.x * X; f0 < total; f0 += (long long)gridDim.x * X) {
+    const long long f = f0 + x;
+    const bool in = f < total;
+    const int t = in ? (int)(f / per_row) : 0, c = in ? (int)(f - (long long)t * per_row) * 8 : 0;
+    const int at = in ? pos[t] : -1;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (at >= 0) {
       const float* a = acc + (long long)at * H + c;
 #pragma unroll 4
-      for (int s = 0; s < splits * (two ? 2 : 1); ++s, a += two ? (s & 1 ? TWO_ROWS * (long long)H : slab - TWO_ROWS * (long long)H) : slab) {
-        const float4 u = __ldcs(reinterpret_cast<const float4*>(a)), v = __ldcs(reinterpret_cast<const float4*>(a + 4));
+      for (int s = y; s < terms; s += Y) {
+        const float* b = a + (two ? (s >> 1) * slab + (s & 1) * (TWO_ROWS * (long long)H) : s * slab);
+        const float4 u = __ldcs(reinterpret_cast<const float4*>(b)), v = __ldcs(reinterpret_cast<const float4*>(b + 4));
         o[0] += u.x; o[1] += u.y; o[2] += u.z; o[3] += u.w;
         o[4] += v.x; o[5] += v.y; o[6] += v.z; o[7] += v.w;
       }
     }
-    Vec8<T> w;
-    w.from_float(o);
-    w.store(out + (long long)t * H + c);
+    if (Y > 1) {
+      __syncthreads();                      // the sums of the last round have been read
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[y][x][j] = o[j];
+      __syncthreads();
+      if (y == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int i = 1; i < Y; ++i) o[j] += part[i][x][j];
+    }
+    if (in && y == 0) {
+      Vec8<T> w;
+      w.from_float(o);
+      w.store(out + (long long)t * H + c);
+    }
   }
 }
 
@@ -1228,9 +1251,13 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   }
   if (a->acc) {
     const long long vecs = (long long)a->T * (a->H / 8);
-    const unsigned grid = (unsigned)std::min<long long>((vecs + 255) / 256, (long long)msb::num_sms() * 16);
-    LCE_AFTER("lce_dhidden", lce_dhidden_kernel<DT>, grid, 256, 0, a->acc, a->count, (long long)a->slab_rows * a->H, two, a->pos,
-              (DT*)a->dhidden, a->T, a->H);
+#define LCE_DHIDDEN(Y)                                                                                                                       \
+  LCE_AFTER("lce_dhidden", (lce_dhidden_kernel<DT, Y>),                                                                                       \
+            (unsigned)std::min<long long>((vecs + 256 / Y - 1) / (256 / Y), (long long)msb::num_sms() * 16), 256, 0, a->acc, a->count,         \
+            (long long)a->slab_rows * a->H, two, a->pos, (DT*)a->dhidden, a->T, a->H)
+    if (a->splits >= 16) LCE_DHIDDEN(8);
+    else LCE_DHIDDEN(1);
+#undef LCE_DHIDDEN
   }
   return 0;
 }
