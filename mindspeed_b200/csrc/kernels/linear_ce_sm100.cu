@@ -10,7 +10,9 @@
 // count, which only the device knows.  When all rows stay, the products read the caller's hidden states directly, else a packed copy.
 //
 // Forward:  scan (part of the rows kernel for short inputs) -> rows (packed copy) -> GEMM whose epilogue keeps (max, where, sum of
-//           exponentials) per row and 128 columns, while four warps a CTA make the K listed logits as dot products -> join.
+//           exponentials) per row and half a tile, and takes listed logits from the accumulators where the lists are sorted; else four
+//           warps a CTA make them as dot products beside it -> join.  (4096 rows, 64 words each, W of 129280 x 4096: the products' rows of
+//           W are 2.1 GB, 0.3 ms as a kernel of its own and as much beside the GEMM.)
 //           The tensor cores cut every addition to their fp32 sums off: a logit comes out 0.26 (H / 16) 2^-24 of itself too small (0.258
 //           to 0.273 measured at H 1024 to 5120; half a unit in the last place for each of the H / 16 additions, of a sum that grows).
 //           The scale 1 / tau of such logits makes that good, and the join computes the largest logit of a row again as a dot product.
@@ -24,7 +26,7 @@
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
-// Up to 128 rows they run on single CTAs with tiles of 128 x 256: half of a pair's 256 rows would be padding, and although W's bytes bound
+// Up to 128 rows they run on single CTAs with tiles of 128 rows: half of a pair's 256 rows would be padding, and although W's bytes bound
 // such calls, products of padding draw the power that the clocks then lack (96 x 128256 x 4096 forward: 215 us at first, 255 at the power
 // limit with pairs).
 #include "msb_common.cuh"
@@ -37,7 +39,6 @@ using namespace msb::sm100;
 namespace {
 
 constexpr int BM = 128;          // rows per CTA; the pair covers 256
-constexpr int BN = 256;
 constexpr int BK = 64;           // 64 16-bit values = one 128-byte swizzle row
 constexpr int UMMA_K = 16;
 constexpr int GROUP_M = 16;      // tile rows that share W panels in L2: forward of 8192 x 128256 x 4096 in 6.7 ms, 7.5 with 8, 6.7 with 32 (backward 20.3 / 20.4 / 21.7)
@@ -62,9 +63,10 @@ struct LceGemm {
   int slab_rows;
   int accumulate;              // OUT32: add to what is there
   int half;                    // operands are fp16 (else bf16)
-  float2* part;                // STATS: [128 columns][part_ld] (max, sum)
+  float2* part;                // STATS: [half a tile's columns][part_ld] (max, sum)
   unsigned char* part_at;      // STATS: column of the max
   long long part_ld;
+  const unsigned long long* sorted;   // STATS: (word << 16 | place) ascending, [T, list], or null: the gathering warps read idx
   const long long* idx;        // STATS: listed words [T, list], their logits go to listed [rows, list]
   const float* teacher;
   float* listed;
@@ -90,11 +92,12 @@ struct LceGemm {
 
 template <int EPI, bool PAIR>
 struct Cfg {
+  static constexpr int TN = 256;   // columns of a tile (the forward of 96 x 128256 x 4096: 208 us, 223 with 128; one token of 32000 x 1024: 25, 30)
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + (EPI == EPI_STATS ? GATHER_WARPS : 0));
   // what the staging leaves of 227 KB
-  static constexpr int NSTAGE = PAIR ? (EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5) : 4;
+  static constexpr int NSTAGE = !PAIR ? 4 : EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5;
   static constexpr int A_BYTES = BM * BK * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? BN / 2 : BN) * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? TN / 2 : TN) * BK * 2;
   static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS || !PAIR ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers, OUT32 on single CTAs half a one
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
   static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
@@ -103,7 +106,7 @@ struct Cfg {
 };
 
 // Work items of a pair (or single CTA): (tile, split of K).  Every role walks its own copy.  Tiles in groups of `group_m` tile rows share panels in L2.
-template <int TILE_M>
+template <int TILE_M, int BN>
 struct Work {
   int num_m, num_n, num_kb, group_m, splits, item, items, stride;
   int m, n, split, kb0, kb1;
@@ -133,6 +136,13 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// One column of the warp's 32 accumulator lanes.
+__device__ __forceinline__ uint32_t tmem_ld_column(uint32_t taddr) {
+  uint32_t v;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr) : "memory");
+  tmem_ld_wait();
+  return v;
 }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, int half) {
   if (half) {
@@ -210,7 +220,7 @@ template <int EPI, bool A_MN, bool B_MN, bool PAIR>
 __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, PAIR>::THREADS, 1)
     lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   using L = Cfg<EPI, PAIR>;
-  constexpr int CTAS = PAIR ? 2 : 1;
+  constexpr int CTAS = PAIR ? 2 : 1, BN = L::TN;
   constexpr int NSTAGE = L::NSTAGE;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // identical in both CTAs of the pair
@@ -225,7 +235,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = PAIR ? cluster_ctarank() : 0;      // 0 = leader
   const int pair = blockIdx.x / CTAS, npairs = gridDim.x / CTAS;
-  constexpr uint32_t TMEM_COLS = 512u;                    // two accumulators of 256 columns
+  constexpr uint32_t TMEM_COLS = 2u * BN;                 // two accumulators
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NSTAGE; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
@@ -258,7 +268,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
       const CUtensorMap* mapA = (EPI <= EPI_DLOGITS && packed) ? &p.tmPacked : &p.tmA;
       const CUtensorMap* mapB = (p.rows_on_k && packed) ? &p.tmPacked : &p.tmB;
       int stage = 0; uint32_t phase = 0;
-      Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
+      Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         const int m0 = (w.m * CTAS + (int)cta) * BM;
         const int n0 = w.n * BN + (int)cta * (BN / 2);
@@ -280,7 +290,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
             for (int j = 0; j < BM / 64; ++j) load(sa + j * (BK * 128), mapA, m0 + j * 64, k0);   // boxes [64 k x 64 m]
           }
           if (!B_MN) {
-            load(sb, mapB, k0, n0);                                                    // box [128 rows x 64 k] (256 on a single CTA)
+            load(sb, mapB, k0, n0);                                                    // box [128 rows x 64 k] (256 on a single CTA of the backward)
           } else {
 #pragma unroll
             for (int j = 0; j < BN / CTAS / 64; ++j)                                   // boxes [64 k x 64 n]; both terms times the same rows
@@ -301,7 +311,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
       const uint32_t idesc = make_idesc_f16(CTAS * BM, BN, p.half ? 0 : 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
       int stage = 0; uint32_t phase = 0;
       int acc = 0; uint32_t acc_phase = 0;
-      Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
+      Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.status, 0x20u)) { alive = false; break; }
         tc_fence_after();
@@ -335,7 +345,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
   } else if (EPI == EPI_STATS && warp >= 2 + EPI_WARPS) {
     // ===================== listed logits (warps 10..13): four words of a row at a time =====================
     const int groups = (p.list + 3) / 4;
-    const long long total = (long long)rows * groups, workers = (long long)gridDim.x * GATHER_WARPS;
+    const long long total = p.sorted ? 0 : (long long)rows * groups, workers = (long long)gridDim.x * GATHER_WARPS;
     for (long long f = (long long)blockIdx.x * GATHER_WARPS + warp - 2 - EPI_WARPS; f < total; f += workers) {
       const int i = (int)(f / groups), k0 = (int)(f - (long long)i * groups) * 4, t = p.rowmap[i];
       long long mine = -1;                              // lane j: place of word k0 + j among this rank's, or -1
@@ -348,14 +358,14 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
     }
   } else {
     // ===================== epilogue (warps 2..9, both CTAs) =====================
-    const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which 128 columns it takes
+    const int q = warp & 3, half = (warp - 2) >> 2;   // TMEM lane quarter this warp may access; which half of the columns it takes
     const uint32_t buf_base = smem_base + L::EPI_OFFSET + (uint32_t)(warp - 2) * L::EPI_BUF;
     const uint32_t lead_tempty[2] = {PAIR ? mapa_u32(tempty_bar(0), 0) : tempty_bar(0), PAIR ? mapa_u32(tempty_bar(1), 0) : tempty_bar(1)};
     const float unscale = (EPI >= EPI_OUT16 && p.scale) ? p.scale[1] : 1.f;
     const float ctau = p.tc_inv_tau * LOG2E;
     uint32_t chunk = 0;
     int acc = 0; uint32_t acc_phase = 0;
-    Work<CTAS * BM> w(M, p.N, K, p.group_m, splits, pair, npairs);
+    Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
     while (alive && w.next()) {
       const int row0 = (w.m * CTAS + (int)cta) * BM + q * 32, row = row0 + lane;
       float coef = 0.f, lse = 0.f, at_label = 0.f;
@@ -369,6 +379,21 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
           label = p.label[t] - p.piece_start;
           at_label = coef == 0.f ? 0.f : (ex2((p.z[row] * p.inv_tau - lse) * LOG2E) - 1.f) * coef;
         }
+      }
+      // the first listed word of this row among the warp's columns
+      const long long c0 = (long long)w.n * BN + half * (BN / 2), c1 = min((long long)p.N, c0 + BN / 2);
+      const unsigned long long* list = nullptr;
+      unsigned long long next = ~0ull;
+      int at_list = 0;
+      if (EPI == EPI_STATS && p.sorted && row < rows) {
+        list = p.sorted + (long long)p.rowmap[row] * p.list;
+        int hi = p.list;
+        while (at_list < hi) {
+          const int mid = (at_list + hi) >> 1;
+          if ((long long)(list[mid] >> 16) < c0) at_list = mid + 1;
+          else hi = mid;
+        }
+        if (at_list < p.list) next = list[at_list];
       }
       if (!mbar_wait_warp(tfull_bar(acc), acc_phase, p.status, 0x30u)) { alive = false; break; }
       tc_fence_after();
@@ -405,7 +430,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
           const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if (cm > m) {
 #pragma unroll
-            for (int j = 63; j >= 0; --j) at = __uint_as_float(rr[j]) == cm ? (c2 & 64) + j : at;
+            for (int j = 63; j >= 0; --j) at = __uint_as_float(rr[j]) == cm ? c2 - half * (BN / 2) + j : at;
           }
           const float mn = fmaxf(m, cm);
           const float base = mn == -INFINITY ? 0.f : mn;
@@ -414,6 +439,19 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
           for (int j = 0; j < 64; ++j) sm[j & 3] += ex2((__uint_as_float(rr[j]) - base) * ctau);
           s = (sm[0] + sm[1]) + (sm[2] + sm[3]);
           m = mn;
+        }
+        if (p.sorted) {
+          for (;;) {
+            const unsigned int hits = __ballot_sync(0xffffffffu, (long long)(next >> 16) < c1);
+            if (!hits) break;
+            const int who = __ffs(hits) - 1;
+            const int col = __shfl_sync(0xffffffffu, (int)((long long)(next >> 16) - (long long)w.n * BN), who);
+            const float z = __uint_as_float(tmem_ld_column(t_row + (uint32_t)col));
+            if (lane == who) {
+              p.listed[(long long)row * p.list + (int)(next & 0xffffu)] = z * (p.tc_inv_tau / p.inv_tau);
+              next = ++at_list < p.list ? list[at_list] : ~0ull;
+            }
+          }
         }
         if (row < rows) {
           const long long o = (long long)(2 * w.n + half) * p.part_ld + row;
@@ -549,21 +587,42 @@ __device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs
 
 struct Splits { int blocks, pairs, most; };        // blocks of 64 words, SM pairs (or SMs) that take the tiles, most splits
 
-// One warp a token.
-__global__ void __launch_bounds__(256) lce_kind_kernel(const long long* __restrict__ idx, const float* __restrict__ teacher, int T, int K,
-                                                       long long vocab, unsigned char* kind) {
+// One warp a token: what its list says, and the words of this rank sorted with their places (bitonic, `padded` = K up to a power of two);
+// the rest of the places behind them as all ones.
+__global__ void __launch_bounds__(128) lce_kind_kernel(const long long* __restrict__ idx, const float* __restrict__ teacher, int T, int K, int padded,
+                                                       long long vocab, long long vocab_start, int words, unsigned char* kind,
+                                                       unsigned long long* sorted) {
   after_previous();
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  extern __shared__ unsigned long long keys_s[];
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  unsigned long long* key = keys_s + (threadIdx.x >> 5) * padded;
   if (t >= T) return;
   bool used = false, bad = false;
-  for (int k = lane; k < K; k += 32) {
-    const long long i = idx[(long long)t * K + k];
-    used |= place_used(i, teacher[(long long)t * K + k], vocab);
-    bad |= i >= vocab;
+  for (int k = lane; k < padded; k += 32) {
+    unsigned long long mine = ~0ull;
+    if (k < K) {
+      const long long i = idx[(long long)t * K + k], v = i - vocab_start;
+      const bool u = place_used(i, teacher[(long long)t * K + k], vocab);
+      used |= u;
+      bad |= i >= vocab;
+      if (u && v >= 0 && v < words) mine = (unsigned long long)v << 16 | (unsigned)k;
+    }
+    key[k] = mine;
   }
   used = __any_sync(0xffffffffu, used);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) kind[t] = bad ? 2 : used ? 1 : 0;
+  for (int size = 2; size <= padded; size <<= 1)
+    for (int gap = size >> 1; gap > 0; gap >>= 1) {
+      __syncwarp();
+      for (int i = lane; i < padded / 2; i += 32) {
+        const int lo = (i / gap) * 2 * gap + i % gap, hi = lo + gap;
+        const unsigned long long x = key[lo], y = key[hi];
+        if ((x > y) == ((lo & size) == 0)) { key[lo] = y; key[hi] = x; }
+      }
+    }
+  __syncwarp();
+  for (int k = lane; k < K; k += 32) sorted[(long long)t * K + k] = key[k];
 }
 
 // Numbers the rows that stay, in the order of the tokens: pos[t] = packed row, -1 ignored, -2 a word outside the vocabulary (also noted
@@ -706,17 +765,17 @@ __device__ __forceinline__ void lce_finish(float m, float s, float dot, float en
   *loss = tau2 * (ent + (m * inv_tau - dot) + ls);       // the two large numbers are subtracted first
 }
 
-// R rows a block, S threads a row over the 128-column parts (neighbouring threads take neighbouring rows); the order of the sums is fixed.
+// R rows a block, S threads a row over the parts of `width` columns (neighbouring threads take neighbouring rows); the order of the sums is fixed.
 // Then one warp a row computes the largest logit again in fp32 and rebases the sum on it: s = 1 + (s - 1) exp((m - m') / tau), m' the new
 // value; for a list it makes the weights q, dot = sum q z / tau and ent = sum q log q.
 // 256 threads and 8 rows keep five blocks on an SM (8192 rows, 128256 words: 52 us with 32 rows a block); few rows take 128 threads each.
 template <typename T, int R, int S>
 __global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* part, const unsigned char* part_at,
-                                                        long long part_ld, int parts, const T* __restrict__ hidden, long long ldh,
+                                                        long long part_ld, int parts, int width, const T* __restrict__ hidden, long long ldh,
                                                         const T* __restrict__ weight, long long ldw, int H, float inv_tau, float tc_inv_tau,
                                                         float tau2, const int* count, const int* rowmap,
                                                         const long long* __restrict__ idx, const float* __restrict__ teacher, int K,
-                                                        long long vocab, const float* z, float* qout,
+                                                        long long vocab, long long vocab_start, int words, const float* z, float* qout,
                                                         float* dot, float* ent, float* mo,
                                                         float* so, float* lse, float* loss) {
   after_previous();
@@ -738,7 +797,7 @@ __global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* part, con
         if (v.x > m) at = i;
         m = mn;
       }
-      at = at * 128 + part_at[(long long)at * part_ld + row];
+      at = at * width + part_at[(long long)at * part_ld + row];
     }
     ms[y][r] = m;
     ss[y][r] = s;
@@ -781,7 +840,8 @@ __global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* part, con
       if (place_used(list[k], a[k], vocab)) {
         const float b = (a[k] - mx) * inv_tau;
         q = ex2(b * LOG2E) / sum;
-        d = fmaf(q, zi[k] * inv_tau, d);
+        const long long v = list[k] - vocab_start;
+        if (v >= 0 && v < words) d = fmaf(q, zi[k] * inv_tau, d);
         if (!(q == 0.f)) e = fmaf(q, b - ls, e);
       }
       qout[(long long)row * K + k] = q;
@@ -789,7 +849,8 @@ __global__ void __launch_bounds__(R * S) lce_join_kernel(const float2* part, con
     d = warp_sum(d);
     e = warp_sum(e);
   } else {
-    d = z[row] * inv_tau;
+    const long long v = idx[t] - vocab_start;
+    d = v >= 0 && v < words ? z[row] * inv_tau : 0.f;
   }
   if (lane == 0) {
     const float m2 = mm == -INFINITY ? mm : again;         // nothing but -inf: NaN, as the formula
@@ -1011,7 +1072,7 @@ int launch_gemm_on(const LceGemm& p, int most_splits, bool first, cudaStream_t s
   auto kern = lce_gemm_kernel<EPI, A_MN, B_MN, PAIR>;
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
-  const long long items = (long long)((p.M + CTAS * BM - 1) / (CTAS * BM)) * ((p.N + BN - 1) / BN) * most_splits;
+  const long long items = (long long)((p.M + CTAS * BM - 1) / (CTAS * BM)) * ((p.N + L::TN - 1) / L::TN) * most_splits;
   const unsigned grid = CTAS * (unsigned)std::min<long long>(items, msb::num_sms() / CTAS);
   if (first) kern<<<grid, L::THREADS, L::TOTAL, s>>>(p);
   else msb::launch_after(kern, dim3(grid), L::THREADS, L::TOTAL, s, p);
@@ -1025,8 +1086,8 @@ int launch_gemm(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
     return launch_gemm_on<EPI, A_MN, B_MN, EPI == EPI_OUT16>(p, most_splits, first, s);
   return launch_gemm_on<EPI, A_MN, B_MN, true>(p, most_splits, first, s);
 }
-// Rows of the box that loads B of such a product: [words, H] as it lies.
-uint32_t words_box(int rows) { return rows <= BM ? BN : BN / 2; }
+// Rows of the boxes that load W as [words, H], for T tokens.
+uint32_t words_box(int T) { return T <= BM ? 256 : 128; }
 
 // 1 / tau for logits that the tensor cores summed over H products (see the top of the file).
 float tc_scale(float inv_tau, int H) { return (float)((double)inv_tau * (1.0 + 0.26 * (H / 16) / 16777216.0)); }
@@ -1050,6 +1111,7 @@ struct MsbLceArgs {
   int* rowmap;                 // [T]
   int* count;                  // [2]: rows that stay, K splits
   unsigned char* kind;         // [T] scratch (lists)
+  unsigned long long* sorted;  // [T, K] scratch (lists)
   void* packed;                // [T, H]
   float* z;                    // [T, K]
   float* q;                    // [T, K]
@@ -1085,8 +1147,9 @@ static int lce_check(const MsbLceArgs* a) {
   MSB_REQUIRE(a->status != nullptr, "linear_ce: status words are required");
   MSB_REQUIRE(a->tau > 0.f, "linear_ce: the temperature must be positive");
   MSB_REQUIRE(a->K == 1 || a->teacher, "linear_ce: lists need teacher logits");
+  MSB_REQUIRE(a->K <= 1024, "linear_ce: %d listed words", a->K);
   MSB_REQUIRE(!a->zt || (a->ldt % 8 == 0 && a->ldt >= a->T && (a->T > TWO_ROWS || a->ldt == TWO_ROWS)), "linear_ce: pitch %d of the kept logits", a->ldt);
-  MSB_REQUIRE(a->piece > 0 && a->piece % BN == 0 && a->splits >= 1, "linear_ce: piece of %d columns, %d splits", a->piece, a->splits);
+  MSB_REQUIRE(a->piece > 0 && a->piece % 256 == 0 && a->splits >= 1, "linear_ce: piece of %d columns, %d splits", a->piece, a->splits);
   return 0;
 }
 
@@ -1099,7 +1162,10 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
   if (!scan) {
     if (a->teacher) {
-      LCE_FIRST("lce_kind", lce_kind_kernel, (a->T + 7) / 8, 256, 0, a->idx, a->teacher, a->T, a->K, a->vocab, a->kind);
+      int padded = 1;
+      while (padded < a->K) padded *= 2;
+      LCE_FIRST("lce_kind", lce_kind_kernel, (a->T + 3) / 4, 128, 4 * padded * 8, a->idx, a->teacher, a->T, a->K, padded, a->vocab, a->vocab_start,
+                a->V, a->kind, a->sorted);
     }
     const long long* labels = a->teacher ? nullptr : a->idx;
     if (a->teacher)
@@ -1129,6 +1195,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.half = a->dtype == MSB_F16;
   p.part = reinterpret_cast<float2*>(a->part); p.part_at = a->part_at; p.part_ld = a->T;
   p.zt = a->zt; p.ldt = a->ldt;
+  p.sorted = a->teacher && !scan ? a->sorted : nullptr;
   p.idx = a->idx; p.teacher = a->teacher; p.listed = a->z; p.list = a->K;
   p.hidden = hidden; p.weight = weight; p.ldh = a->ldh; p.ldw = a->ldw; p.vocab_start = a->vocab_start; p.vocab = a->vocab;
   p.width = a->H; p.words = a->V;
@@ -1136,10 +1203,11 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.inv_tau = inv_tau; p.tc_inv_tau = tc_scale(inv_tau, a->H);
   p.status = a->status;
   if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, false, s))) return rc;
+  constexpr int width = 128;
 #define LCE_JOIN(R, S)                                                                                                                       \
-  LCE_AFTER("lce_join", (lce_join_kernel<DT, R, S>), (a->T + R - 1) / R, R * S, 0, p.part, p.part_at, p.part_ld, (a->V + 127) / 128, hidden,    \
-            a->ldh, weight, a->ldw, a->H, inv_tau, p.tc_inv_tau, tau2, a->count, a->rowmap, a->idx, a->teacher, a->K, a->vocab, a->z, a->q,    \
-            a->dot, a->ent, a->mx, a->sum, a->lse, a->loss)
+  LCE_AFTER("lce_join", (lce_join_kernel<DT, R, S>), (a->T + R - 1) / R, R * S, 0, p.part, p.part_at, p.part_ld, (a->V + width - 1) / width, width, hidden, \
+            a->ldh, weight, a->ldw, a->H, inv_tau, p.tc_inv_tau, tau2, a->count, a->rowmap, a->idx, a->teacher, a->K, a->vocab, a->vocab_start, \
+            a->V, a->z, a->q, a->dot, a->ent, a->mx, a->sum, a->lse, a->loss)
   if (a->T <= 1024) LCE_JOIN(4, 128);
   else LCE_JOIN(8, 32);
 #undef LCE_JOIN

@@ -47,7 +47,7 @@ TWO_ROWS = 64
 class _Args(ctypes.Structure):
     _fields_ = [("hidden", _P), ("weight", _P), ("idx", _P), ("teacher", _P), ("ldh", _LL), ("ldw", _LL), ("vocab_start", _LL), ("vocab", _LL),
                 ("ignore_index", _LL), ("T", _I), ("H", _I), ("V", _I), ("K", _I), ("dtype", _I), ("tau", _F), ("pos", _P), ("rowmap", _P),
-                ("count", _P), ("kind", _P), ("packed", _P), ("z", _P), ("q", _P), ("dot", _P), ("ent", _P), ("lse", _P), ("loss", _P),
+                ("count", _P), ("kind", _P), ("sorted", _P), ("packed", _P), ("z", _P), ("q", _P), ("dot", _P), ("ent", _P), ("lse", _P), ("loss", _P),
                 ("part", _P), ("part_at", _P), ("zt", _P), ("ldt", _I), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
                 ("splits", _I), ("slab_rows", _I), ("dhidden", _P), ("dweight", _P), ("dweight_fp32_add", _I), ("scale", _P), ("status", _P)]
 
@@ -140,18 +140,20 @@ class _LinearLoss(torch.autograd.Function):
         with _on_device(dev):
             kept = torch.empty(T * H // 2 + V * ldt + 2 * T * K + 3 * T + 2, dtype=torch.float32, device=dev)
             parts = (V + 255) // 256 * 2
-            scratch = torch.empty(2 * parts * T + 4 * T + (parts * T + T + 3) // 4, dtype=torch.float32, device=dev)
+            lists = 0 if job.teacher is None else 2 * T * K
+            scratch = torch.empty(lists + 2 * parts * T + 4 * T + (parts * T + T + 3) // 4, dtype=torch.float32, device=dev)
             loss = torch.empty(hidden.shape[:-1], dtype=torch.float32, device=dev)
             a = job.args(h, w, job.idx, job.teacher, kept)
             a.loss = loss.data_ptr()
-            a.part = at = scratch.data_ptr()
+            a.sorted = at = scratch.data_ptr()
+            a.part = at = at + 4 * lists
             a.dot = at = at + 8 * parts * T
             a.ent = at + 4 * T
             a.part_at = at + 16 * T
             a.kind = at + 16 * T + parts * T
             st = loader.stream_ptr()
             if job.world > 1:
-                at = 2 * parts * T
+                at = lists + 2 * parts * T
                 dot, ent, mx, sm = (scratch[at + i * T:at + (i + 1) * T] for i in range(4))
                 a.mx, a.sum = mx.data_ptr(), sm.data_ptr()
             loader.check(L.msb_lce_forward(a, st), "linear_ce_forward")
