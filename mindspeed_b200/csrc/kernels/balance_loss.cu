@@ -108,29 +108,44 @@ __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __res
   int c[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) { P[i] = 0.f; c[i] = 0; }
-  for (long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp; r0 < S; r0 += (long long)gridDim.x * WARPS * rows_per_warp) {
-    const bool in = r0 + sub < S;
+  const long long stride = (long long)gridDim.x * WARPS * rows_per_warp;
+  // the next rows are loaded while these are summed (for wide rows only: two rows of more than 32 experts a lane do not fit the registers)
+  constexpr int AHEAD = N <= 16 ? 2 : 1;
+  float x[AHEAD][N];
+  uint32_t m[AHEAD][NJ];
+  auto fetch = [&](long long r0, float* xr, uint32_t* mr) {
     const long long at = ((r0 + sub) * B + seq) * E;
-    float x[N], slope[N];
-    uint32_t m[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int e = (l + lanes * j) * VEC;
-      m[j] = 0;
+      mr[j] = 0;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) x[j * VEC + v] = -INFINITY;
-      if (in && e < E) {
-        load_row<VEC>(logits + at + e, x + j * VEC);
-        m[j] = VEC == 4 ? *reinterpret_cast<const uint32_t*>(map + at + e) : (uint32_t)map[at + e];
+      for (int v = 0; v < VEC; ++v) xr[j * VEC + v] = -INFINITY;
+      if (r0 + sub < S && e < E) {
+        load_row<VEC>(logits + at + e, xr + j * VEC);
+        mr[j] = VEC == 4 ? *reinterpret_cast<const uint32_t*>(map + at + e) : (uint32_t)map[at + e];
       }
     }
-    scores<N, SIGMOID>(x, slope, lanes);
-    if (in) {
+  };
+  long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp;
+  if (AHEAD == 2 && r0 < S) fetch(r0, x[0], m[0]);
+  for (; r0 < S; r0 += stride) {
+    if (AHEAD == 2) fetch(r0 + stride, x[AHEAD - 1], m[AHEAD - 1]);
+    else fetch(r0, x[0], m[0]);
+    float slope[N];
+    scores<N, SIGMOID>(x[0], slope, lanes);
+    if (r0 + sub < S) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (!((l + lanes * (i / VEC)) * VEC >= E)) P[i] += x[i];
-        c[i] += (m[i / VEC] >> (8 * (i % VEC))) & 0xffu ? 1 : 0;
+        if (!((l + lanes * (i / VEC)) * VEC >= E)) P[i] += x[0][i];
+        c[i] += (m[0][i / VEC] >> (8 * (i % VEC))) & 0xffu ? 1 : 0;
       }
+    }
+    if (AHEAD == 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[0][i] = x[AHEAD - 1][i];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) m[0][j] = m[AHEAD - 1][j];
     }
   }
   for (int o = lanes; o < 32; o <<= 1)
@@ -177,6 +192,7 @@ __global__ void __launch_bounds__(1024) balance_join_kernel(const float* psum, c
   float P = 0.f;
   int c = 0;
   if (e < E)
+#pragma unroll 4
     for (int b = y; b < blocks; b += 32) {
       const long long at = ((long long)seq * blocks + b) * E + e;
       P += psum[at];
@@ -227,31 +243,43 @@ __global__ void __launch_bounds__(WARPS * 32) balance_grad_kernel(const T* __res
     const int e = (l + lanes * (i / VEC)) * VEC + i % VEC;
     f[i] = e < E ? load[(long long)seq * E + e] : 0.f;
   }
-  for (long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp; r0 < S; r0 += (long long)gridDim.x * WARPS * rows_per_warp) {
-    const bool in = r0 + sub < S;
+  const long long stride = (long long)gridDim.x * WARPS * rows_per_warp;
+  constexpr int AHEAD = N <= 16 ? 2 : 1;        // as above
+  float x[AHEAD][N];
+  auto fetch = [&](long long r0, float* xr) {
     const long long at = ((r0 + sub) * B + seq) * E;
-    float x[N], slope[N];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int e = (l + lanes * j) * VEC;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) x[j * VEC + v] = -INFINITY;
-      if (in && e < E) load_row<VEC>(logits + at + e, x + j * VEC);
+      for (int v = 0; v < VEC; ++v) xr[j * VEC + v] = -INFINITY;
+      if (r0 + sub < S && e < E) load_row<VEC>(logits + at + e, xr + j * VEC);
     }
-    scores<N, SIGMOID>(x, slope, lanes);
+  };
+  long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp;
+  if (AHEAD == 2 && r0 < S) fetch(r0, x[0]);
+  for (; r0 < S; r0 += stride) {
+    if (AHEAD == 2) fetch(r0 + stride, x[AHEAD - 1]);
+    else fetch(r0, x[0]);
+    float slope[N];
+    scores<N, SIGMOID>(x[0], slope, lanes);
     float d = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) d = fmaf(x[i], f[i], d);
+    for (int i = 0; i < N; ++i) d = fmaf(x[0][i], f[i], d);
     d = lanes_sum(d, lanes);
 #pragma unroll
     for (int i = 0; i < N; ++i) slope[i] *= (f[i] - d) * gs;
-    if (in) {
+    if (r0 + sub < S) {
+      const long long at = ((r0 + sub) * B + seq) * E;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int e = (l + lanes * j) * VEC;
         if (e < E) store_row<VEC>(grad + at + e, slope + j * VEC);
       }
     }
+    if (AHEAD == 2)
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[0][i] = x[AHEAD - 1][i];
   }
 }
 

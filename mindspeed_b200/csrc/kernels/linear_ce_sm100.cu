@@ -41,7 +41,10 @@ namespace {
 constexpr int BM = 128;          // rows per CTA; the pair covers 256
 constexpr int BK = 64;           // 64 16-bit values = one 128-byte swizzle row
 constexpr int UMMA_K = 16;
-constexpr int GROUP_M = 16;      // tile rows that share W panels in L2: forward of 8192 x 128256 x 4096 in 6.7 ms, 7.5 with 8, 6.7 with 32 (backward 20.3 / 20.4 / 21.7)
+// tile rows that share the other operand's panels in L2.  Logits: 16 keep W's bytes from DRAM at three times its size (forward of 8192 x
+// 128256 x 4096 in 6.7 ms, 7.5 with 8, 6.7 with 32).  Gradients: sums over thousands of words or tokens, whose panels do not outlive a
+// round of tiles in L2; 8 make the rounds square (8192 tokens: dz and weight gradient 13.4 ms, 13.8 with 16, 14.3 with 32).
+constexpr int GROUP_LOGITS = 16, GROUP_GRADS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 constexpr int EPI_WARPS = 8;       // two a quarter of the 128 accumulator lanes, each half of the columns
@@ -1191,7 +1194,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   if ((rc = make_tmap_2d(&p.tmB, weight, dt, 2, a->V, a->H, a->ldw, words_box(a->T), BK))) return rc;
   p.M = a->T; p.N = a->V; p.K = a->H;
   p.rows = a->count; p.all_rows = a->T;
-  p.group_m = GROUP_M;
+  p.group_m = GROUP_LOGITS;
   p.half = a->dtype == MSB_F16;
   p.part = reinterpret_cast<float2*>(a->part); p.part_at = a->part_at; p.part_ld = a->T;
   p.zt = a->zt; p.ldt = a->ldt;
@@ -1245,7 +1248,6 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   LceGemm p;
   memset(&p, 0, sizeof(p));
   p.rows = a->count; p.all_rows = a->T;
-  p.group_m = GROUP_M;
   p.half = a->dtype == MSB_F16;
   p.rowmap = a->rowmap; p.lse = a->lse;
   p.g = a->g; p.g_stride = (int)a->g_stride; p.g_factor = a->tau;
@@ -1279,7 +1281,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BM, BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, words_box(a->T), BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
-      p.M = a->T; p.N = cols; p.K = a->H; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
+      p.M = a->T; p.N = cols; p.K = a->H; p.group_m = GROUP_LOGITS; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
       if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, v0 == 0 && !a->scale, s))) return rc;
     }
     if (a->teacher) {
@@ -1294,7 +1296,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
-      p.M = dz_rows; p.N = a->H; p.K = cols; p.rows_on_k = 0; p.split = 1; p.two = two; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
+      p.M = dz_rows; p.N = a->H; p.K = cols; p.group_m = GROUP_GRADS; p.rows_on_k = 0; p.split = 1; p.two = two; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
       rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, false, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, false, s);
       if (rc) return rc;
     }
@@ -1304,7 +1306,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, a->hidden, dt, 2, a->T, a->H, a->ldh, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BK, 64))) return rc;
-      p.M = cols; p.N = a->H; p.K = a->T; p.rows_on_k = 1; p.split = 0; p.two = two;
+      p.M = cols; p.N = a->H; p.K = a->T; p.group_m = GROUP_GRADS; p.rows_on_k = 1; p.split = 0; p.two = two;
       if (a->dweight_fp32_add) {
         if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
