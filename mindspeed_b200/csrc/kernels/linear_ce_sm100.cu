@@ -36,6 +36,8 @@
 using namespace msb;
 using namespace msb::sm100;
 
+extern "C" int msb_gemm_get_cta_limit();   // gemm_sm100.cu
+
 namespace {
 
 constexpr int BM = 128;          // rows per CTA; the pair covers 256
@@ -1068,6 +1070,12 @@ __global__ void __launch_bounds__(256) lce_dhidden_kernel(const float* acc, cons
     MSB_CHECK_LAUNCH(name);                                    \
   } while (0)
 
+// SMs that the products may take: all, or as many as the caller has left to GEMM-class kernels.
+int product_sms() {
+  const int cap = msb_gemm_get_cta_limit(), sms = msb::num_sms();
+  return cap > 0 && cap < sms ? std::max(cap, 2) : sms;
+}
+
 template <int EPI, bool A_MN, bool B_MN, bool PAIR>
 int launch_gemm_on(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
   using L = Cfg<EPI, PAIR>;
@@ -1076,7 +1084,7 @@ int launch_gemm_on(const LceGemm& p, int most_splits, bool first, cudaStream_t s
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
   const long long items = (long long)((p.M + CTAS * BM - 1) / (CTAS * BM)) * ((p.N + L::TN - 1) / L::TN) * most_splits;
-  const unsigned grid = CTAS * (unsigned)std::min<long long>(items, msb::num_sms() / CTAS);
+  const unsigned grid = CTAS * (unsigned)std::min<long long>(items, product_sms() / CTAS);
   if (first) kern<<<grid, L::THREADS, L::TOTAL, s>>>(p);
   else msb::launch_after(kern, dim3(grid), L::THREADS, L::TOTAL, s, p);
   MSB_CHECK_LAUNCH("lce_gemm");
@@ -1161,7 +1169,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const float inv_tau = 1.f / a->tau, tau2 = a->tau * a->tau;
   const DT* hidden = (const DT*)a->hidden;
   const DT* weight = (const DT*)a->weight;
-  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, a->T <= BM ? msb::num_sms() : msb::num_sms() / 2, a->splits};
+  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, a->T <= BM ? product_sms() : product_sms() / 2, a->splits};
   const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
   if (!scan) {
     if (a->teacher) {

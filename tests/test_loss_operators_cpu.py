@@ -136,6 +136,30 @@ def test_refusals():
             call()
 
 
+def test_first_call_is_not_captured(monkeypatch):
+    from mindspeed_b200.ops import gemm as G
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    monkeypatch.setattr(G, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        M._status(torch.device("cpu"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert M._status(torch.device("cpu")).numel() == 4
+
+
+def test_status_words_name_the_vocabulary(monkeypatch):
+    from mindspeed_b200.ops import gemm as G
+    words = torch.tensor([0, 0x703, 0, 0], dtype=torch.int32)
+    monkeypatch.setattr(G, "_status", {torch.device("cpu"): words})
+    with pytest.raises(RuntimeError, match="outside the vocabulary"):
+        G.check_status()
+    assert not words.any()
+    G.check_status()
+    words[0] = 0x21
+    with pytest.raises(RuntimeError, match="time-out"):
+        G.check_status()
+
+
 def test_no_tokens():
     h, w, lab, idx, a, _ = _inputs()
     for loss in (linear_cross_entropy(h[:0], w, lab[:0]), linear_topk_distillation(h[:0], w, a[:0], idx[:0])):
