@@ -21,8 +21,9 @@
 //           the 16-bit type of the operands (the tensor cores take nothing wider next to them): half a step on each term, as much as the
 //           rounding of the result itself.  With fp16, dz is scaled by a power of two that puts the largest |g| at 2^14 or above, so that
 //           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
-// Few rows: where there are at most 64 or the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them (transposed, [V, rows]: rows are
-//           the lanes of the epilogue), and an elementwise pass makes dz of them: one reading of W less, a quarter of all traffic.
+// Few rows: where there are at most 64, or the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them
+//           (transposed, [V, rows]: rows are the lanes of the epilogue), and an elementwise pass makes dz of them: one reading of W less,
+//           a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 -> 755 us).
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
@@ -95,15 +96,21 @@ struct LceGemm {
   unsigned int* status;
 };
 
-template <int EPI, bool PAIR>
+// HOW a product is tiled: on single CTAs (128 x 256), on pairs (256 x 256, two accumulators that take turns), or on pairs with both
+// accumulators side by side (256 x 512).
+enum How : int { SINGLE = 0, PAIRED = 1, WIDE = 2 };
+constexpr int BN = 256;            // columns of an accumulator
+
+template <int EPI, int HOW>
 struct Cfg {
-  static constexpr int TN = 256;   // columns of a tile (the forward of 96 x 128256 x 4096: 208 us, 223 with 128; one token of 32000 x 1024: 25, 30)
+  static constexpr int CTAS = HOW == SINGLE ? 1 : 2, SUBS = HOW == WIDE ? 2 : 1;
   static constexpr int THREADS = 64 + 32 * (EPI_WARPS + (EPI == EPI_STATS ? GATHER_WARPS : 0));
   // what the staging leaves of 227 KB
-  static constexpr int NSTAGE = !PAIR ? 4 : EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5;
-  static constexpr int A_BYTES = BM * BK * 2;
-  static constexpr int STAGE_BYTES = A_BYTES + (PAIR ? TN / 2 : TN) * BK * 2;
-  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS || !PAIR ? 4096 : 8192;   // 32 rows x 64 columns of the output type; OUT16 has two buffers, OUT32 on single CTAs half a one
+  static constexpr int NSTAGE = HOW != PAIRED ? 4 : EPI == EPI_STATS ? 7 : EPI == EPI_DLOGITS ? 6 : 5;
+  static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN / CTAS * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + SUBS * B_BYTES;
+  // 32 rows x 64 columns of the output type; twice that for OUT16 where there is room (two buffers), half for OUT32 where there is not
+  static constexpr int EPI_BUF = EPI == EPI_STATS ? 0 : EPI == EPI_DLOGITS || HOW != PAIRED ? 4096 : 8192;
   static constexpr int EPI_OFFSET = NSTAGE * STAGE_BYTES;
   static constexpr int BAR_OFFSET = EPI_OFFSET + EPI_WARPS * EPI_BUF;
   static constexpr int TOTAL = BAR_OFFSET + 256 + 1024;
@@ -111,12 +118,12 @@ struct Cfg {
 };
 
 // Work items of a pair (or single CTA): (tile, split of K).  Every role walks its own copy.  Tiles in groups of `group_m` tile rows share panels in L2.
-template <int TILE_M, int BN>
+template <int TILE_M, int TILE_N>
 struct Work {
   int num_m, num_n, num_kb, group_m, splits, item, items, stride;
   int m, n, split, kb0, kb1;
   __device__ Work(int M, int N, int K, int group_m_, int splits_, int pair, int npairs)
-      : num_m((M + TILE_M - 1) / TILE_M), num_n((N + BN - 1) / BN), num_kb((K + BK - 1) / BK), splits(splits_), item(pair),
+      : num_m((M + TILE_M - 1) / TILE_M), num_n((N + TILE_N - 1) / TILE_N), num_kb((K + BK - 1) / BK), splits(splits_), item(pair),
         stride(npairs), m(0), n(0), split(0), kb0(0), kb1(0) {
     group_m = min(group_m_, max(num_m, 1));
     items = num_m * num_n * splits;
@@ -221,12 +228,12 @@ __device__ __forceinline__ void dots_of_row(const LceGemm& p, int i, int k0, int
 
 // EPI_STATS / EPI_DLOGITS: A = hidden [M, K], B = W [N, K].      Hidden gradient: A = dz [M, K], B = W [K, N].
 // Weight gradient: A = dz [K, M], B = hidden [K, N], rows on K.  A_MN tells how dz lies in memory ([tokens, words] or transposed).
-template <int EPI, bool A_MN, bool B_MN, bool PAIR>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, PAIR>::THREADS, 1)
+template <int EPI, bool A_MN, bool B_MN, int HOW>
+__global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(Cfg<EPI, HOW>::THREADS, 1)
     lce_gemm_kernel(const __grid_constant__ LceGemm p) {
-  using L = Cfg<EPI, PAIR>;
-  constexpr int CTAS = PAIR ? 2 : 1, BN = L::TN;
-  constexpr int NSTAGE = L::NSTAGE;
+  using L = Cfg<EPI, HOW>;
+  constexpr bool PAIR = HOW != SINGLE;
+  constexpr int CTAS = L::CTAS, SUBS = L::SUBS, NSTAGE = L::NSTAGE;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // identical in both CTAs of the pair
   const uint32_t bar_base = smem_base + L::BAR_OFFSET;
@@ -273,15 +280,16 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
       const CUtensorMap* mapA = (EPI <= EPI_DLOGITS && packed) ? &p.tmPacked : &p.tmA;
       const CUtensorMap* mapB = (p.rows_on_k && packed) ? &p.tmPacked : &p.tmB;
       int stage = 0; uint32_t phase = 0;
-      Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
+      Work<CTAS * BM, SUBS * BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
       while (alive && w.next()) {
         const int m0 = (w.m * CTAS + (int)cta) * BM;
-        const int n0 = w.n * BN + (int)cta * (BN / 2);
+        const int n0 = w.n * (SUBS * BN) + (int)cta * (BN / 2);
+        const int subs = SUBS == 2 && n0 - (int)cta * (BN / 2) + BN >= p.N ? 1 : SUBS;      // the second half may lie past the last column
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.status, 0x10u)) { alive = false; break; }
           const uint32_t sa = smem_base + stage * L::STAGE_BYTES;
           const uint32_t sb = sa + L::A_BYTES;
-          if (cta == 0) mbar_arrive_expect_tx(full_bar(stage), CTAS * L::STAGE_BYTES);
+          if (cta == 0) mbar_arrive_expect_tx(full_bar(stage), CTAS * (L::A_BYTES + subs * L::B_BYTES));
           const uint32_t lead_full = PAIR ? mapa_u32(full_bar(stage), 0) : full_bar(stage);
           auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
             if (PAIR) tma_load_2d_pair(dst, map, lead_full, x, y);
@@ -294,12 +302,18 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j) load(sa + j * (BK * 128), mapA, m0 + j * 64, k0);   // boxes [64 k x 64 m]
           }
-          if (!B_MN) {
-            load(sb, mapB, k0, n0);                                                    // box [128 rows x 64 k] (256 on a single CTA of the backward)
-          } else {
 #pragma unroll
-            for (int j = 0; j < BN / CTAS / 64; ++j)                                   // boxes [64 k x 64 n]; both terms times the same rows
-              load(sb + j * (BK * 128), mapB, n0 + j * 64, p.rows_on_k && p.two ? 0 : k0);
+          for (int h = 0; h < SUBS; ++h) {
+            if (h >= subs) break;
+            const uint32_t sh = sb + h * L::B_BYTES;
+            const int nh = n0 + h * BN;
+            if (!B_MN) {
+              load(sh, mapB, k0, nh);                                                  // box [128 rows x 64 k] (256 on a single CTA)
+            } else {
+#pragma unroll
+              for (int j = 0; j < BN / CTAS / 64; ++j)                                 // boxes [64 k x 64 n]; both terms times the same rows
+                load(sh + j * (BK * 128), mapB, nh + j * 64, p.rows_on_k && p.two ? 0 : k0);
+            }
           }
           if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
         }
@@ -315,36 +329,87 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
     if (lane == 0 && cta == 0) {
       const uint32_t idesc = make_idesc_f16(CTAS * BM, BN, p.half ? 0 : 1, A_MN ? 1 : 0, B_MN ? 1 : 0);
       int stage = 0; uint32_t phase = 0;
-      int acc = 0; uint32_t acc_phase = 0;
-      Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
-      while (alive && w.next()) {
-        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.status, 0x20u)) { alive = false; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(full_bar(stage), phase, p.status, 0x21u)) { alive = false; break; }
+      Work<CTAS * BM, SUBS * BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
+      if constexpr (SUBS == 1) {
+        int acc = 0; uint32_t acc_phase = 0;
+        while (alive && w.next()) {
+          if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.status, 0x20u)) { alive = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_base + stage * L::STAGE_BYTES;
-          const uint32_t sb = sa + L::A_BYTES;
+          const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+          for (int kb = w.kb0; kb < w.kb1; ++kb) {
+            if (!mbar_wait(full_bar(stage), phase, p.status, 0x21u)) { alive = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_base + stage * L::STAGE_BYTES;
+            const uint32_t sb = sa + L::A_BYTES;
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) {
+              // K-major: advance 16 elements = 32 bytes inside the swizzled row; MN-major: 16 k-rows = 2048 bytes
+              const uint64_t adesc = A_MN ? make_smem_desc(sa + k * (UMMA_K * 128), BK * 128, 1024)
+                                          : make_smem_desc(sa + k * (UMMA_K * 2), 0, 1024);
+              const uint64_t bdesc = B_MN ? make_smem_desc(sb + k * (UMMA_K * 128), BK * 128, 1024)
+                                          : make_smem_desc(sb + k * (UMMA_K * 2), 0, 1024);
+              if (PAIR) umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+              else umma_f16(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            }
+            // both CTAs may refill this stage once these MMAs have read it
+            if (PAIR) umma_commit_pair(empty_bar(stage), 3);
+            else umma_commit(empty_bar(stage));
+            if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
+          }
+          if (!alive) break;
+          if (PAIR) umma_commit_pair(tfull_bar(acc), 3);          // accumulator complete in both CTAs
+          else umma_commit(tfull_bar(acc));
+          if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+      } else {
+        uint32_t turn0 = 0, turn1 = 0;                            // phases of the two accumulators' barriers
+        auto into = [&](int st, int h, uint32_t add) {            // the products of one stage for accumulator h
+          const uint32_t sa = smem_base + st * L::STAGE_BYTES, sb = sa + L::A_BYTES + h * L::B_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k) {
-            // K-major: advance 16 elements = 32 bytes inside the swizzled row; MN-major: 16 k-rows = 2048 bytes
             const uint64_t adesc = A_MN ? make_smem_desc(sa + k * (UMMA_K * 128), BK * 128, 1024)
                                         : make_smem_desc(sa + k * (UMMA_K * 2), 0, 1024);
             const uint64_t bdesc = B_MN ? make_smem_desc(sb + k * (UMMA_K * 128), BK * 128, 1024)
                                         : make_smem_desc(sb + k * (UMMA_K * 2), 0, 1024);
-            if (PAIR) umma_f16_pair(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
-            else umma_f16(d_tmem, adesc, bdesc, idesc, (kb != w.kb0 || k != 0) ? 1u : 0u);
+            umma_f16_pair(tmem_base + h * BN, adesc, bdesc, idesc, k != 0 ? 1u : add);
           }
-          // both CTAs may refill this stage once these MMAs have read it
-          if (PAIR) umma_commit_pair(empty_bar(stage), 3);
-          else umma_commit(empty_bar(stage));
-          if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
+        };
+        while (alive && w.next()) {
+          const bool both = (w.n * SUBS + 1) * BN < p.N;          // else the second half lies past the last column
+          if (!mbar_wait(tempty_bar(0), turn0 ^ 1u, p.status, 0x20u)) { alive = false; break; }
+          tc_fence_after();
+          int kb = w.kb0;
+          if (both) {
+            // the first blocks go into the first accumulator while the epilogue still reads the second; their stages wait for it
+            const int lead = min(NSTAGE - 1, w.kb1 - w.kb0);
+            const int from = stage;
+            for (int i = 0; i < lead; ++i, ++kb) {
+              if (!mbar_wait(full_bar(stage), phase, p.status, 0x21u)) { alive = false; break; }
+              tc_fence_after();
+              into(stage, 0, i != 0 ? 1u : 0u);
+              if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
+            }
+            if (!alive || !mbar_wait(tempty_bar(1), turn1 ^ 1u, p.status, 0x22u)) { alive = false; break; }
+            tc_fence_after();
+            for (int i = 0; i < lead; ++i) {
+              const int st = from + i < NSTAGE ? from + i : from + i - NSTAGE;
+              into(st, 1, i != 0 ? 1u : 0u);
+              umma_commit_pair(empty_bar(st), 3);
+            }
+          }
+          for (; kb < w.kb1; ++kb) {
+            if (!mbar_wait(full_bar(stage), phase, p.status, 0x21u)) { alive = false; break; }
+            tc_fence_after();
+            into(stage, 0, kb != w.kb0 ? 1u : 0u);
+            if (both) into(stage, 1, 1u);
+            umma_commit_pair(empty_bar(stage), 3);
+            if (++stage == NSTAGE) { stage = 0; phase ^= 1u; }
+          }
+          if (!alive) break;
+          umma_commit_pair(tfull_bar(0), 3);                      // (with nothing to sum at once: the epilogue writes zeros)
+          turn0 ^= 1u;
+          if (both) { umma_commit_pair(tfull_bar(1), 3); turn1 ^= 1u; }
         }
-        if (!alive) break;
-        if (PAIR) umma_commit_pair(tfull_bar(acc), 3);          // accumulator complete in both CTAs
-        else umma_commit(tfull_bar(acc));
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
     }
   } else if (EPI == EPI_STATS && warp >= 2 + EPI_WARPS) {
@@ -369,8 +434,8 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
     const float unscale = (EPI >= EPI_OUT16 && p.scale) ? p.scale[1] : 1.f;
     const float ctau = p.tc_inv_tau * LOG2E;
     uint32_t chunk = 0;
-    int acc = 0; uint32_t acc_phase = 0;
-    Work<CTAS * BM, BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
+    int acc = 0; uint32_t turn[2] = {0, 0};
+    Work<CTAS * BM, SUBS * BN> w(M, p.N, K, p.group_m, splits, pair, npairs);
     while (alive && w.next()) {
       const int row0 = (w.m * CTAS + (int)cta) * BM + q * 32, row = row0 + lane;
       float coef = 0.f, lse = 0.f, at_label = 0.f;
@@ -385,163 +450,181 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(Cfg<EPI, 
           at_label = coef == 0.f ? 0.f : (ex2((p.z[row] * p.inv_tau - lse) * LOG2E) - 1.f) * coef;
         }
       }
-      // the first listed word of this row among the warp's columns
-      const long long c0 = (long long)w.n * BN + half * (BN / 2), c1 = min((long long)p.N, c0 + BN / 2);
+      // the first listed word of this row at or behind the warp's first column, for each accumulator
       const unsigned long long* list = nullptr;
-      unsigned long long next = ~0ull;
-      int at_list = 0;
-      if (EPI == EPI_STATS && p.sorted && row < rows) {
-        list = p.sorted + (long long)p.rowmap[row] * p.list;
-        int hi = p.list;
-        while (at_list < hi) {
-          const int mid = (at_list + hi) >> 1;
-          if ((long long)(list[mid] >> 16) < c0) at_list = mid + 1;
-          else hi = mid;
+      int first_listed[SUBS];
+      if (EPI == EPI_STATS && p.sorted) {
+        list = row < rows ? p.sorted + (long long)p.rowmap[row] * p.list : nullptr;
+#pragma unroll
+        for (int h = 0; h < SUBS; ++h) {
+          int lo = 0, hi = list ? p.list : 0;
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((long long)(list[mid] >> 16) < (long long)(w.n * SUBS + h) * BN + half * (BN / 2)) lo = mid + 1;
+            else hi = mid;
+          }
+          first_listed[h] = list ? lo : p.list;
         }
-        if (at_list < p.list) next = list[at_list];
       }
-      if (!mbar_wait_warp(tfull_bar(acc), acc_phase, p.status, 0x30u)) { alive = false; break; }
-      tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
-      if (EPI == EPI_STATS) {
-        // online softmax over this warp's columns of the row; differences are taken before the scaling so that the terms that weigh
-        // most (z near the maximum) keep their bits
-        float m = -INFINITY, s = 0.f;
-        int at = 0;
 #pragma unroll 1
-        for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
-          const int col0 = w.n * BN + c2, left = p.N - col0;
-          if (left <= 0) break;
-          uint32_t rr[64];
-          tmem_ld_32x32(t_row + (uint32_t)c2, rr);
-          tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
-          tmem_ld_wait();
-          if (left < 64) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j >= left) rr[j] = 0xff800000u;          // -inf: columns past the vocabulary
-          }
-          if (p.zt && row < rows) {
-            float* z = p.zt + (long long)col0 * p.ldt + row;
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j < left) z[(long long)j * p.ldt] = __uint_as_float(rr[j]);
-          }
-          float mx[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) mx[u] = __uint_as_float(rr[u]);
-#pragma unroll
-          for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(rr[j]));
-          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (cm > m) {
-#pragma unroll
-            for (int j = 63; j >= 0; --j) at = __uint_as_float(rr[j]) == cm ? c2 - half * (BN / 2) + j : at;
-          }
-          const float mn = fmaxf(m, cm);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          float sm[4] = {s * ex2((m - base) * ctau), 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 64; ++j) sm[j & 3] += ex2((__uint_as_float(rr[j]) - base) * ctau);
-          s = (sm[0] + sm[1]) + (sm[2] + sm[3]);
-          m = mn;
+      for (int sub = 0; sub < SUBS; ++sub) {
+        const int tn = w.n * SUBS + sub;
+        if (SUBS == 2) {
+          if (tn * BN >= p.N) break;                      // the second half lies past the last column
+          acc = sub;
         }
-        if (p.sorted) {
-          for (;;) {
-            const unsigned int hits = __ballot_sync(0xffffffffu, (long long)(next >> 16) < c1);
-            if (!hits) break;
-            const int who = __ffs(hits) - 1;
-            const int col = __shfl_sync(0xffffffffu, (int)((long long)(next >> 16) - (long long)w.n * BN), who);
-            const float z = __uint_as_float(tmem_ld_column(t_row + (uint32_t)col));
-            if (lane == who) {
-              p.listed[(long long)row * p.list + (int)(next & 0xffffu)] = z * (p.tc_inv_tau / p.inv_tau);
-              next = ++at_list < p.list ? list[at_list] : ~0ull;
-            }
-          }
+        const long long c1 = min((long long)p.N, (long long)tn * BN + (half + 1) * (BN / 2));
+        int at_list = 0;
+        unsigned long long next = ~0ull;
+        if (EPI == EPI_STATS && p.sorted) {
+          at_list = SUBS == 2 && sub ? first_listed[SUBS - 1] : first_listed[0];
+          if (at_list < p.list) next = list[at_list];
         }
-        if (row < rows) {
-          const long long o = (long long)(2 * w.n + half) * p.part_ld + row;
-          p.part[o] = make_float2(m, s);
-          p.part_at[o] = (unsigned char)at;
-        }
-      } else {
-        const uint32_t sw = (uint32_t)(lane & 7);
-        const bool empty = w.kb1 == w.kb0;                // nothing to sum: no rows, or more splits than blocks of a short last piece
+        if (!mbar_wait_warp(tfull_bar(acc), turn[acc], p.status, 0x30u)) { alive = false; break; }
+        tc_fence_after();
+        const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+        if (EPI == EPI_STATS) {
+          // online softmax over this warp's columns of the row; differences are taken before the scaling so that the terms that weigh
+          // most (z near the maximum) keep their bits
+          float m = -INFINITY, s = 0.f;
+          int at = 0;
 #pragma unroll 1
-        for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
-          const int col0 = w.n * BN + c2;
-          if (col0 >= p.N) break;                       // the rest of this tile is beyond the last column
-          uint32_t rr[64];
-          tmem_ld_32x32(t_row + (uint32_t)c2, rr);
-          tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
-          tmem_ld_wait();
-          if (EPI == EPI_DLOGITS) {
-            // a row with no gradient writes zeros even where its logits are not finite
+          for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
+            const int col0 = tn * BN + c2, left = p.N - col0;
+            if (left <= 0) break;
+            uint32_t rr[64];
+            tmem_ld_32x32(t_row + (uint32_t)c2, rr);
+            tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
+            tmem_ld_wait();
+            if (left < 64) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              const float e = ex2(fmaf(__uint_as_float(rr[j]), p.tc_inv_tau, -lse) * LOG2E) * coef;
-              rr[j] = __float_as_uint(coef == 0.f ? 0.f : e);
+              for (int j = 0; j < 64; ++j)
+                if (j >= left) rr[j] = 0xff800000u;          // -inf: columns past the vocabulary
             }
-            const long long j0 = label - col0;
-            if (__any_sync(0xffffffffu, j0 >= 0 && j0 < 64)) {
+            if (p.zt && row < rows) {
+              float* z = p.zt + (long long)col0 * p.ldt + row;
 #pragma unroll
-              for (int j = 0; j < 64; ++j) rr[j] = j0 == j ? __float_as_uint(at_label) : rr[j];
+              for (int j = 0; j < 64; ++j)
+                if (j < left) z[(long long)j * p.ldt] = __uint_as_float(rr[j]);
             }
-          } else {
+            float mx[4];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) rr[j] = empty ? 0u : __float_as_uint(__uint_as_float(rr[j]) * unscale);
+            for (int u = 0; u < 4; ++u) mx[u] = __uint_as_float(rr[u]);
+#pragma unroll
+            for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(rr[j]));
+            const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (cm > m) {
+#pragma unroll
+              for (int j = 63; j >= 0; --j) at = __uint_as_float(rr[j]) == cm ? c2 - half * (BN / 2) + j : at;
+            }
+            const float mn = fmaxf(m, cm);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            float sm[4] = {s * ex2((m - base) * ctau), 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sm[j & 3] += ex2((__uint_as_float(rr[j]) - base) * ctau);
+            s = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+            m = mn;
           }
-          const uint32_t sw_row = (uint32_t)lane * 128u;
-          // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box; rows past the last are never read
-          const int y = p.split ? w.split * p.slab_rows + row0 : row0;
-          const bool inside = p.split ? (p.two ? row0 < p.slab_rows && (row0 & (TWO_ROWS - 1)) < rows : row0 < rows) : row0 < p.M;
-          constexpr int BOXES = EPI == EPI_OUT32 ? 2 : 1, TOGETHER = EPI == EPI_OUT32 && PAIR ? 2 : 1;   // boxes of 128-byte rows; in one go
-#pragma unroll
-          for (int b0 = 0; b0 < BOXES; b0 += TOGETHER) {
-            const uint32_t buf = buf_base + (EPI == EPI_OUT16 ? (chunk++ & 1u) * 4096u : 0u);
-            if (lane == 0) tma_store_wait_read<EPI == EPI_OUT16 ? 1 : 0>();   // the store that last read this buffer is done with it
-            __syncwarp();
-#pragma unroll
-            for (int b = b0; b < b0 + TOGETHER; ++b) {
-              const uint32_t row_addr = buf + (uint32_t)(b - b0) * 4096u + sw_row;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {                 // 16-byte chunk j of the row: eight 16-bit or four 32-bit columns
-                uint32_t v[4];
-                if (EPI == EPI_OUT32) {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) v[e] = rr[32 * b + 4 * j + e];
-                } else {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) v[e] = pack16(__uint_as_float(rr[8 * j + 2 * e]), __uint_as_float(rr[8 * j + 2 * e + 1]), p.half);
-                }
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + ((((uint32_t)j) ^ sw) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                             "r"(v[3])
-                             : "memory");
+          if (p.sorted) {
+            for (;;) {
+              const unsigned int hits = __ballot_sync(0xffffffffu, (long long)(next >> 16) < c1);
+              if (!hits) break;
+              const int who = __ffs(hits) - 1;
+              const int col = __shfl_sync(0xffffffffu, (int)((long long)(next >> 16) - (long long)tn * BN), who);
+              const float z = __uint_as_float(tmem_ld_column(t_row + (uint32_t)col));
+              if (lane == who) {
+                p.listed[(long long)row * p.list + (int)(next & 0xffffu)] = z * (p.tc_inv_tau / p.inv_tau);
+                next = ++at_list < p.list ? list[at_list] : ~0ull;
               }
             }
-            fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
-            __syncwarp();
-            if (lane == 0) {
+          }
+          if (row < rows) {
+            const long long o = (long long)(2 * tn + half) * p.part_ld + row;
+            p.part[o] = make_float2(m, s);
+            p.part_at[o] = (unsigned char)at;
+          }
+        } else {
+          const uint32_t sw = (uint32_t)(lane & 7);
+          const bool empty = w.kb1 == w.kb0;                // nothing to sum: no rows, or more splits than blocks of a short last piece
+#pragma unroll 1
+          for (int c2 = half * (BN / 2); c2 < (half + 1) * (BN / 2); c2 += 64) {
+            const int col0 = tn * BN + c2;
+            if (col0 >= p.N) break;                       // the rest of this tile is beyond the last column
+            uint32_t rr[64];
+            tmem_ld_32x32(t_row + (uint32_t)c2, rr);
+            tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
+            tmem_ld_wait();
+            if (EPI == EPI_DLOGITS) {
+              // a row with no gradient writes zeros even where its logits are not finite
+#pragma unroll
+              for (int j = 0; j < 64; ++j) {
+                const float e = ex2(fmaf(__uint_as_float(rr[j]), p.tc_inv_tau, -lse) * LOG2E) * coef;
+                rr[j] = __float_as_uint(coef == 0.f ? 0.f : e);
+              }
+              const long long j0 = label - col0;
+              if (__any_sync(0xffffffffu, j0 >= 0 && j0 < 64)) {
+#pragma unroll
+                for (int j = 0; j < 64; ++j) rr[j] = j0 == j ? __float_as_uint(at_label) : rr[j];
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) rr[j] = empty ? 0u : __float_as_uint(__uint_as_float(rr[j]) * unscale);
+            }
+            const uint32_t sw_row = (uint32_t)lane * 128u;
+            // hidden gradient: slabs of `slab_rows` rows, a multiple of the 32 rows of a box; rows past the last are never read
+            const int y = p.split ? w.split * p.slab_rows + row0 : row0;
+            const bool inside = p.split ? (p.two ? row0 < p.slab_rows && (row0 & (TWO_ROWS - 1)) < rows : row0 < rows) : row0 < p.M;
+            constexpr int BOXES = EPI == EPI_OUT32 ? 2 : 1, TOGETHER = EPI == EPI_OUT32 && L::EPI_BUF == 8192 ? 2 : 1;   // boxes of 128-byte rows; in one go
+#pragma unroll
+            for (int b0 = 0; b0 < BOXES; b0 += TOGETHER) {
+              constexpr bool TURNS = EPI == EPI_OUT16 && L::EPI_BUF == 8192;
+              const uint32_t buf = buf_base + (TURNS ? (chunk++ & 1u) * 4096u : 0u);
+              if (lane == 0) tma_store_wait_read<TURNS ? 1 : 0>();   // the store that last read this buffer is done with it
+              __syncwarp();
 #pragma unroll
               for (int b = b0; b < b0 + TOGETHER; ++b) {
-                const int x = col0 + 32 * b;
-                const uint32_t src = buf + (uint32_t)(b - b0) * 4096u;
-                if (inside && x < p.N) {
-                  if (EPI == EPI_OUT32 && p.accumulate) tma_reduce_add_2d(&p.tmD, src, x, y);
-                  else tma_store_2d(&p.tmD, src, x, y);
+                const uint32_t row_addr = buf + (uint32_t)(b - b0) * 4096u + sw_row;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {                 // 16-byte chunk j of the row: eight 16-bit or four 32-bit columns
+                  uint32_t v[4];
+                  if (EPI == EPI_OUT32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = rr[32 * b + 4 * j + e];
+                  } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = pack16(__uint_as_float(rr[8 * j + 2 * e]), __uint_as_float(rr[8 * j + 2 * e + 1]), p.half);
+                  }
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + ((((uint32_t)j) ^ sw) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                               "r"(v[3])
+                               : "memory");
                 }
               }
-              tma_store_commit();
+              fence_proxy_async_smem();                       // generic-proxy writes -> visible to the TMA store
+              __syncwarp();
+              if (lane == 0) {
+#pragma unroll
+                for (int b = b0; b < b0 + TOGETHER; ++b) {
+                  const int x = col0 + 32 * b;
+                  const uint32_t src = buf + (uint32_t)(b - b0) * 4096u;
+                  if (inside && x < p.N) {
+                    if (EPI == EPI_OUT32 && p.accumulate) tma_reduce_add_2d(&p.tmD, src, x, y);
+                    else tma_store_2d(&p.tmD, src, x, y);
+                  }
+                }
+                tma_store_commit();
+              }
             }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {                                       // this warp has read its part of the accumulator
+          if (PAIR) mbar_arrive_remote(lead_tempty[acc]);
+          else mbar_arrive(lead_tempty[acc]);
+        }
+        turn[acc] ^= 1u;
+        if (SUBS == 1) acc ^= 1;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {                                       // this warp has read its part of the accumulator
-        if (PAIR) mbar_arrive_remote(lead_tempty[acc]);
-        else mbar_arrive(lead_tempty[acc]);
-      }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) tma_store_wait<0>();                 // staging buffers are read and the stores are complete before exit
   }
@@ -573,13 +656,14 @@ __device__ __forceinline__ int list_kind(const long long* idx, const float* teac
 
 // K splits of the hidden gradient, for `n` rows.  Its tiles (256 rows x 256 of H) are few where there are few rows, or fill the last round of
 // the SM pairs badly; split along the vocabulary every pair gets a part, at the price of writing and adding more results.  Times in us: a
-// block of 64 words takes a tile 0.37, its read-out 2; the slabs move at 6 TB/s.  One warp; all lanes get the result.
-__device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs, int most, int lane) {
-  const int tiles = max(1, (n + 255) / 256 * ((H + 255) / 256));
+// block of 64 words takes a tile 0.40 (0.72 a wide one, subs = 2), its read-out 2; the slabs move at 6 TB/s.  One warp; all lanes get the result.
+__device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs, int most, int subs, int lane) {
+  const int tiles = max(1, (n + 255) / 256 * ((H + 256 * subs - 1) / (256 * subs)));
   float best_t = INFINITY;
   int best = 1;
   for (int s = lane + 1; s <= most; s += 32) {
-    const float t = (float)((tiles * s + pairs - 1) / pairs) * ((float)((blocks + s - 1) / s) * 0.37f + 2.f) + (float)s * n * H * (8.f / 6e6f);
+    const float tile = (float)((blocks + s - 1) / s) * (subs == 2 ? 0.72f : 0.40f) + 2.f;
+    const float t = (float)((tiles * s + pairs - 1) / pairs) * tile + (float)s * n * H * (8.f / 6e6f);
     if (t < best_t) { best_t = t; best = s; }
   }
   for (int o = 16; o > 0; o >>= 1) {
@@ -590,7 +674,7 @@ __device__ __forceinline__ int choose_splits(int n, int H, int blocks, int pairs
   return best;
 }
 
-struct Splits { int blocks, pairs, most; };        // blocks of 64 words, SM pairs (or SMs) that take the tiles, most splits
+struct Splits { int blocks, pairs, most, subs; };        // blocks of 64 words, SM pairs (or SMs) that take the tiles, most splits
 
 // One warp a token: what its list says, and the words of this rank sorted with their places (bitonic, `padded` = K up to a power of two);
 // the rest of the places behind them as all ones.
@@ -678,7 +762,7 @@ __global__ void __launch_bounds__(1024) lce_scan_kernel(const long long* __restr
     }
   }
   if (warp == 0) {
-    const int s = choose_splits(base, H, sp.blocks, sp.pairs, sp.most, lane);
+    const int s = choose_splits(base, H, sp.blocks, sp.pairs, sp.most, sp.subs, lane);
     if (lane == 0) { count[0] = base; count[1] = s; }
   }
 }
@@ -736,7 +820,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const uint4* __restrict__
         }
       }
       if (warp == 0) {
-        const int s = choose_splits(n, H, sp.blocks, sp.pairs, sp.most, lane);
+        const int s = choose_splits(n, H, sp.blocks, sp.pairs, sp.most, sp.subs, lane);
         if (lane == 0) { count[0] = n; count[1] = s; }
       }
     }
@@ -1076,27 +1160,47 @@ int product_sms() {
   return cap > 0 && cap < sms ? std::max(cap, 2) : sms;
 }
 
-template <int EPI, bool A_MN, bool B_MN, bool PAIR>
+template <int EPI, bool A_MN, bool B_MN, int HOW>
 int launch_gemm_on(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
-  using L = Cfg<EPI, PAIR>;
-  constexpr int CTAS = PAIR ? 2 : 1;
-  auto kern = lce_gemm_kernel<EPI, A_MN, B_MN, PAIR>;
+  using L = Cfg<EPI, HOW>;
+  auto kern = lce_gemm_kernel<EPI, A_MN, B_MN, HOW>;
   static std::atomic<unsigned long long> stated{0};
   if (int bad = msb::allow_smem((const void*)kern, L::TOTAL, "lce_gemm", stated)) return bad;
-  const long long items = (long long)((p.M + CTAS * BM - 1) / (CTAS * BM)) * ((p.N + L::TN - 1) / L::TN) * most_splits;
-  const unsigned grid = CTAS * (unsigned)std::min<long long>(items, product_sms() / CTAS);
+  const long long items = (long long)((p.M + L::CTAS * BM - 1) / (L::CTAS * BM)) * ((p.N + L::SUBS * BN - 1) / (L::SUBS * BN)) * most_splits;
+  const unsigned grid = L::CTAS * (unsigned)std::min<long long>(items, product_sms() / L::CTAS);
   if (first) kern<<<grid, L::THREADS, L::TOTAL, s>>>(p);
   else msb::launch_after(kern, dim3(grid), L::THREADS, L::TOTAL, s, p);
   MSB_CHECK_LAUNCH("lce_gemm");
   return 0;
 }
-// Single CTAs for up to 128 output rows (see the top of the file); the weight gradient's output rows are words.
 template <int EPI, bool A_MN, bool B_MN>
-int launch_gemm(const LceGemm& p, int most_splits, bool first, cudaStream_t s) {
-  if (EPI != EPI_OUT16 && !p.rows_on_k && p.M <= BM)
-    return launch_gemm_on<EPI, A_MN, B_MN, EPI == EPI_OUT16>(p, most_splits, first, s);
-  return launch_gemm_on<EPI, A_MN, B_MN, true>(p, most_splits, first, s);
+int launch_gemm(const LceGemm& p, How how, int most_splits, bool first, cudaStream_t s) {
+  if constexpr (EPI != EPI_OUT16)
+    if (how == SINGLE) return launch_gemm_on<EPI, A_MN, B_MN, SINGLE>(p, most_splits, first, s);
+  if (how == WIDE) return launch_gemm_on<EPI, A_MN, B_MN, WIDE>(p, most_splits, first, s);
+  return launch_gemm_on<EPI, A_MN, B_MN, PAIRED>(p, most_splits, first, s);
 }
+
+// How a product of M x N with sums over K is tiled: by its modelled time in us, rounds of tiles over the SM pairs.  A block of 64 of the
+// sum takes a pair 0.40 on 256 x 256 and 0.72 on 256 x 512 (A is staged once for both halves: shared memory, whose bandwidth bounds the
+// former, moves a quarter less, and so do L2 and the power it takes), but nothing hides the read-out of the wide tile, 2.  `rows` of at
+// most 128 take single CTAs.  (In turn on one GPU at its power limit, 8192 x 128256 x 4096: forward 6.63 -> 6.45 ms, backward 20.3 -> 19.4;
+// 1500 x 60000 x 1024, where the rule keeps pairs: forward 190, 193 wide.)  The rule counts all tokens: how many stay is not known here.
+float modelled_us(long long M, long long N, long long K, int splits, How how) {
+  const int pairs = std::max(1, product_sms() / 2), width = how == WIDE ? 512 : 256;
+  const long long tiles = ((M + 255) / 256) * ((N + width - 1) / width) * splits, blocks = ((K + BK - 1) / BK + splits - 1) / splits;
+  return (float)((tiles + pairs - 1) / pairs) * (how == WIDE ? 0.72f * blocks + 2.f : 0.40f * blocks);
+}
+How choose_how(long long M, long long N, long long K, int most_splits = 1) {
+  float best[2] = {INFINITY, INFINITY};
+  for (int s = 1; s <= most_splits; ++s) {
+    best[0] = std::min(best[0], modelled_us(M, N, K, s, PAIRED));
+    best[1] = std::min(best[1], modelled_us(M, N, K, s, WIDE));
+  }
+  return best[1] < best[0] ? WIDE : PAIRED;
+}
+How rows_how(int rows, long long N, long long K, int most_splits = 1) { return rows <= BM ? SINGLE : choose_how(rows, N, K, most_splits); }
+
 // Rows of the boxes that load W as [words, H], for T tokens.
 uint32_t words_box(int T) { return T <= BM ? 256 : 128; }
 
@@ -1151,6 +1255,9 @@ struct MsbLceArgs {
   unsigned int* status;        // [0] expired waits, [1] words outside the vocabulary
 };
 
+// Tiles of the hidden gradient (both directions ask: the forward counts its splits).
+static How dhidden_how(const MsbLceArgs* a) { return rows_how(a->T, a->H, std::min(a->piece, a->V), a->splits); }
+
 static int lce_check(const MsbLceArgs* a) {
   MSB_REQUIRE(a->T > 0 && a->H > 0 && a->V > 0 && a->K > 0, "linear_ce: empty problem T=%d H=%d V=%d K=%d", a->T, a->H, a->V, a->K);
   MSB_REQUIRE(a->dtype == MSB_BF16 || a->dtype == MSB_F16, "linear_ce: dtype code %d is not bf16 or fp16", a->dtype);
@@ -1169,7 +1276,8 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   const float inv_tau = 1.f / a->tau, tau2 = a->tau * a->tau;
   const DT* hidden = (const DT*)a->hidden;
   const DT* weight = (const DT*)a->weight;
-  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, a->T <= BM ? product_sms() : product_sms() / 2, a->splits};
+  const Splits sp = {(std::min(a->piece, a->V) + BK - 1) / BK, a->T <= BM ? product_sms() : product_sms() / 2, a->splits,
+                     dhidden_how(a) == WIDE ? 2 : 1};
   const bool scan = a->T <= SCAN_MOST && a->K <= SCAN_LIST;
   if (!scan) {
     if (a->teacher) {
@@ -1213,7 +1321,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.rowmap = a->rowmap;
   p.inv_tau = inv_tau; p.tc_inv_tau = tc_scale(inv_tau, a->H);
   p.status = a->status;
-  if ((rc = launch_gemm<EPI_STATS, false, false>(p, 1, false, s))) return rc;
+  if ((rc = launch_gemm<EPI_STATS, false, false>(p, rows_how(a->T, a->V, a->H), 1, false, s))) return rc;
   constexpr int width = 128;
 #define LCE_JOIN(R, S)                                                                                                                       \
   LCE_AFTER("lce_join", (lce_join_kernel<DT, R, S>), (a->T + R - 1) / R, R * S, 0, p.part, p.part_at, p.part_ld, (a->V + width - 1) / width, width, hidden, \
@@ -1290,7 +1398,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, words_box(a->T), BK))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, dz, dt, 2, a->T, cols, a->ldz, 32, 64))) return rc;
       p.M = a->T; p.N = cols; p.K = a->H; p.group_m = GROUP_LOGITS; p.rows_on_k = 0; p.split = 0; p.two = 0; p.piece_start = a->vocab_start + v0;
-      if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, 1, v0 == 0 && !a->scale, s))) return rc;
+      if ((rc = launch_gemm<EPI_DLOGITS, false, false>(p, rows_how(a->T, cols, a->H), 1, v0 == 0 && !a->scale, s))) return rc;
     }
     if (a->teacher) {
       const long long places = (long long)a->T * a->K;
@@ -1304,8 +1412,10 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
-      p.M = dz_rows; p.N = a->H; p.K = cols; p.group_m = GROUP_GRADS; p.rows_on_k = 0; p.split = 1; p.two = two; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
-      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, a->splits, false, s) : launch_gemm<EPI_OUT32, false, true>(p, a->splits, false, s);
+      p.M = dz_rows; p.N = a->H; p.K = cols; p.group_m = GROUP_GRADS; p.rows_on_k = 0; p.two = two;
+      p.split = 1; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
+      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, dhidden_how(a), a->splits, false, s)
+                 : launch_gemm<EPI_OUT32, false, true>(p, dhidden_how(a), a->splits, false, s);
       if (rc) return rc;
     }
     if (a->dweight) {
@@ -1315,14 +1425,15 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if ((rc = make_tmap_2d(&p.tmB, a->hidden, dt, 2, a->T, a->H, a->ldh, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmPacked, a->packed, dt, 2, a->T, a->H, a->H, BK, 64))) return rc;
       p.M = cols; p.N = a->H; p.K = a->T; p.group_m = GROUP_GRADS; p.rows_on_k = 1; p.split = 0; p.two = two;
+      const How how = choose_how(cols, a->H, a->T);
       if (a->dweight_fp32_add) {
         if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
-        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, 1, false, s) : launch_gemm<EPI_OUT32, true, true>(p, 1, false, s);
+        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT32, true, true>(p, how, 1, false, s);
       } else {
         if ((rc = make_tmap_2d(&p.tmD, (DT*)a->dweight + v0 * a->H, dt, 2, cols, a->H, a->H, 32, 64))) return rc;
         p.accumulate = 0;
-        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, 1, false, s) : launch_gemm<EPI_OUT16, true, true>(p, 1, false, s);
+        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT16, true, true>(p, how, 1, false, s);
       }
       if (rc) return rc;
     }
@@ -1344,7 +1455,8 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
 MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   if (int rc = lce_check(a)) return rc;
   MSB_REQUIRE(a->zt || (a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V)), "linear_ce: pitch %lld of a piece of %d columns", a->ldz, a->piece);
-  MSB_REQUIRE(!a->acc || (a->slab_rows >= (a->zt && a->T <= TWO_ROWS ? 2 * TWO_ROWS : a->T) && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
+  const int dz_rows = a->zt && a->T <= TWO_ROWS ? 2 * TWO_ROWS : a->T;
+  MSB_REQUIRE(!a->acc || (a->slab_rows >= dz_rows && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
               "linear_ce: %d slabs of %d rows", a->splits, a->slab_rows);
   return a->dtype == MSB_F16 ? lce_backward<__half>(a, s) : lce_backward<__nv_bfloat16>(a, s);
 }
