@@ -9,6 +9,7 @@
   python -m mindspeed_b200.benchmarks.ncu_targets fp8_wgrad   # 2 launches of the fp8 GEMM with row-wise scales on both sides
   python -m mindspeed_b200.benchmarks.ncu_targets grouped     # grouped expert GEMMs, 64 experts of about 384 rows: fwd / dgrad / wgrad
   python -m mindspeed_b200.benchmarks.ncu_targets mla_heads   # latent-attention head kernels, forward and backward
+  python -m mindspeed_b200.benchmarks.ncu_targets losses      # output projection with cross entropy (4096 and 96 rows), router balance loss
 
 Inputs exceed the 126 MB L2 but stay well under 2 GB on the device; there are only a handful of launches, so a
 ``--set full`` capture ends by itself within a minute or two.
@@ -161,6 +162,21 @@ def mla_heads():
     torch.cuda.synchronize()
 
 
+def losses():
+    from ..ops import gemm as G
+    from ..ops.balance_loss import router_balance_loss
+    from ..ops.linear_cross_entropy import linear_cross_entropy
+    for rows, vocab, hidden in ((4096, 32000, 4096), (96, 65536, 4096)):
+        h = torch.randn(rows, hidden, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        w = (torch.randn(vocab, hidden, device="cuda") * 0.02).to(torch.bfloat16).requires_grad_(True)
+        linear_cross_entropy(h, w, torch.randint(0, vocab, (rows,), device="cuda")).mean().backward()
+    x = torch.randn(65536, 256, device="cuda", requires_grad=True)
+    rmap = torch.zeros(65536, 256, dtype=torch.bool, device="cuda").scatter_(1, x.detach().topk(8, 1)[1], True)
+    router_balance_loss(x, rmap, 8, 0.01)[0].backward()
+    torch.cuda.synchronize()
+    G.check_status()
+
+
 if __name__ == "__main__":
     {"gemm": gemm, "elementwise": elementwise, "fp8": fp8, "gemm_tp8": gemm_tp8, "flash": flash, "quant": quant, "fp8_wgrad": fp8_wgrad,
-     "grouped": grouped, "mla_heads": mla_heads}[sys.argv[1] if len(sys.argv) > 1 else "gemm"]()
+     "grouped": grouped, "mla_heads": mla_heads, "losses": losses}[sys.argv[1] if len(sys.argv) > 1 else "gemm"]()

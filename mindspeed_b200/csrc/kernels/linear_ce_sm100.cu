@@ -483,6 +483,17 @@ __global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(
         if (!mbar_wait_warp(tfull_bar(acc), turn[acc], p.status, 0x30u)) { alive = false; break; }
         tc_fence_after();
         const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+        // gives this warp's part of the accumulator back: as soon as the last of it is in registers
+        bool held = true;
+        auto hand_back = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_remote(lead_tempty[acc]);
+            else mbar_arrive(lead_tempty[acc]);
+          }
+          held = false;
+        };
         if (EPI == EPI_STATS) {
           // online softmax over this warp's columns of the row; differences are taken before the scaling so that the terms that weigh
           // most (z near the maximum) keep their bits
@@ -496,6 +507,7 @@ __global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(
             tmem_ld_32x32(t_row + (uint32_t)c2, rr);
             tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
             tmem_ld_wait();
+            if (!p.sorted && (c2 & 64)) hand_back();
             if (left < 64) {
 #pragma unroll
               for (int j = 0; j < 64; ++j)
@@ -554,6 +566,7 @@ __global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(
             tmem_ld_32x32(t_row + (uint32_t)c2, rr);
             tmem_ld_32x32(t_row + (uint32_t)(c2 + 32), rr + 32);
             tmem_ld_wait();
+            if (c2 & 64) hand_back();
             if (EPI == EPI_DLOGITS) {
               // a row with no gradient writes zeros even where its logits are not finite
 #pragma unroll
@@ -616,12 +629,7 @@ __global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {                                       // this warp has read its part of the accumulator
-          if (PAIR) mbar_arrive_remote(lead_tempty[acc]);
-          else mbar_arrive(lead_tempty[acc]);
-        }
+        if (held) hand_back();
         turn[acc] ^= 1u;
         if (SUBS == 1) acc ^= 1;
       }
