@@ -74,17 +74,26 @@ def _model(fused, score, kind):
 
 @pytest.fixture(scope="module")
 def one_rank():
-    import os
+    """A process group of this process alone, gone again (and nothing left in the environment) when the module's tests end."""
+    import socket
     import torch.distributed as dist
     from mindspeed_b200.parallel import parallel_state as ps
     from mindspeed_b200.parallel.random import model_parallel_cuda_manual_seed
-    if not dist.is_initialized():
-        os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT="29571", RANK="0", WORLD_SIZE="1")
-        dist.init_process_group("nccl", rank=0, world_size=1)
-    if not ps.model_parallel_is_initialized():
+    mine = not dist.is_initialized()
+    if mine:
+        with socket.socket() as s:
+            s.bind(("127.0.0.1", 0))
+            port = s.getsockname()[1]
+        dist.init_process_group("nccl", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1)
+    parallel = not ps.model_parallel_is_initialized()
+    if parallel:
         ps.initialize_model_parallel()
     model_parallel_cuda_manual_seed(1)
     yield
+    if parallel:
+        ps.destroy_model_parallel()
+    if mine:
+        dist.destroy_process_group()
 
 
 @pytest.mark.parametrize("score,kind", [("softmax", "aux_loss"), ("sigmoid", "seq_aux_loss")])
