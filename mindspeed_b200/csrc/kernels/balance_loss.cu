@@ -7,12 +7,14 @@
 //   dx_e = g C s_e (1 - s_e) / n (f_e - sum p f)     sigmoid, n the normaliser
 // Token t belongs to sequence t mod B ([s, b] order); the loss over the whole batch is B = 1.
 //
-// Bound by the memory rate (logits and map read once, gradient written once) or, for short batches, by the launches: two forward, one
-// backward.  A row lives in the registers of 1 to 32 lanes (VEC experts a load, NJ loads), so a warp takes up to 32 rows at once; the
+// Bound by the memory rate (logits and map read once, gradient written once) or, for short batches, by the launches: one each way, two
+// forward for long ones.  A row lives in the registers of 1 to 32 lanes (VEC experts a load, NJ loads), so a warp takes up to 32 rows at once; the
 // sums over tokens stay in registers until the block ends and are joined in a fixed order: the same bits on every run.
 #include "msb_common.cuh"
+#include "msb_sm100.cuh"
 #include <algorithm>
 using namespace msb;
+using namespace msb::sm100;
 
 namespace {
 
@@ -92,24 +94,17 @@ __device__ __forceinline__ void scores(float* x, float* slope, int lanes) {
   }
 }
 
-// grid (blocks, B): partial sums of p and counts of the block's tokens.  `lanes` lanes a row; expert of (lane l, load j, element v) is
-// (l + lanes j) VEC + v.
+// Sums of p and counts of one sequence over the rows of warp `wid` of `warps`; every lane has its experts' of the whole warp.  `lanes` lanes
+// a row; expert of (lane l, load j, element v) is (l + lanes j) VEC + v.
 template <typename T, int VEC, int NJ, bool SIGMOID>
-__global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S,
-                                                                 int B, int E, int lanes, float* __restrict__ psum, int* __restrict__ csum,
-                                                                 unsigned int* __restrict__ ticket) {
-  after_previous();
-  extern __shared__ float sh[];                 // [WARPS][E]
+__device__ __forceinline__ void sum_rows(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S, int B, int E, int lanes,
+                                         int seq, int wid, int warps, float* P, int* c) {
   constexpr int N = NJ * VEC;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (lanes - 1), sub = lane / lanes, rows_per_warp = 32 / lanes;
-  const int seq = blockIdx.y;
-  if (blockIdx.x == 0 && seq == 0 && threadIdx.x == 0) *ticket = 0;
-  float P[N];
-  int c[N];
+  const int lane = threadIdx.x & 31, l = lane & (lanes - 1), sub = lane / lanes, rows_per_warp = 32 / lanes;
 #pragma unroll
   for (int i = 0; i < N; ++i) { P[i] = 0.f; c[i] = 0; }
-  const long long stride = (long long)gridDim.x * WARPS * rows_per_warp;
-  // the next rows are loaded while these are summed (for wide rows only: two rows of more than 32 experts a lane do not fit the registers)
+  const long long stride = (long long)warps * rows_per_warp;
+  // the next rows are loaded while these are summed (not for wide rows: two rows of more than 16 experts a lane do not fit the registers)
   constexpr int AHEAD = N <= 16 ? 2 : 1;
   float x[AHEAD][N];
   uint32_t m[AHEAD][NJ];
@@ -127,7 +122,7 @@ __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __res
       }
     }
   };
-  long long r0 = ((long long)blockIdx.x * WARPS + warp) * rows_per_warp;
+  long long r0 = (long long)wid * rows_per_warp;
   if (AHEAD == 2 && r0 < S) fetch(r0, x[0], m[0]);
   for (; r0 < S; r0 += stride) {
     if (AHEAD == 2) fetch(r0 + stride, x[AHEAD - 1], m[AHEAD - 1]);
@@ -154,9 +149,16 @@ __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __res
       P[i] += __shfl_xor_sync(0xffffffffu, P[i], o);
       c[i] += __shfl_xor_sync(0xffffffffu, c[i], o);
     }
-  const long long out = ((long long)seq * gridDim.x + blockIdx.x) * E;
+}
+
+// Joins the warps of a block in a fixed order: `take(e, P, c)` for each expert.  sh: [warps][E] floats.
+template <int VEC, int NJ, typename Take>
+__device__ __forceinline__ void join_warps(float* sh, const float* P, const int* c, int warps, int E, int lanes, Take take) {
+  constexpr int N = NJ * VEC;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (lanes - 1), sub = lane / lanes;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
+    __syncthreads();                              // what was in `sh` has been read
     if (sub == 0)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -164,19 +166,96 @@ __global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __res
         if (e < E) sh[warp * E + e] = pass ? __int_as_float(c[i]) : P[i];
       }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += WARPS * 32) {
-      if (pass) {
-        int t = 0;
-        for (int w = 0; w < WARPS; ++w) t += __float_as_int(sh[w * E + e]);
-        csum[out + e] = t;
-      } else {
-        float t = 0.f;
-        for (int w = 0; w < WARPS; ++w) t += sh[w * E + e];
-        psum[out + e] = t;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+      float p = 0.f;
+      int n = 0;
+      for (int w = 0; w < warps; ++w) {
+        if (pass) n += __float_as_int(sh[w * E + e]);
+        else p += sh[w * E + e];
       }
+      take(e, pass, p, n);
     }
-    __syncthreads();
   }
+}
+
+// grid (blocks, B): partial sums of p and counts of the block's tokens.
+template <typename T, int VEC, int NJ, bool SIGMOID>
+__global__ void __launch_bounds__(WARPS * 32) balance_sums_kernel(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S,
+                                                                 int B, int E, int lanes, float* psum, int* csum, unsigned int* ticket) {
+  after_previous();
+  extern __shared__ float sh[];                 // [WARPS][E]
+  const int seq = blockIdx.y;
+  if (blockIdx.x == 0 && seq == 0 && threadIdx.x == 0) *ticket = 0;
+  float P[NJ * VEC];
+  int c[NJ * VEC];
+  sum_rows<T, VEC, NJ, SIGMOID>(logits, map, S, B, E, lanes, seq, blockIdx.x * WARPS + (threadIdx.x >> 5), gridDim.x * WARPS, P, c);
+  const long long out = ((long long)seq * gridDim.x + blockIdx.x) * E;
+  join_warps<VEC, NJ>(sh, P, c, WARPS, E, lanes, [&](int e, int pass, float p, int n) {
+    if (pass) csum[out + e] = n;
+    else psum[out + e] = p;
+  });
+}
+
+// The whole forward of a short batch in one launch: one cluster of eight CTAs, whose sums meet in distributed shared memory.  (Such calls are
+// bound by the host, for which a launch is 5 us.)
+constexpr int CLUSTER = 8, SMALL_WARPS = 16, SMALL_EXPERTS = 512, SMALL_CELLS = 1024;   // cells: sequences x experts
+constexpr long long SMALL_ELEMENTS = 1 << 19;
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+template <typename T, int VEC, int NJ, bool SIGMOID>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SMALL_WARPS * 32)
+    balance_small_kernel(const T* __restrict__ logits, const unsigned char* __restrict__ map, int S, int B, int E, int lanes, float scale,
+                         float* load, float* loss, long long* counts) {
+  extern __shared__ float sh[];                 // [SMALL_WARPS][E]
+  __shared__ float ps[SMALL_CELLS];
+  __shared__ int cs[SMALL_CELLS];
+  __shared__ float red[32], mine;
+  const uint32_t rank = cluster_ctarank();
+  for (int seq = 0; seq < B; ++seq) {
+    float P[NJ * VEC];
+    int c[NJ * VEC];
+    sum_rows<T, VEC, NJ, SIGMOID>(logits, map, S, B, E, lanes, seq, (int)rank * SMALL_WARPS + (threadIdx.x >> 5), CLUSTER * SMALL_WARPS, P, c);
+    join_warps<VEC, NJ>(sh, P, c, SMALL_WARPS, E, lanes, [&](int e, int pass, float p, int n) {
+      if (pass) cs[seq * E + e] = n;
+      else ps[seq * E + e] = p;
+    });
+  }
+  __syncwarp();
+  cluster_sync_all();
+  // each CTA joins a share of the experts
+  const int each = (E + CLUSTER - 1) / CLUSTER, mine_e = (int)rank * each + (int)threadIdx.x;
+  const bool owner = (int)threadIdx.x < each && mine_e < E;
+  float products = 0.f;
+  long long tokens = 0;
+  if (owner)
+    for (int seq = 0; seq < B; ++seq) {
+      const int cell = seq * E + mine_e;
+      float p = 0.f;
+      int n = 0;
+#pragma unroll
+      for (uint32_t r = 0; r < CLUSTER; ++r) {
+        p += __uint_as_float(ld_cluster(mapa_u32(smem_u32(ps + cell), r)));
+        n += (int)ld_cluster(mapa_u32(smem_u32(cs + cell), r));
+      }
+      load[cell] = (float)n;
+      products += p * (float)n;
+      tokens += n;
+    }
+  if (owner) counts[mine_e] = tokens;
+  products = block_sum(products, red);
+  if (threadIdx.x == 0) mine = products;
+  __syncwarp();
+  cluster_sync_all();
+  if (rank == 0 && threadIdx.x == 0) {
+    float s = 0.f;
+    for (uint32_t r = 0; r < CLUSTER; ++r) s += __uint_as_float(ld_cluster(mapa_u32(smem_u32(&mine), r)));
+    *loss = s * scale;
+  }
+  __syncwarp();
+  cluster_sync_all();                           // no CTA leaves while its shared memory is read
 }
 
 // grid (ceil(E / 32), B), 32 experts x 32 slices of the blocks: loads f, the products' sum; the last block to end adds those in order and
@@ -313,10 +392,8 @@ int bal_check(int S, int B, int E) {
   return 0;
 }
 
-}  // namespace
-
-// Blocks a sequence that both directions launch, and that the forward's scratch is sized by ([B, blocks, E] floats and ints).
-MSB_API int msb_balance_blocks(int S, int B, int E) {
+// blocks a sequence
+int balance_grid(int S, int B, int E) {
   const int units = E % 4 == 0 ? E / 4 : E;
   int lanes = 32;
   while (lanes > 1 && lanes / 2 >= units) lanes /= 2;
@@ -326,12 +403,30 @@ MSB_API int msb_balance_blocks(int S, int B, int E) {
   return (int)std::min(want, cap);
 }
 
+}  // namespace
+
+// Blocks a sequence that the forward launches, by which its scratch is sized ([B, blocks, E] floats and ints).
+// 0: a short batch, whose forward is one launch and needs none.
+MSB_API int msb_balance_blocks(int S, int B, int E) {
+  if ((long long)S * B * E <= SMALL_ELEMENTS && E <= SMALL_EXPERTS && (long long)B * E <= SMALL_CELLS) return 0;
+  return balance_grid(S, B, E);
+}
 MSB_API int msb_balance_forward(const void* logits, const unsigned char* map, int S, int B, int E, int sigmoid, float scale, int dtype,
                                 float* psum, int* csum, int blocks, float* load, float* lpart, unsigned int* ticket, float* loss,
                                 long long* counts, cudaStream_t s) {
   if (int rc = bal_check(S, B, E)) return rc;
   const Shape sh = shape_of(E, ((uintptr_t)logits & 15) == 0 && ((uintptr_t)map & 3) == 0);
   const dim3 grid(blocks, B);
+  if (blocks == 0) {
+#define BAL_CALL(T, V, NJ, SIG)                                                                                                         \
+  if constexpr ((V) * (NJ) <= 16)                                                                                                       \
+    balance_small_kernel<T, V, NJ, SIG><<<CLUSTER, SMALL_WARPS * 32, SMALL_WARPS * E * 4, s>>>((const T*)logits, map, S, B, E, sh.lanes, \
+                                                                                              scale, load, loss, counts)
+    BAL_DISPATCH(BAL_CALL)
+#undef BAL_CALL
+    MSB_CHECK_LAUNCH("balance_small");
+    return 0;
+  }
 #define BAL_CALL(T, V, NJ, SIG)                                                                                                        \
   balance_sums_kernel<T, V, NJ, SIG><<<grid, WARPS * 32, WARPS * E * 4, s>>>((const T*)logits, map, S, B, E, sh.lanes, psum, csum, ticket)
   BAL_DISPATCH(BAL_CALL)
@@ -346,7 +441,7 @@ MSB_API int msb_balance_backward(const void* logits, const float* load, int S, i
                                  void* grad, cudaStream_t s) {
   if (int rc = bal_check(S, B, E)) return rc;
   const Shape sh = shape_of(E, (((uintptr_t)logits | (uintptr_t)grad) & 15) == 0);
-  const dim3 grid(msb_balance_blocks(S, B, E), B);
+  const dim3 grid(balance_grid(S, B, E), B);
 #define BAL_CALL(T, V, NJ, SIG) \
   balance_grad_kernel<T, V, NJ, SIG><<<grid, WARPS * 32, 0, s>>>((const T*)logits, load, S, B, E, sh.lanes, scale, g, (T*)grad)
   BAL_DISPATCH(BAL_CALL)

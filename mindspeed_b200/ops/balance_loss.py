@@ -44,7 +44,7 @@ class _BalanceLoss(torch.autograd.Function):
         with _on_device(dev):
             blocks = _blocks(S, B, E)
             n = B * blocks * E
-            parts = B * ((E + 31) // 32)
+            parts = B * ((E + 31) // 32) if blocks else -1
             buf = torch.empty(B * E + 2 * n + parts + 1, dtype=torch.float32, device=dev)   # loads; sums of p, counts, joined products, ticket
             loss = torch.empty((), dtype=torch.float32, device=dev)
             counts = torch.empty(E, dtype=torch.int64, device=dev)

@@ -45,7 +45,7 @@ def _run(x, rmap, k, score, B, g=1.0):
 
 @pytest.mark.parametrize("T,E,k,B", [(1, 1, 1, 1), (1, 8, 2, 1), (7, 5, 2, 1), (64, 2, 1, 4), (500, 64, 6, 4), (1023, 33, 8, 3), (4096, 256, 8, 1),
                                      (300, 60, 4, 2), (129, 1000, 8, 3), (65, 1023, 3, 1), (20000, 16, 2, 2), (96, 130, 2, 1), (50, 512, 8, 2),
-                                     (40, 1024, 2, 4)])
+                                     (40, 1024, 2, 4), (70000, 8, 2, 1), (34, 4, 1, 17), (8191, 64, 4, 1), (513, 129, 2, 1)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_values_and_gradient(T, E, k, B, score, dtype):
