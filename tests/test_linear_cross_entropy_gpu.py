@@ -305,6 +305,31 @@ def test_incoming_gradients_of_any_layout_and_no_second_derivative():
         torch.autograd.grad(loss.sum(), hh, create_graph=True)
 
 
+@pytest.mark.parametrize("T", [30, 200])
+def test_saved_tensors_that_move_and_recomputation(T):
+    from torch.utils.checkpoint import checkpoint
+    from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy
+    V, H = 700, 64
+    h, w, fav, g, gen = _inputs(T, V, H, FP16)
+    idx, a = torch.randint(0, V, (T, 3), generator=gen, device="cuda"), torch.randn(T, 3, generator=gen, device="cuda")
+    want_ce, want_kd = _ce(h, w, fav, g), _kd(h, w, a, idx, 2.0, g)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        for got, want in ((_ce(h, w, fav, g), want_ce), (_kd(h, w, a, idx, 2.0, g), want_kd)):
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = checkpoint(lambda x, y: linear_cross_entropy(x, y, fav), hg, wg, use_reentrant=False)
+    got = torch.autograd.grad(loss, (hg, wg), g)
+    assert torch.equal(got[0], want_ce[1]) and torch.equal(got[1], want_ce[2])
+    loss = linear_cross_entropy(hg, wg, fav)
+    for _ in range(2):                              # twice through the same graph
+        got = torch.autograd.grad(loss, (hg, wg), g, retain_graph=True)
+        assert torch.equal(got[0], want_ce[1]) and torch.equal(got[1], want_ce[2])
+    with torch.no_grad():
+        wg.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, (hg, wg), g)
+
+
 def test_half_of_the_gpu():
     """Under a limit of CTAs the same numbers come out (the hidden gradient's splits may differ, and with them the order of its sums)."""
     from mindspeed_b200.ops.gemm import cta_limit

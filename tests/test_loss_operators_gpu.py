@@ -121,3 +121,39 @@ def test_mixture_of_experts_model(one_rank, score, kind):
         assert torch.isfinite(gb[n]).all()
         assert float((ga[n] - gb[n]).norm()) <= 10 * 2.0 ** -8 * float(ga[n].norm()) + 1e-12, n
     assert any("router" in n for n in ga)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_dense_model_and_main_grad(one_rank, tied, accumulate):
+    """Output weight of its own or the embedding's, gradients returned or added to fp32 main_grad; bounds as above."""
+    from mindspeed_b200.config import TransformerConfig
+    from mindspeed_b200.models.gpt_model import GPTModel
+    ids = torch.randint(0, 3000, (2, 96), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    labels = ids.roll(-1, 1)
+    pos = torch.arange(96, device="cuda").expand(2, -1)
+    got, state = [], None
+    for fused in (False, True):
+        cfg = TransformerConfig(num_layers=1, hidden_size=256, num_attention_heads=4, ffn_hidden_size=512, hidden_dropout=0.0, attention_dropout=0.0,
+                                optimization_level=1, params_dtype=BF16, bf16=True, add_bias_linear=False, normalization="RMSNorm",
+                                gradient_accumulation_fusion=accumulate, linear_cross_entropy_fusion=fused)
+        m = GPTModel(cfg, vocab_size=3000, max_sequence_length=96, position_embedding_type="rope",
+                     share_embeddings_and_output_weights=tied).cuda().train()
+        state = m.state_dict() if state is None else state
+        m.load_state_dict(state)
+        if accumulate:
+            for p in m.parameters():
+                p.main_grad = torch.zeros_like(p, dtype=torch.float32)
+        losses = []
+        for _ in range(2):                          # two micro-batches
+            loss = m(ids, pos, None, labels=labels)
+            loss.mean().backward()
+            losses.append(loss.detach())
+        assert torch.equal(*losses)
+        got.append((losses[0], {n: (p.main_grad.clone() if accumulate else 0) + (p.grad.float() if p.grad is not None else 0)
+                                for n, p in m.named_parameters()}))
+    (la, ga), (lb, gb) = got
+    assert float((la - lb).abs().max()) <= 2 * 2.0 ** -8 * 8 + 1e-4
+    for n in ga:
+        assert torch.isfinite(gb[n]).all() and gb[n].any()
+        assert float((ga[n] - gb[n]).norm()) <= 10 * 2.0 ** -8 * float(ga[n].norm()) + 1e-12, n
