@@ -21,9 +21,11 @@
 //           the 16-bit type of the operands (the tensor cores take nothing wider next to them): half a step on each term, as much as the
 //           rounding of the result itself.  With fp16, dz is scaled by a power of two that puts the largest |g| at 2^14 or above, so that
 //           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
-// Few rows: where there are at most 64, or the logits in fp32 take at most an eighth of the weight's bytes, the forward keeps them
-//           (transposed, [V, rows]: rows are the lanes of the epilogue), and an elementwise pass makes dz of them: one reading of W less,
-//           a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 -> 755 us).
+// Kept logits: the forward can keep the fp32 logits of the first words (transposed, [words, rows]: rows are the lanes of the epilogue),
+//           and an elementwise pass makes dz of them instead of the GEMM.  Few rows (at most 64, or the logits take at most an eighth of
+//           the weight's bytes) keep all: one reading of W less, a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 ->
+//           755 us).  More rows keep what the caller's limit holds, where H is wide enough (KEEP_BYTES and KEEP_WIDTH in
+//           ops/linear_cross_entropy.py, with the figures of both sides).
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.
@@ -81,8 +83,8 @@ struct LceGemm {
   const void* weight;
   long long ldh, ldw, vocab_start, vocab;
   int width, words;            // H, words of this rank
-  float* zt;                   // STATS: keep the logits, [N][ldt], or null
-  int ldt;
+  float* zt;                   // STATS: keep the logits of the first `kept` columns, [kept][ldt], or null
+  int ldt, kept;
   const float* lse;            // DLOGITS: per packed row, in units of z / tau
   const int* rowmap;           // DLOGITS: packed row -> token
   const float* g;              // DLOGITS: gradient of the token's loss
@@ -513,11 +515,11 @@ __global__ void __cluster_dims__(HOW == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(
               for (int j = 0; j < 64; ++j)
                 if (j >= left) rr[j] = 0xff800000u;          // -inf: columns past the vocabulary
             }
-            if (p.zt && row < rows) {
+            if (col0 < p.kept && row < rows) {
               float* z = p.zt + (long long)col0 * p.ldt + row;
 #pragma unroll
               for (int j = 0; j < 64; ++j)
-                if (j < left) z[(long long)j * p.ldt] = __uint_as_float(rr[j]);
+                if (j < left) z[(long long)j * p.ldt] = __uint_as_float(rr[j]);      // (`kept` is N or a multiple of 64)
             }
             float mx[4];
 #pragma unroll
@@ -1037,64 +1039,64 @@ __global__ void __launch_bounds__(256) lce_listed_kernel(T* dz, long long ld_row
   if (two) dz[(i + TWO_ROWS) * ld_row + v * ld_word] = from_f<T>(d - to_f(hi));
 }
 
-// dz of kept logits, both [V, ldt] with the rows innermost: eight rows of one word a thread.  Rows past the last are zero.  TWO: dz is
-// [V, 2 ldt], the second half what the rounding of the first left.
+// dz of kept logits, both [words, ldt] with the rows innermost: eight rows of one word a thread, 256 rows a block (grid.y).  Rows past the
+// last are zero up to the next multiple of 64, which is what the products read.  TWO: dz is [words, 2 ldt], the second half what the
+// rounding of the first left.
 template <typename T, bool TWO>
-__global__ void __launch_bounds__(256) lce_dz_kernel(const float* zt, T* dz, int ldt, int V, const float* lse,
+__global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int words, const float* lse,
                                                      const long long* __restrict__ label, const float* z,
-                                                     const int* rowmap, const int* count, long long vocab_start,
+                                                     const int* rowmap, const int* count, long long word_start,
                                                      const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
                                                      float tc_inv_tau, const float* scale) {
   after_previous();
-  const int groups = ldt / 8, n = *count;
-  // the block's threads take (256 / groups) words a round, always the same rows
-  const int per = max(1, 256 / groups), grp = threadIdx.x % groups, sub = threadIdx.x / groups;
+  const int n = *count, groups = min(ldt, (n + 63) / 64 * 64) / 8 - (int)blockIdx.y * 32;
+  if (groups <= 0) return;
+  // the block's threads take `per` words a round, always the same rows
+  const int wide = min(groups, 32), per = 256 / wide, sub = threadIdx.x / wide;
   if (sub >= per) return;
-  for (int g0 = grp; g0 < groups; g0 += 256) {
-    float coef[8], ls[8], atl[8];
-    long long lab[8];
+  const int r0 = ((int)blockIdx.y * 32 + (int)threadIdx.x % wide) * 8;
+  float coef[8], ls[8], atl[8];
+  long long lab[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = g0 * 8 + j;
-      coef[j] = ls[j] = atl[j] = 0.f;
-      lab[j] = -1;
-      if (i < n) {
-        const int t = rowmap[i];
-        coef[j] = g[(long long)t * g_stride] * g_factor;
-        if (scale) coef[j] *= scale[0];
-        ls[j] = lse[i];
-        if (label) {
-          lab[j] = label[t] - vocab_start;
-          atl[j] = (ex2((z[i] * inv_tau - ls[j]) * LOG2E) - 1.f) * coef[j];
-        }
+  for (int j = 0; j < 8; ++j) {
+    const int i = r0 + j;
+    coef[j] = ls[j] = atl[j] = 0.f;
+    lab[j] = -1;
+    if (i < n) {
+      const int t = rowmap[i];
+      coef[j] = g[(long long)t * g_stride] * g_factor;
+      if (scale) coef[j] *= scale[0];
+      ls[j] = lse[i];
+      if (label) {
+        lab[j] = label[t] - word_start;
+        atl[j] = (ex2((z[i] * inv_tau - ls[j]) * LOG2E) - 1.f) * coef[j];
       }
     }
+  }
 #pragma unroll 2
-    for (int v = blockIdx.x * per + sub; v < V; v += gridDim.x * per) {
-      const long long o = (long long)v * ldt + g0 * 8;
-      Vec8<float> x;
-      x.load(zt + o);
-      float f[8];
-      x.to_float(f);
+  for (long long v = (long long)blockIdx.x * per + sub; v < words; v += (long long)gridDim.x * per) {
+    Vec8<float> x;
+    x.load(zt + v * ldt + r0);
+    float f[8];
+    x.to_float(f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], tc_inv_tau, -ls[j]) * LOG2E) * coef[j];
-        f[j] = coef[j] == 0.f ? 0.f : e;
-      }
-      Vec8<T> w;
+    for (int j = 0; j < 8; ++j) {
+      const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], tc_inv_tau, -ls[j]) * LOG2E) * coef[j];
+      f[j] = coef[j] == 0.f ? 0.f : e;
+    }
+    Vec8<T> w;
+    w.from_float(f);
+    if (TWO) {
+      T* at = dz + v * 2 * ldt + r0;
+      w.store(at);
+      float hi[8];
+      w.to_float(hi);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] -= hi[j];
       w.from_float(f);
-      if (TWO) {
-        T* at = dz + (long long)v * 2 * ldt + g0 * 8;
-        w.store(at);
-        float hi[8];
-        w.to_float(hi);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] -= hi[j];
-        w.from_float(f);
-        w.store(at + ldt);
-      } else {
-        w.store(dz + o);
-      }
+      w.store(at + ldt);
+    } else {
+      w.store(dz + v * ldt + r0);
     }
   }
 }
@@ -1244,14 +1246,15 @@ struct MsbLceArgs {
   float* loss;                 // [T]
   float* part;                 // [ceil(V / 256) * 2, T] pairs, scratch
   unsigned char* part_at;      // [ceil(V / 256) * 2, T] scratch
-  float* zt;                   // [V, ldt] logits kept for the backward, or null
+  float* zt;                   // [kept, ldt] logits of the first `kept` words, for the backward, or null
   int ldt;                     // T rounded up to a multiple of 8; TWO_ROWS for up to so many tokens
+  int kept;                    // V, or a multiple of 64
   float* mx;                   // [T], [T]: local statistics for the vocabulary-parallel form, else null
   float* sum;
   // backward
   const float* g;
   long long g_stride;          // 0: one value for all tokens
-  void* dz;                    // [T, piece] scratch, row pitch ldz; with zt [V, ldt], or [V, 2 TWO_ROWS]
+  void* dz;                    // scratch of a piece: [T, piece], row pitch ldz; of kept words [piece, ldt], or [piece, 2 TWO_ROWS]
   long long ldz;
   int piece;                   // columns of a piece (a multiple of 256)
   float* acc;                  // [splits, slab_rows, H] fp32 scratch, or null: no hidden gradient
@@ -1275,6 +1278,8 @@ static int lce_check(const MsbLceArgs* a) {
   MSB_REQUIRE(a->K == 1 || a->teacher, "linear_ce: lists need teacher logits");
   MSB_REQUIRE(a->K <= 1024, "linear_ce: %d listed words", a->K);
   MSB_REQUIRE(!a->zt || (a->ldt % 8 == 0 && a->ldt >= a->T && (a->T > TWO_ROWS || a->ldt == TWO_ROWS)), "linear_ce: pitch %d of the kept logits", a->ldt);
+  MSB_REQUIRE(a->zt ? a->kept == a->V || (a->kept > 0 && a->kept < a->V && a->kept % 64 == 0 && a->T > TWO_ROWS) : a->kept == 0,
+              "linear_ce: logits of %d words kept", a->kept);
   MSB_REQUIRE(a->piece > 0 && a->piece % 256 == 0 && a->splits >= 1, "linear_ce: piece of %d columns, %d splits", a->piece, a->splits);
   return 0;
 }
@@ -1321,7 +1326,7 @@ static int lce_forward(const MsbLceArgs* a, cudaStream_t s) {
   p.group_m = GROUP_LOGITS;
   p.half = a->dtype == MSB_F16;
   p.part = reinterpret_cast<float2*>(a->part); p.part_at = a->part_at; p.part_ld = a->T;
-  p.zt = a->zt; p.ldt = a->ldt;
+  p.zt = a->zt; p.ldt = a->ldt; p.kept = a->kept;
   p.sorted = a->teacher && !scan ? a->sorted : nullptr;
   p.idx = a->idx; p.teacher = a->teacher; p.listed = a->z; p.list = a->K;
   p.hidden = hidden; p.weight = weight; p.ldh = a->ldh; p.ldw = a->ldw; p.vocab_start = a->vocab_start; p.vocab = a->vocab;
@@ -1379,20 +1384,20 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   p.label = label; p.z = a->z;
   p.scale = a->scale;
   p.status = a->status;
-  const int piece = a->zt ? a->V : a->piece;       // kept logits are few
   const int two = a->zt && a->T <= TWO_ROWS, dz_rows = two ? 2 * TWO_ROWS : a->T, dz_ld = two ? 2 * TWO_ROWS : a->ldt;
-  int rc;
-  for (long long v0 = 0; v0 < a->V; v0 += piece) {
-    const int cols = (int)std::min<long long>(piece, a->V - v0);
+  int rc, cols;
+  for (long long v0 = 0; v0 < a->V; v0 += cols) {
+    const bool kept = v0 < a->kept;
+    cols = (int)std::min<long long>(a->piece, (kept ? a->kept : a->V) - v0);
     const DT* w = (const DT*)a->weight + v0 * a->ldw;
     // dz of the piece
-    if (a->zt) {
-      const int per = std::max(1, 256 / (a->ldt / 8));
-      const int grid = (int)std::min<long long>((a->V + per - 1) / per, (long long)msb::num_sms() * 8);
+    if (kept) {
+      const int wide = (a->ldt + 255) / 256, per = 256 / std::min(32, a->ldt / 8);
+      const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>((cols + per - 1) / per, (long long)msb::num_sms() * 8 / wide)), wide);
 #define LCE_DZ(HOW, TWO)                                                                                                                     \
-  HOW("lce_dz", (lce_dz_kernel<DT, TWO>), grid, 256, 0, a->zt, dz, a->ldt, a->V, a->lse, label, a->z, a->rowmap, a->count, a->vocab_start,      \
-      a->g, (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
-      if (a->scale) {
+  HOW("lce_dz", (lce_dz_kernel<DT, TWO>), grid, 256, 0, a->zt + v0 * a->ldt, dz, a->ldt, cols, a->lse, label, a->z, a->rowmap, a->count,        \
+      a->vocab_start + v0, a->g, (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
+      if (a->scale || v0 > 0) {
         if (two) LCE_DZ(LCE_AFTER, true);
         else LCE_DZ(LCE_AFTER, false);
       } else {
@@ -1410,24 +1415,24 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
     }
     if (a->teacher) {
       const long long places = (long long)a->T * a->K;
-      LCE_AFTER("lce_listed", lce_listed_kernel<DT>, (unsigned)((places + 255) / 256), 256, 0, dz, a->zt ? 1 : a->ldz, a->zt ? dz_ld : 1, two,
+      LCE_AFTER("lce_listed", lce_listed_kernel<DT>, (unsigned)((places + 255) / 256), 256, 0, dz, kept ? 1 : a->ldz, kept ? dz_ld : 1, two,
                 a->idx, a->z, a->q, a->lse, a->rowmap, a->count, a->K, a->vocab_start + v0, cols, a->g, (int)a->g_stride, a->tau, inv_tau,
                 a->scale);
     }
     if (a->acc) {
-      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BK, 64);
+      if (kept) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BK, 64);
       else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BM, BK);
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, w, dt, 2, cols, a->H, a->ldw, BK, 64))) return rc;
       if ((rc = make_tmap_2d(&p.tmD, a->acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (uint64_t)a->splits * a->slab_rows, a->H, a->H, 32, 32))) return rc;
       p.M = dz_rows; p.N = a->H; p.K = cols; p.group_m = GROUP_GRADS; p.rows_on_k = 0; p.two = two;
       p.split = 1; p.slab_rows = a->slab_rows; p.accumulate = v0 > 0;
-      rc = a->zt ? launch_gemm<EPI_OUT32, true, true>(p, dhidden_how(a), a->splits, false, s)
+      rc = kept ? launch_gemm<EPI_OUT32, true, true>(p, dhidden_how(a), a->splits, false, s)
                  : launch_gemm<EPI_OUT32, false, true>(p, dhidden_how(a), a->splits, false, s);
       if (rc) return rc;
     }
     if (a->dweight) {
-      if (a->zt) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BM, BK);
+      if (kept) rc = make_tmap_2d(&p.tmA, dz, dt, 2, cols, dz_rows, dz_ld, BM, BK);
       else rc = make_tmap_2d(&p.tmA, dz, dt, 2, a->T, cols, a->ldz, BK, 64);
       if (rc) return rc;
       if ((rc = make_tmap_2d(&p.tmB, a->hidden, dt, 2, a->T, a->H, a->ldh, BK, 64))) return rc;
@@ -1437,11 +1442,11 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
       if (a->dweight_fp32_add) {
         if ((rc = make_tmap_2d(&p.tmD, (float*)a->dweight + v0 * a->H, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, a->H, a->H, 32, 32))) return rc;
         p.accumulate = 1;
-        rc = a->zt ? launch_gemm<EPI_OUT32, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT32, true, true>(p, how, 1, false, s);
+        rc = kept ? launch_gemm<EPI_OUT32, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT32, true, true>(p, how, 1, false, s);
       } else {
         if ((rc = make_tmap_2d(&p.tmD, (DT*)a->dweight + v0 * a->H, dt, 2, cols, a->H, a->H, 32, 64))) return rc;
         p.accumulate = 0;
-        rc = a->zt ? launch_gemm<EPI_OUT16, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT16, true, true>(p, how, 1, false, s);
+        rc = kept ? launch_gemm<EPI_OUT16, false, true>(p, how, 1, false, s) : launch_gemm<EPI_OUT16, true, true>(p, how, 1, false, s);
       }
       if (rc) return rc;
     }
@@ -1462,7 +1467,7 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
 // Hidden and weight gradients, a piece of the vocabulary at a time.
 MSB_API int msb_lce_backward(const MsbLceArgs* a, cudaStream_t s) {
   if (int rc = lce_check(a)) return rc;
-  MSB_REQUIRE(a->zt || (a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V)), "linear_ce: pitch %lld of a piece of %d columns", a->ldz, a->piece);
+  MSB_REQUIRE(a->kept == a->V || (a->ldz % 8 == 0 && a->ldz >= std::min(a->piece, a->V)), "linear_ce: pitch %lld of a piece of %d columns", a->ldz, a->piece);
   const int dz_rows = a->zt && a->T <= TWO_ROWS ? 2 * TWO_ROWS : a->T;
   MSB_REQUIRE(!a->acc || (a->slab_rows >= dz_rows && a->slab_rows % 32 == 0 && (long long)a->splits * a->slab_rows < 0x7fffffffll),
               "linear_ce: %d slabs of %d rows", a->splits, a->slab_rows);

@@ -5,9 +5,10 @@
   linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices)     per-token tau^2 KL(teacher's top words || student)
 
 Both take ``hidden`` [..., H] and ``weight`` [V, H] in bf16 or fp16 (H a multiple of 8) and return the loss in fp32 with the leading shape
-of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token, the backward makes the logits again, a
-piece of the vocabulary at a time.  (For few tokens, at most 64 or a sixteenth of H, the fp32 logits are
-kept instead: at most an eighth of the weight's bytes, or 256 bytes a word.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
+of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token and, in training, at most ``KEEP_BYTES``
+(2 GiB) of fp32 logits, as far as they go over the vocabulary; the backward makes the others again.  Both directions work on a piece of the
+vocabulary at a time.  (For few tokens, at most 64 or a sixteenth of H, all logits are kept: at most an eighth of the weight's bytes, or
+256 bytes a word.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
 teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
 
 A label or teacher index beyond the vocabulary gives its token loss NaN and no gradient, and makes ``ops.gemm.check_status`` raise.
@@ -39,6 +40,13 @@ _P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_flo
 #: bytes of the 16-bit logit gradients that the backward holds at a time, and of the fp32 partial results of the hidden gradient
 PIECE_BYTES = 512 << 20
 SLAB_BYTES = 256 << 20
+#: bytes of fp32 logits that a call keeps from its forward to its backward, which then makes those of the remaining words again.  0 keeps
+#: none (but for few tokens).  Keeping costs about 2 ps a logit, making it again 2 H / 1.3 PFLOP/s: at least KEEP_WIDTH hidden columns
+#: (both directions, us, made again -> kept: 1000 x 60000 x 1024 480 -> 513, 2048 x 32000 x 2048 917 -> 845, 4096 x 129280 x 4096
+#: 13400 -> 10800), and at least KEEP_LEAST words, which fill the products' tiles.
+KEEP_BYTES = 2 << 30
+KEEP_WIDTH = 1536
+KEEP_LEAST = 8192
 MAX_LIST = 1024
 #: up to so many tokens the logits are kept whatever H is, and their gradients go into the products in two 16-bit terms
 TWO_ROWS = 64
@@ -48,7 +56,7 @@ class _Args(ctypes.Structure):
     _fields_ = [("hidden", _P), ("weight", _P), ("idx", _P), ("teacher", _P), ("ldh", _LL), ("ldw", _LL), ("vocab_start", _LL), ("vocab", _LL),
                 ("ignore_index", _LL), ("T", _I), ("H", _I), ("V", _I), ("K", _I), ("dtype", _I), ("tau", _F), ("pos", _P), ("rowmap", _P),
                 ("count", _P), ("kind", _P), ("sorted", _P), ("packed", _P), ("z", _P), ("q", _P), ("dot", _P), ("ent", _P), ("lse", _P), ("loss", _P),
-                ("part", _P), ("part_at", _P), ("zt", _P), ("ldt", _I), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
+                ("part", _P), ("part_at", _P), ("zt", _P), ("ldt", _I), ("kept", _I), ("mx", _P), ("sum", _P), ("g", _P), ("g_stride", _LL), ("dz", _P), ("ldz", _LL), ("piece", _I), ("acc", _P),
                 ("splits", _I), ("slab_rows", _I), ("dhidden", _P), ("dweight", _P), ("dweight_fp32_add", _I), ("scale", _P), ("status", _P)]
 
 
@@ -79,15 +87,23 @@ def _rows(t):
 
 
 @functools.lru_cache(maxsize=64)
-def _plan(T, H, V, piece_bytes, slab_bytes, train):
-    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits or 0 where none are).
+def _plan(T, H, V, piece_bytes, slab_bytes, train, keep_bytes=KEEP_BYTES):
+    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits, words whose logits are kept).
 
     The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
-    four times are never better.  Logits are kept where they take, in fp32, at most an eighth of the weight's bytes, or 64 rows."""
+    four times are never better.  The logits of all words are kept where they take, in fp32, at most an eighth of the weight's bytes, or
+    64 rows; else, where that is faster, of as many words as go into ``keep_bytes``."""
     cols = min(max(256, piece_bytes // (2 * T) // 256 * 256), (V + 255) // 256 * 256)
     tiles = -(-H // 256)
     splits = max(1, min(64, -(-296 // tiles), slab_bytes // ((T + 31) // 32 * 32 * H * 4)))
-    return cols, splits, 0 if not train else TWO_ROWS if T <= TWO_ROWS else (T + 7) // 8 * 8 if 16 * T <= H else 0
+    ldt = TWO_ROWS if T <= TWO_ROWS else (T + 7) // 8 * 8
+    kept = 0
+    if train and (T <= TWO_ROWS or 16 * T <= H):
+        kept = V
+    elif train and H >= KEEP_WIDTH:
+        kept = min(V, keep_bytes // (4 * ldt) // 256 * 256)
+        kept = kept if kept >= min(V, KEEP_LEAST) else 0
+    return cols, splits, ldt if kept else 0, kept
 
 
 def _lib():
@@ -116,14 +132,14 @@ class _Job:
         4-byte words."""
         (T, H), (V, _) = h.shape, w.shape
         K = self.K
-        piece, splits, ldt = self.plan
+        piece, splits, ldt, words = self.plan
         at = kept.data_ptr()
-        z = at + 2 * T * H + 4 * V * ldt
+        z = at + 2 * T * H + 4 * words * ldt
         pos = z + 8 * T * K + 4 * T
         return _Args(hidden=h.data_ptr(), weight=w.data_ptr(), idx=idx.data_ptr(), teacher=None if teacher is None else teacher.data_ptr(),
                      ldh=h.stride(0) if T > 1 else H, ldw=w.stride(0) if V > 1 else H, vocab_start=self.rank * V, vocab=self.world * V,
                      ignore_index=self.ignore_index, T=T, H=H, V=V, K=K, dtype=code(h.dtype), tau=self.tau, packed=at,
-                     zt=at + 2 * T * H if ldt else None, ldt=ldt, z=z, q=z + 4 * T * K, lse=z + 8 * T * K, pos=pos, rowmap=pos + 4 * T,
+                     zt=at + 2 * T * H if ldt else None, ldt=ldt, kept=words, z=z, q=z + 4 * T * K, lse=z + 8 * T * K, pos=pos, rowmap=pos + 4 * T,
                      count=pos + 8 * T, piece=piece, splits=splits, status=_status(h.device).data_ptr())
 
 
@@ -134,11 +150,11 @@ class _LinearLoss(torch.autograd.Function):
         dev = hidden.device
         h, w = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
         (T, H), V, K = h.shape, w.shape[0], job.K
-        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train)
+        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train, KEEP_BYTES)
         job.shape = hidden.shape
-        ldt = job.plan[2]
+        _, _, ldt, words = job.plan
         with _on_device(dev):
-            kept = torch.empty(T * H // 2 + V * ldt + 2 * T * K + 3 * T + 2, dtype=torch.float32, device=dev)
+            kept = torch.empty(T * H // 2 + words * ldt + 2 * T * K + 3 * T + 2, dtype=torch.float32, device=dev)
             parts = (V + 255) // 256 * 2
             lists = 0 if job.teacher is None else 2 * T * K
             scratch = torch.empty(lists + 2 * parts * T + 4 * T + (parts * T + T + 3) // 4, dtype=torch.float32, device=dev)
@@ -183,15 +199,15 @@ class _LinearLoss(torch.autograd.Function):
         dev = h.device
         h, w = _rows(h), _rows(w)
         (T, H), V = h.shape, w.shape[0]
-        piece, splits, ldt = job.plan
+        piece, splits, ldt, words = job.plan
         with _on_device(dev):
             one = not any(g.stride()) or g.numel() == 1      # an expanded scalar, as a sum's backward gives
             if not one and not g.is_contiguous():
                 g = g.contiguous()
             two = ldt and T <= TWO_ROWS
-            ldz = 0 if ldt else min(piece, (V + 7) // 8 * 8)
+            ldz = 0 if words == V else min(piece, (V + 7) // 8 * 8)
             slab_rows = 2 * TWO_ROWS if two else (T + 31) // 32 * 32
-            dz_words = (V * (2 if two else 1) * ldt if ldt else T * ldz) // 2
+            dz_words = max(min(piece, words) * (2 if two else 1) * ldt, T * ldz) // 2
             scratch = torch.empty(dz_words + (splits * slab_rows * H if need_h else 0) + 2, dtype=torch.float32, device=dev)
             a = job.args(h, w, idx, teacher, kept)
             a.g, a.g_stride = g.data_ptr(), 0 if one else 1
@@ -236,7 +252,7 @@ def _linear_loss_ref(hidden, weight, idx, q, ent, tau, group):
     world = 1 if group is None else dist.get_world_size(group)
     rank = 0 if group is None else dist.get_rank(group)
     V = weight.shape[0]
-    keep = (q.sum(1) > 0).nonzero().squeeze(1)
+    keep = (q.sum(1) != 0).nonzero().squeeze(1)          # (a teacher's NaN stays in)
     x = hidden.reshape(-1, hidden.shape[-1]).index_select(0, keep)
     idx, q, ent_k = idx.index_select(0, keep), q.index_select(0, keep), ent.index_select(0, keep)
     z = (x.float() @ weight.float().t()) / tau

@@ -139,6 +139,53 @@ def test_pieces_and_splits(dtype, monkeypatch):
         _compare(_kd(h, w, a, idx, 2.0, g), h, w, _kd_target(idx, a, 2.0), 2.0, g)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,V,H,left", [(300, 3000, 136, 0), (300, 3000, 136, 130), (1030, 777, 64, 300), (65, 2049, 72, 64), (70, 600, 64, 70)])
+def test_kept_logits(T, V, H, left, dtype, monkeypatch):
+    """Logits of all words, of the first ones and of none kept, in one piece or several; memory that the call gets holds NaN.  Loss and
+    weight gradient are the same bits: the same sums, rounded the same way."""
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    h, w, fav, g, gen = _inputs(T, V, H, dtype)
+    order = torch.randperm(T, generator=gen, device="cuda")[:left]
+    fav[order] = -100
+    idx = torch.randint(0, V, (T, 5), generator=gen, device="cuda")
+    idx[:, 4] = idx[:, 0]
+    a = torch.randn(T, 5, generator=gen, device="cuda")
+    a[order] = float("-inf")
+    monkeypatch.setattr(M, "KEEP_WIDTH", 64)
+    monkeypatch.setattr(M, "KEEP_LEAST", 256)
+    ldt = (T + 7) // 8 * 8
+    first = None
+    for keep, words in ((0, 0), (4 * ldt * 300, 256), (4 * ldt * (V + 255), V), (4 * ldt * 530, 512)):
+        for piece in (M.PIECE_BYTES, 2 * T * 300):
+            assert M._plan(T, H, V, piece, M.SLAB_BYTES, True, keep)[3] == words
+            monkeypatch.setattr(M, "KEEP_BYTES", keep)
+            monkeypatch.setattr(M, "PIECE_BYTES", piece)
+            for call, target, tau in ((lambda: _ce(h, w, fav, g), _ce_target(fav), 1.0), (lambda: _kd(h, w, a, idx, 2.0, g), _kd_target(idx, a, 2.0), 2.0)):
+                torch.cuda.synchronize()
+                torch.cuda.empty_cache()
+                poison = [torch.full((n,), float("nan"), device="cuda") for n in (1 << 16, 1 << 18, 1 << 20, 1 << 22, 1 << 22, 1 << 22)]
+                del poison
+                got = call()
+                _compare(got, h, w, target, tau, g)
+                first = {} if first is None else first
+                want = first.setdefault(tau, got)
+                assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+        monkeypatch.undo()
+        monkeypatch.setattr(M, "KEEP_WIDTH", 64)
+        monkeypatch.setattr(M, "KEEP_LEAST", 256)
+
+
+def test_kept_logits_of_a_wide_layer(monkeypatch):
+    """The default rule at a size that it applies to: half of the words kept."""
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    T, V, H = 200, 20000, 1536
+    monkeypatch.setattr(M, "KEEP_BYTES", 4 * T * 10000)
+    assert M._plan(T, H, V, M.PIECE_BYTES, M.SLAB_BYTES, True, M.KEEP_BYTES)[2:] == (200, 9984)
+    h, w, fav, g, gen = _inputs(T, V, H, BF16)
+    _compare(_ce(h, w, fav, g), h, w, _ce_target(fav), 1.0, g)
+
+
 def test_layouts():
     """Leading axes, rows of a wider buffer, an unaligned view, 32-bit labels, a scalar's expanded gradient, another ignore index."""
     from mindspeed_b200.ops.linear_cross_entropy import linear_cross_entropy

@@ -110,6 +110,30 @@ def test_balance_loss_is_the_one_of_the_router(score):
         assert torch.allclose(torch.autograd.grad(loss, x)[0], torch.autograd.grad(want, x, retain_graph=True)[0], atol=1e-9)
 
 
+def test_logits_that_are_kept():
+    from mindspeed_b200.ops import linear_cross_entropy as M
+    def kept(T, H, V, train=True, keep=M.KEEP_BYTES):
+        return M._plan(T, H, V, M.PIECE_BYTES, M.SLAB_BYTES, train, keep)[2:]
+    assert kept(1, 64, 1000) == (64, 1000) and kept(64, 64, 1000, keep=0) == (64, 1000)      # few tokens
+    assert kept(100, 1600, 500000, keep=0) == (104, 500000)                                  # an eighth of the weight's bytes
+    assert kept(101, 1600, 500000, keep=0) == (0, 0) == kept(101, 1600, 500000, train=False) == kept(1, 64, 1000, train=False)
+    assert kept(4096, 4096, 32001) == (4096, 32001)
+    assert kept(4090, 1024, 32001) == (0, 0)                                                 # making them again costs less
+    T, V = 30001, 150000
+    ldt, words = kept(T, 4096, V)
+    assert ldt == 30008 and words % 256 == 0 and 4 * ldt * words <= M.KEEP_BYTES < 4 * ldt * (words + 256)
+    assert kept(2 ** 17, 4096, V) == (0, 0)                                                  # too few words to fill the products
+
+
+def test_teacher_without_a_number():
+    from mindspeed_b200.ops.linear_cross_entropy import linear_topk_distillation
+    h, w = torch.randn(3, 8), torch.randn(10, 8)
+    a, idx = torch.zeros(3, 2), torch.tensor([[0, 1]] * 3)
+    a[1, 0] = float("nan")
+    loss = linear_topk_distillation(h, w, a, idx)
+    assert torch.isnan(loss).tolist() == [False, True, False]
+
+
 def test_refusals():
     h, w, lab, idx, a, _ = _inputs()
     for call, err, msg in ((lambda: linear_cross_entropy(h, w[:, :8], lab), ValueError, "do not fit"),
