@@ -1039,28 +1039,30 @@ __global__ void __launch_bounds__(256) lce_listed_kernel(T* dz, long long ld_row
   if (two) dz[(i + TWO_ROWS) * ld_row + v * ld_word] = from_f<T>(d - to_f(hi));
 }
 
-// dz of kept logits, both [words, ldt] with the rows innermost: eight rows of one word a thread, 256 rows a block (grid.y).  Rows past the
-// last are zero up to the next multiple of 64, which is what the products read.  TWO: dz is [words, 2 ldt], the second half what the
-// rounding of the first left.
+// dz of kept logits, both [words, ldt] with the rows innermost: eight rows of one word a thread, 256 rows a block.  Rows past the last
+// are zero up to the next multiple of 64, which is what the products read.  TWO: dz is [words, 2 ldt], the second half what the rounding of
+// the first left.  Bound by the memory rate: one wave of blocks, with the logits of DZ_AHEAD words of each thread in flight (4096 rows x
+// 32000 words 120 us, 6.5 TB/s: two words at four blocks an SM spill, 129; four waves of blocks of three words 138).
+constexpr int DZ_AHEAD = 4, DZ_RESIDENT = 2;
 template <typename T, bool TWO>
-__global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int words, const float* lse,
-                                                     const long long* __restrict__ label, const float* z,
-                                                     const int* rowmap, const int* count, long long word_start,
-                                                     const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
-                                                     float tc_inv_tau, const float* scale) {
+__global__ void __launch_bounds__(256, DZ_RESIDENT) lce_dz_kernel(const float* __restrict__ zt, T* __restrict__ dz, int ldt, int words, const float* lse,
+                                                        const long long* __restrict__ label, const float* z,
+                                                        const int* rowmap, const int* count, long long word_start,
+                                                        const float* __restrict__ g, int g_stride, float g_factor, float inv_tau,
+                                                        float tc_inv_tau, const float* scale) {
   after_previous();
-  const int n = *count, groups = min(ldt, (n + 63) / 64 * 64) / 8 - (int)blockIdx.y * 32;
-  if (groups <= 0) return;
-  // the block's threads take `per` words a round, always the same rows
-  const int wide = min(groups, 32), per = 256 / wide, sub = threadIdx.x / wide;
+  const int n = *count, groups = min(ldt, (n + 63) / 64 * 64) / 8, chunks = (groups + 31) / 32;
+  if (n == 0) return;
+  // block b takes rows of chunk b mod chunks; its threads take `per` words a round, always the same rows
+  const int chunk = (int)blockIdx.x % chunks, wide = min(groups - chunk * 32, 32), per = 256 / wide, sub = threadIdx.x / wide;
   if (sub >= per) return;
-  const int r0 = ((int)blockIdx.y * 32 + (int)threadIdx.x % wide) * 8;
-  float coef[8], ls[8], atl[8];
-  long long lab[8];
+  const int r0 = (chunk * 32 + (int)threadIdx.x % wide) * 8;
+  float coef[8], ls[8];
+  int lab[8];                                   // word of the piece that is the row's label, or -1
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int i = r0 + j;
-    coef[j] = ls[j] = atl[j] = 0.f;
+    coef[j] = ls[j] = 0.f;
     lab[j] = -1;
     if (i < n) {
       const int t = rowmap[i];
@@ -1068,35 +1070,52 @@ __global__ void __launch_bounds__(256) lce_dz_kernel(const float* __restrict__ z
       if (scale) coef[j] *= scale[0];
       ls[j] = lse[i];
       if (label) {
-        lab[j] = label[t] - word_start;
-        atl[j] = (ex2((z[i] * inv_tau - ls[j]) * LOG2E) - 1.f) * coef[j];
+        const long long l = label[t] - word_start;
+        if (l >= 0 && l < words) lab[j] = (int)l;
       }
     }
   }
-#pragma unroll 2
-  for (long long v = (long long)blockIdx.x * per + sub; v < words; v += (long long)gridDim.x * per) {
-    Vec8<float> x;
-    x.load(zt + v * ldt + r0);
-    float f[8];
-    x.to_float(f);
+  const unsigned step = ((gridDim.x - chunk + chunks - 1) / chunks) * per;
+  unsigned v = (blockIdx.x / chunks) * per + sub;
+  const long long hop = (long long)step * ldt;
+  const float* from = zt + (long long)v * ldt + r0;
+  T* to = dz + (long long)v * (TWO ? 2 : 1) * ldt + r0;
+  while (v < (unsigned)words) {
+    Vec8<float> x[DZ_AHEAD];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = lab[j] == v ? atl[j] : ex2(fmaf(f[j], tc_inv_tau, -ls[j]) * LOG2E) * coef[j];
-      f[j] = coef[j] == 0.f ? 0.f : e;
-    }
-    Vec8<T> w;
-    w.from_float(f);
-    if (TWO) {
-      T* at = dz + v * 2 * ldt + r0;
-      w.store(at);
-      float hi[8];
-      w.to_float(hi);
+    for (int u = 0; u < DZ_AHEAD; ++u)
+      if (v + u * step < (unsigned)words) x[u].load(from + u * hop);
+    from += DZ_AHEAD * hop;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] -= hi[j];
+    for (int u = 0; u < DZ_AHEAD; ++u) {
+      if (v >= (unsigned)words) return;
+      float f[8];
+      x[u].to_float(f);
+      bool listed = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e = ex2(fmaf(f[j], tc_inv_tau, -ls[j]) * LOG2E) * coef[j];
+        f[j] = coef[j] == 0.f ? 0.f : e;
+        listed |= lab[j] == (int)v;
+      }
+      if (listed) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (lab[j] == (int)v && coef[j] != 0.f) f[j] = (ex2((z[r0 + j] * inv_tau - ls[j]) * LOG2E) - 1.f) * coef[j];
+      }
+      Vec8<T> w;
       w.from_float(f);
-      w.store(at + ldt);
-    } else {
-      w.store(dz + v * ldt + r0);
+      w.store(to);
+      if (TWO) {
+        float hi[8];
+        w.to_float(hi);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] -= hi[j];
+        w.from_float(f);
+        w.store(to + ldt);
+      }
+      v += step;
+      to += TWO ? 2 * hop : hop;
     }
   }
 }
@@ -1392,8 +1411,9 @@ static int lce_backward(const MsbLceArgs* a, cudaStream_t s) {
     const DT* w = (const DT*)a->weight + v0 * a->ldw;
     // dz of the piece
     if (kept) {
-      const int wide = (a->ldt + 255) / 256, per = 256 / std::min(32, a->ldt / 8);
-      const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>((cols + per - 1) / per, (long long)msb::num_sms() * 8 / wide)), wide);
+      const int chunks = (a->ldt + 255) / 256, per = 256 / std::min(32, a->ldt / 8);
+      const long long most = (long long)((cols + per - 1) / per) * chunks;
+      const unsigned grid = (unsigned)std::max<long long>(chunks, std::min<long long>(most, (long long)msb::num_sms() * DZ_RESIDENT));
 #define LCE_DZ(HOW, TWO)                                                                                                                     \
   HOW("lce_dz", (lce_dz_kernel<DT, TWO>), grid, 256, 0, a->zt + v0 * a->ldt, dz, a->ldt, cols, a->lse, label, a->z, a->rowmap, a->count,        \
       a->vocab_start + v0, a->g, (int)a->g_stride, a->tau, inv_tau, p.tc_inv_tau, a->scale)
