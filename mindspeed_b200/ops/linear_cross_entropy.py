@@ -41,11 +41,11 @@ _P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_flo
 PIECE_BYTES = 512 << 20
 SLAB_BYTES = 256 << 20
 #: bytes of fp32 logits that a call keeps from its forward to its backward, which then makes those of the remaining words again.  0 keeps
-#: none (but for few tokens).  Keeping costs about 2 ps a logit, making it again 2 H / 1.3 PFLOP/s: at least KEEP_WIDTH hidden columns
-#: (both directions, us, made again -> kept: 1000 x 60000 x 1024 480 -> 513, 2048 x 32000 x 2048 917 -> 845, 4096 x 129280 x 4096
-#: 13400 -> 10800), and at least KEEP_LEAST words, which fill the products' tiles.
+#: none (but for few tokens).  A kept logit costs what its bytes take, making it again 2 H / 1.3 PFLOP/s: at least KEEP_WIDTH hidden columns
+#: (both directions, us, made again -> kept: 1024 x 128256 x 512 579 -> 606, 766 x 50257 x 768 333 -> 316, 2048 x 32000 x 1024 515 -> 485,
+#: 2048 x 50000 x 1536 1065 -> 945, 4096 x 129280 x 4096 13000 -> 10700), and at least KEEP_LEAST words, which fill the products' tiles.
 KEEP_BYTES = 2 << 30
-KEEP_WIDTH = 1536
+KEEP_WIDTH = 640
 KEEP_LEAST = 8192
 MAX_LIST = 1024
 #: up to so many tokens the logits are kept whatever H is, and their gradients go into the products in two 16-bit terms
@@ -86,11 +86,14 @@ def _rows(t):
     return t
 
 
-@functools.lru_cache(maxsize=64)
-def _plan(T, H, V, piece_bytes, slab_bytes, train, keep_bytes=KEEP_BYTES):
-    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits, words whose logits are kept).
+def _plan(T, H, V, piece_bytes, slab_bytes, train, keep_bytes=None):
+    """(columns of a piece, most K splits of the hidden gradient, pitch of kept logits, words whose logits are kept)."""
+    return _planned(T, H, V, piece_bytes, slab_bytes, train, KEEP_BYTES if keep_bytes is None else keep_bytes, KEEP_WIDTH, KEEP_LEAST)
 
-    The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
+
+@functools.lru_cache(maxsize=64)
+def _planned(T, H, V, piece_bytes, slab_bytes, train, keep_bytes, keep_width, keep_least):
+    """The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
     four times are never better.  The logits of all words are kept where they take, in fp32, at most an eighth of the weight's bytes, or
     64 rows; else, where that is faster, of as many words as go into ``keep_bytes``."""
     cols = min(max(256, piece_bytes // (2 * T) // 256 * 256), (V + 255) // 256 * 256)
@@ -100,9 +103,9 @@ def _plan(T, H, V, piece_bytes, slab_bytes, train, keep_bytes=KEEP_BYTES):
     kept = 0
     if train and (T <= TWO_ROWS or 16 * T <= H):
         kept = V
-    elif train and H >= KEEP_WIDTH:
+    elif train and H >= keep_width:
         kept = min(V, keep_bytes // (4 * ldt) // 256 * 256)
-        kept = kept if kept >= min(V, KEEP_LEAST) else 0
+        kept = kept if kept >= min(V, keep_least) else 0
     return cols, splits, ldt if kept else 0, kept
 
 
@@ -150,7 +153,7 @@ class _LinearLoss(torch.autograd.Function):
         dev = hidden.device
         h, w = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
         (T, H), V, K = h.shape, w.shape[0], job.K
-        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train, KEEP_BYTES)
+        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train)
         job.shape = hidden.shape
         _, _, ldt, words = job.plan
         with _on_device(dev):

@@ -118,7 +118,7 @@ def test_logits_that_are_kept():
     assert kept(100, 1600, 500000, keep=0) == (104, 500000)                                  # an eighth of the weight's bytes
     assert kept(101, 1600, 500000, keep=0) == (0, 0) == kept(101, 1600, 500000, train=False) == kept(1, 64, 1000, train=False)
     assert kept(4096, 4096, 32001) == (4096, 32001)
-    assert kept(4090, 1024, 32001) == (0, 0)                                                 # making them again costs less
+    assert kept(4090, 512, 32001) == (0, 0) and kept(4090, 1024, 32001) == (4096, 32001)                                                 # making them again costs less
     T, V = 30001, 150000
     ldt, words = kept(T, 4096, V)
     assert ldt == 30008 and words % 256 == 0 and 4 * ldt * words <= M.KEEP_BYTES < 4 * ldt * (words + 256)
