@@ -122,3 +122,37 @@ def test_refusals_on_the_gpu():
         router_balance_loss(torch.zeros(2, 1025, device="cuda"), torch.zeros(2, 1025, dtype=torch.bool, device="cuda"), 2, 0.01)
     with pytest.raises(ValueError, match="on cpu"):
         router_balance_loss(x, rmap.cpu(), 2, 0.01)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,E,batch", [(512, 2, 1), (4096, 6, 4), (3000, 256, 3)])
+def test_balanced_loads_have_no_gradient(T, E, batch, score):
+    """Every expert takes every token: f is the same for all, and f_e - sum p f is 0 but for what the sigmoid's normaliser adds, a factor
+    of 1e-20 / sum s (at most 1e-18 here) of f = S.  The gradient is that times at most C g."""
+    from mindspeed_b200.ops.balance_loss import router_balance_loss
+    x = torch.randn(T, E, device="cuda", generator=torch.Generator(device="cuda").manual_seed(T)).requires_grad_(True)
+    loss, counts = router_balance_loss(x, torch.ones(T, E, dtype=torch.bool, device="cuda"), E, 0.01, score, batch)
+    loss.backward()
+    S = T // batch
+    assert bool((counts == T).all())
+    assert float(x.grad.abs().max()) <= 1e-18 * S * 0.01 * E / (S * S * E * batch)
+
+
+def test_scores_that_do_not_add_up_to_one():
+    """Sigmoids so small that the normaliser's 1e-20 counts, against the formula in 64 bits.  A score's relative error is at most 2^-20, and
+    the differences of the loads are exact: each of the E + 2 terms of f_e - sum p f is off by 2^-19 of the largest load."""
+    from mindspeed_b200.ops.balance_loss import router_balance_loss
+    T, E = 64, 12
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = (-46 + torch.randn(T, E, device="cuda", generator=gen)).requires_grad_(True)
+    rmap = torch.rand(T, E, device="cuda", generator=gen) < torch.linspace(0.2, 0.9, E, device="cuda")
+    loss, _ = router_balance_loss(x, rmap, 2, 0.01, "sigmoid")
+    loss.backward()
+    s = torch.sigmoid(x.detach().double())
+    n = s.sum(1, keepdim=True) + 1e-20
+    f = rmap.double().sum(0)
+    c = 0.01 * E / (T * T * 2)
+    slope = s * (1 - s) / n * c
+    want = slope * (f - (s / n * f).sum(1, keepdim=True))
+    assert ((x.grad.double() - want).abs() <= slope * f.max() * (E + 2) * 2.0 ** -19).all()
+    assert abs(float(loss) - float(c * ((s / n).sum(0) * f).sum())) <= 2.0 ** -18 * float(loss)
