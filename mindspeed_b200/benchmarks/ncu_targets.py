@@ -165,11 +165,12 @@ def mla_heads():
 def losses():
     from ..ops import gemm as G
     from ..ops.balance_loss import router_balance_loss
-    from ..ops.linear_cross_entropy import linear_cross_entropy
+    from ..ops import linear_cross_entropy as L
+    L.KEEP_BYTES = 256 << 20                  # logits of half the words of the first case: both ways of its backward run
     for rows, vocab, hidden in ((4096, 32000, 4096), (96, 65536, 4096)):
         h = torch.randn(rows, hidden, device="cuda", dtype=torch.bfloat16, requires_grad=True)
         w = (torch.randn(vocab, hidden, device="cuda") * 0.02).to(torch.bfloat16).requires_grad_(True)
-        linear_cross_entropy(h, w, torch.randint(0, vocab, (rows,), device="cuda")).mean().backward()
+        L.linear_cross_entropy(h, w, torch.randint(0, vocab, (rows,), device="cuda")).mean().backward()
     x = torch.randn(65536, 256, device="cuda", requires_grad=True)
     rmap = torch.zeros(65536, 256, dtype=torch.bool, device="cuda").scatter_(1, x.detach().topk(8, 1)[1], True)
     router_balance_loss(x, rmap, 8, 0.01)[0].backward()

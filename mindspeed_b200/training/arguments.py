@@ -56,7 +56,7 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--attention-softmax-in-fp32", action="store_true")
     g.add_argument("--use-flash-attn", action="store_true")
     g.add_argument("--linear-cross-entropy-fusion", action="store_true",
-                   help="output projection and cross entropy in one operator that keeps no logits (bf16 / fp16 on a GPU)")
+                   help="output projection and cross entropy in one operator that keeps a bounded part of the logits at most (bf16 / fp16 on a GPU)")
     g.add_argument("--mtp-num-layers", type=int, default=None)
     g.add_argument("--mtp-loss-scaling-factor", type=float, default=0.1)
 
