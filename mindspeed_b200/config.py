@@ -59,6 +59,7 @@ class ModelParallelConfig:
     tp_comm_overlap_rs: bool = True
     cross_entropy_loss_fusion: bool = False
     linear_cross_entropy_fusion: bool = False
+    linear_cross_entropy_memory_mb: int = 0
 
     pipeline_dtype: Optional[torch.dtype] = None
     variable_seq_lengths: bool = False

@@ -1,4 +1,4 @@
-// Output projection with its loss, without the [tokens, vocab] matrix of logits (bf16 / fp16, sm_100a).
+// Output projection with its loss, with a bounded part of the [tokens, vocab] matrix of logits in memory (bf16 / fp16, sm_100a).
 //
 //   z = hidden W^T,   lse_t = log sum_v exp(z_tv / tau),   loss_t = tau^2 sum_k q_tk (log q_tk - z_t,i(t,k) / tau + lse_t)
 //   dz_tv = g_t tau (exp(z_tv / tau - lse_t) - sum_{k: i(t,k) = v} q_tk),   d hidden = dz W,   dW = dz^T hidden
@@ -23,7 +23,7 @@
 //           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
 // Kept logits: the forward can keep the fp32 logits of the first words (transposed, [words, rows]: rows are the lanes of the epilogue),
 //           and an elementwise pass makes dz of them instead of the GEMM.  Few rows (at most 64, or the logits take at most an eighth of
-//           the weight's bytes) keep all: one reading of W less, a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 ->
+//           the weight's bytes, but for rows rounded up to 8) keep all: one reading of W less, a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 ->
 //           755 us).  More rows keep what the caller's limit holds, where H is wide enough (KEEP_BYTES and KEEP_WIDTH in
 //           ops/linear_cross_entropy.py, with the figures of both sides).
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.

@@ -2,7 +2,7 @@
 
 forward(input_ids, position_ids, attention_mask, labels) -> per-token loss [b, s] when labels are
 given on the last pipeline stage, else logits [b, s, V/tp] or hidden states for the next stage.  With --linear-cross-entropy-fusion the
-loss comes straight from the hidden states (ops/linear_cross_entropy.py) and no logits are kept.
+loss comes straight from the hidden states (ops/linear_cross_entropy.py) in no more memory than the logits would take.
 """
 from __future__ import annotations
 
@@ -157,8 +157,8 @@ class GPTModel(nn.Module):
         return loss.transpose(0, 1).contiguous()  # [b, s]
 
     def _linear_loss_operands(self, hidden, weight):
-        """(hidden states [s, b, h] of all tokens, weight, vocabulary group, accumulate into main_grad) for the operators that make the loss
-        without the logits, or None where somebody watches or has replaced what they pass by, or the kernels take other types."""
+        """(hidden states [s, b, h] of all tokens, weight, keyword arguments) for the operators that make the loss without the logits, or None
+        where somebody watches or has replaced what they pass by, or the kernels take other types."""
         out = self.output_layer
         weight = out.weight if weight is None else weight
         if (observed(out, ColumnParallelLinear) or out.bias is not None or type(self).compute_language_model_loss is not _OWN_LOSS
@@ -173,7 +173,9 @@ class GPTModel(nn.Module):
         mg = getattr(weight, "main_grad", None)
         into = (out.gradient_accumulation_fusion and mg is not None and mg.dtype == torch.float32 and mg.is_contiguous()
                 and mg.shape == weight.shape and mg.data_ptr() % 16 == 0)
-        return hidden, weight, out.tp_group if out.world > 1 else None, into
+        mb = self.config.linear_cross_entropy_memory_mb
+        limit = mb << 20 if mb else hidden.numel() // hidden.shape[-1] * weight.shape[0] * hidden.element_size()      # the logits' own bytes
+        return hidden, weight, dict(group=out.tp_group if out.world > 1 else None, accumulate_main_grad=into, memory_limit=limit)
 
     def linear_language_model_loss(self, hidden, labels, weight=None):
         """Per-token loss [b, s] by the fused output projection and cross entropy (--linear-cross-entropy-fusion), or None."""
@@ -181,8 +183,8 @@ class GPTModel(nn.Module):
         if ops is None:
             return None
         from ..ops.linear_cross_entropy import linear_cross_entropy
-        h, w, group, into = ops
-        return linear_cross_entropy(h, w, labels.transpose(0, 1), group=group, accumulate_main_grad=into).transpose(0, 1).contiguous()
+        h, w, how = ops
+        return linear_cross_entropy(h, w, labels.transpose(0, 1), **how).transpose(0, 1).contiguous()
 
     def distillation_loss(self, hidden, labels, targets, temperature, weight=None):
         """[2, b, s]: the divergence from a teacher's top words, ``targets`` = (logits, indices) [b, s, K], and next to it the cross entropy
@@ -191,11 +193,11 @@ class GPTModel(nn.Module):
         if ops is None:
             raise RuntimeError("the distillation loss from top words takes a bf16 or fp16 model whose output layer and loss are not replaced")
         from ..ops.linear_cross_entropy import linear_cross_entropy, linear_topk_distillation
-        h, w, group, into = ops
+        h, w, how = ops
         logits, indices = (t.transpose(0, 1) for t in targets)
-        kl = linear_topk_distillation(h, w, logits, indices, temperature, group=group, accumulate_main_grad=into)
+        kl = linear_topk_distillation(h, w, logits, indices, temperature, **how)
         with torch.no_grad():
-            ce = linear_cross_entropy(h, w, labels.transpose(0, 1), group=group)
+            ce = linear_cross_entropy(h, w, labels.transpose(0, 1), group=how["group"])
         return torch.stack((kl, ce)).transpose(1, 2).contiguous()
 
     def sharded_state_dict(self, prefix="", sharded_offsets=(), metadata=None):

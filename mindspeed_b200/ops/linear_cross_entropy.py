@@ -1,15 +1,21 @@
-"""Output projection and its loss in one operator, without the [tokens, vocab] matrix of logits
+"""Output projection and its loss in one operator, which holds a bounded part of the [tokens, vocab] matrix of logits at most
 (csrc/kernels/linear_ce_sm100.cu).
 
   linear_cross_entropy(hidden, weight, labels)                                  per-token cross entropy of softmax(hidden weight^T)
   linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices)     per-token tau^2 KL(teacher's top words || student)
 
 Both take ``hidden`` [..., H] and ``weight`` [V, H] in bf16 or fp16 (H a multiple of 8) and return the loss in fp32 with the leading shape
-of ``hidden``; any gradient may come back on it.  The forward keeps a maximum and a sum per token and, in training, at most ``KEEP_BYTES``
-(2 GiB) of fp32 logits, as far as they go over the vocabulary; the backward makes the others again.  Both directions work on a piece of the
-vocabulary at a time.  (For few tokens, at most 64 or a sixteenth of H, all logits are kept: at most an eighth of the weight's bytes, or
-256 bytes a word.)  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative, or all
-teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
+of ``hidden``; any gradient may come back on it.  Tokens without a label (``ignore_index``) or without a teacher word (all indices negative,
+or all teacher logits -inf) have loss 0 and no gradient, whatever their hidden states hold, and cost nothing in the products.
+
+Memory.  From the forward to the backward a call keeps a copy of the hidden states (packed where tokens left), the listed logits and
+weights (8 bytes a listed word), and, in training, at most ``KEEP_BYTES`` (2 GiB) of fp32 logits, as far as they go over the vocabulary;
+the backward makes the others again.  The backward works on a piece of the vocabulary at a time: 16-bit gradients of its logits
+(``PIECE_BYTES``, 512 MiB) and fp32 parts of the hidden gradient (``SLAB_BYTES``, 256 MiB, or one part where that is more).  That can be
+more than the 16-bit logits of all tokens (4096 x 129280: 2.8 GB next to 1.1): ``memory_limit`` bounds all of it, in bytes, and what
+does not fit is made again.  The least that a call can do with is the copy, one part of the hidden gradient and a piece of 256 words; the
+forward's statistics (9 bytes a token and 128 words) come and go before the pieces and are not counted.  Calls of few tokens, at most 64 or
+a sixteenth of H, are not limited and keep all logits: an eighth of the weight's bytes (for rows rounded up to 8), or 256 bytes a word.
 
 A label or teacher index beyond the vocabulary gives its token loss NaN and no gradient, and makes ``ops.gemm.check_status`` raise.
 
@@ -40,7 +46,7 @@ _P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_flo
 #: bytes of the 16-bit logit gradients that the backward holds at a time, and of the fp32 partial results of the hidden gradient
 PIECE_BYTES = 512 << 20
 SLAB_BYTES = 256 << 20
-#: bytes of fp32 logits that a call keeps from its forward to its backward, which then makes those of the remaining words again.  0 keeps
+#: most bytes of fp32 logits that a call keeps from its forward to its backward, which then makes those of the remaining words again.  0 keeps
 #: none (but for few tokens).  A kept logit costs what its bytes take, making it again 2 H / 1.3 PFLOP/s: at least KEEP_WIDTH hidden columns
 #: (both directions, us, made again -> kept: 1024 x 128256 x 512 579 -> 606, 766 x 50257 x 768 333 -> 316, 2048 x 32000 x 1024 515 -> 485,
 #: 2048 x 50000 x 1536 1065 -> 945, 4096 x 129280 x 4096 13000 -> 10700), and at least KEEP_LEAST words, which fill the products' tiles.
@@ -91,6 +97,24 @@ def _plan(T, H, V, piece_bytes, slab_bytes, train, keep_bytes=None):
     return _planned(T, H, V, piece_bytes, slab_bytes, train, KEEP_BYTES if keep_bytes is None else keep_bytes, KEEP_WIDTH, KEEP_LEAST)
 
 
+def _budget(T, H, V, K, limit):
+    """(bytes of a piece, of the hidden gradient's parts, of kept logits) for a call that may hold ``limit`` bytes: an eighth for the parts, a
+    quarter for the piece and what is left for logits; the piece gets all of that where none are kept.  Few tokens are not limited: their
+    logits are small next to the weight, and pieces of some hundred words would cost many launches."""
+    if limit is None or T <= TWO_ROWS or 16 * T <= H:
+        return PIECE_BYTES, SLAB_BYTES, KEEP_BYTES
+    ldt = (T + 7) // 8 * 8
+    least = 512 * ldt                                     # a piece of 256 words
+    rest = max(0, limit - (2 * T * H + 8 * T * K + 12 * T + 16))
+    slab = min(SLAB_BYTES, limit // 8, max(0, rest - least))
+    rest = max(0, rest - max(slab, (T + 31) // 32 * 32 * H * 4))
+    piece = min(PIECE_BYTES, limit // 4)
+    keep = min(KEEP_BYTES, rest - max(piece, least))
+    if keep <= 0 or not _plan(T, H, V, piece, slab, True, keep)[3]:
+        piece, keep = min(PIECE_BYTES, rest), 0
+    return piece * T // ldt, slab, keep
+
+
 @functools.lru_cache(maxsize=64)
 def _planned(T, H, V, piece_bytes, slab_bytes, train, keep_bytes, keep_width, keep_least):
     """The device chooses among the splits for the rows that stay (choose_splits in the kernel file); more of them than fill the 74 SM pairs
@@ -122,10 +146,11 @@ def _lib():
 class _Job:
     """One call: its targets and what stays the same in both directions.  (Autograd passes it along as one argument; every argument of a
     function costs host time, and short calls are bound by that.)"""
-    __slots__ = ("idx", "teacher", "K", "tau", "ignore_index", "group", "world", "rank", "main_grad", "train", "plan", "shape")
+    __slots__ = ("idx", "teacher", "K", "tau", "ignore_index", "group", "world", "rank", "main_grad", "limit", "train", "plan", "shape")
 
-    def __init__(self, hidden, weight, idx, teacher, K, tau, ignore_index, group, main_grad):
+    def __init__(self, hidden, weight, idx, teacher, K, tau, ignore_index, group, main_grad, limit):
         self.idx, self.teacher, self.K, self.tau, self.ignore_index, self.group = idx, teacher, K, tau, ignore_index, group
+        self.limit = limit
         self.world, self.rank = (1, 0) if group is None else (dist.get_world_size(group), dist.get_rank(group))
         self.main_grad = weight if main_grad else None
         self.train = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
@@ -153,7 +178,8 @@ class _LinearLoss(torch.autograd.Function):
         dev = hidden.device
         h, w = _rows(hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])), _rows(weight)
         (T, H), V, K = h.shape, w.shape[0], job.K
-        job.plan = _plan(T, H, V, PIECE_BYTES, SLAB_BYTES, job.train)
+        piece_bytes, slab_bytes, keep_bytes = _budget(T, H, V, K, job.limit)
+        job.plan = _plan(T, H, V, piece_bytes, slab_bytes, job.train, keep_bytes)
         job.shape = hidden.shape
         _, _, ldt, words = job.plan
         with _on_device(dev):
@@ -275,7 +301,7 @@ def _linear_loss_ref(hidden, weight, idx, q, ent, tau, group):
     return out.reshape(hidden.shape[:-1])
 
 
-def _check(name, hidden, weight, target, accumulate_main_grad):
+def _check(name, hidden, weight, target, accumulate_main_grad, memory_limit):
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"{name}: hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not fit")
     if weight.shape[0] == 0 or weight.shape[1] == 0:
@@ -286,6 +312,8 @@ def _check(name, hidden, weight, target, accumulate_main_grad):
         raise TypeError(f"{name}: labels and indices are integers, not {target.dtype}")
     if not (hidden.device == weight.device == target.device):
         raise ValueError(f"{name}: hidden on {hidden.device}, weight on {weight.device}, targets on {target.device}")
+    if memory_limit is not None and not memory_limit >= 0:
+        raise ValueError(f"{name}: memory_limit is a number of bytes or None, not {memory_limit}")
     if accumulate_main_grad:
         mg = getattr(weight, "main_grad", None)
         if mg is None or mg.dtype != torch.float32 or mg.shape != weight.shape or not mg.is_contiguous() or mg.device != weight.device:
@@ -321,16 +349,17 @@ def _main_grad_hook(weight):
     return w
 
 
-def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, accumulate_main_grad=False):
+def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, accumulate_main_grad=False, memory_limit=None):
     """Cross entropy of ``softmax(hidden @ weight.T)`` against ``labels`` [...], per token, fp32."""
-    _check("linear_cross_entropy", hidden, weight, labels, accumulate_main_grad)
+    _check("linear_cross_entropy", hidden, weight, labels, accumulate_main_grad, memory_limit)
     if labels.shape != hidden.shape[:-1]:
         raise ValueError(f"linear_cross_entropy: labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
     if labels.numel() == 0:
         return _none(hidden, weight)
     idx = labels if labels.dtype == torch.int64 and labels.is_contiguous() else labels.long().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, None, 1, 1.0, int(ignore_index), group, accumulate_main_grad))
+        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, None, 1, 1.0, int(ignore_index), group, accumulate_main_grad,
+                                                       None if memory_limit is None else int(memory_limit)))
     idx = idx.reshape(-1)
     world = 1 if group is None else dist.get_world_size(group)
     kept = idx != ignore_index
@@ -341,12 +370,13 @@ def linear_cross_entropy(hidden, weight, labels, ignore_index=-100, group=None, 
     return _linear_loss_ref(hidden, w, idx.unsqueeze(1), q, torch.zeros_like(q[:, 0]), 1.0, group)
 
 
-def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, temperature=1.0, group=None, accumulate_main_grad=False):
+def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, temperature=1.0, group=None, accumulate_main_grad=False,
+                             memory_limit=None):
     """``temperature^2 KL(q || p)`` per token, fp32: q is the softmax of ``teacher_logits`` [..., K] at the temperature over the listed words
     ``teacher_indices`` [..., K] (negative: unused place; a word may be listed more than once), p the student's softmax over the whole
     vocabulary.  The teacher gets no gradient."""
     name = "linear_topk_distillation"
-    _check(name, hidden, weight, teacher_indices, accumulate_main_grad)
+    _check(name, hidden, weight, teacher_indices, accumulate_main_grad, memory_limit)
     K = teacher_indices.shape[-1] if teacher_indices.dim() else 0
     if teacher_logits.shape != teacher_indices.shape or teacher_indices.shape[:-1] != hidden.shape[:-1]:
         raise ValueError(f"{name}: teacher logits {tuple(teacher_logits.shape)} and indices {tuple(teacher_indices.shape)} "
@@ -363,7 +393,8 @@ def linear_topk_distillation(hidden, weight, teacher_logits, teacher_indices, te
     idx = teacher_indices.reshape(-1, K).long().contiguous()
     a = teacher_logits.detach().reshape(-1, K).float().contiguous()
     if loader.use_kernels(hidden):
-        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, a, K, tau, 0, group, accumulate_main_grad))
+        return _LinearLoss.apply(hidden, weight, _Job(hidden, weight, idx, a, K, tau, 0, group, accumulate_main_grad,
+                                                       None if memory_limit is None else int(memory_limit)))
     world = 1 if group is None else dist.get_world_size(group)
     if bool((idx >= world * weight.shape[0]).any()):
         raise IndexError(f"{name}: a teacher index outside the vocabulary")

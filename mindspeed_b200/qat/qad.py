@@ -6,7 +6,8 @@ linears run on fake-quantised weights).  Every micro-batch the teacher's logits 
 tokens, and the student is trained on the KL divergence from the teacher's distribution alone: temperature
 ``--kl-temperature`` (loss scaled by T^2), weight ``--kl-loss-weight``, ``--kl-loss-reduction`` mean (over unmasked
 tokens) or sum.  With ``--kl-teacher-topk`` K the teacher's K largest logits of each token, normalised among themselves, stand
-for its distribution; the student's logits are then not kept either (ops/linear_cross_entropy.py).  The cross entropy against the labels is computed without a graph and reported next to it.  With
+for its distribution; the student's logits are then not held either, but for a bounded part (ops/linear_cross_entropy.py,
+``--linear-cross-entropy-memory-mb``).  The cross entropy against the labels is computed without a graph and reported next to it.  With
 vocabulary-parallel logits the softmax normalisers are reduced over the tensor-parallel group, so the loss equals the
 single-rank one.  Dense models without pipeline parallelism only: the loss needs both models' logits for the same
 micro-batch on one rank.

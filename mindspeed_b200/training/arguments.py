@@ -57,6 +57,9 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--use-flash-attn", action="store_true")
     g.add_argument("--linear-cross-entropy-fusion", action="store_true",
                    help="output projection and cross entropy in one operator that keeps a bounded part of the logits at most (bf16 / fp16 on a GPU)")
+    g.add_argument("--linear-cross-entropy-memory-mb", type=int, default=0,
+                   help="MiB that each call of --linear-cross-entropy-fusion or --kl-teacher-topk may hold for logits and their gradients; more of "
+                        "it saves products, up to 2.8 GiB (0: as much as the 16-bit logits would take)")
     g.add_argument("--mtp-num-layers", type=int, default=None)
     g.add_argument("--mtp-loss-scaling-factor", type=float, default=0.1)
 
@@ -341,6 +344,8 @@ def _core_validate(args):
         args.use_distributed_optimizer = True                        # optimizer state (and reduce-scattered gradients) sharded
     if args.manual_gc and args.manual_gc_interval < 0:
         raise AssertionError("--manual-gc-interval must not be negative")
+    if getattr(args, "linear_cross_entropy_memory_mb", 0) < 0:
+        raise AssertionError("--linear-cross-entropy-memory-mb must not be negative")
     args.params_dtype = torch.bfloat16 if args.bf16 else torch.float16 if args.fp16 else torch.float32
     if args.bf16:
         args.accumulate_allreduce_grads_in_fp32 = True
