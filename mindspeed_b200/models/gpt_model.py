@@ -177,14 +177,21 @@ class GPTModel(nn.Module):
         limit = mb << 20 if mb else hidden.numel() // hidden.shape[-1] * weight.shape[0] * hidden.element_size()      # the logits' own bytes
         return hidden, weight, dict(group=out.tp_group if out.world > 1 else None, accumulate_main_grad=into, memory_limit=limit)
 
+    def _words_or_ignored(self, labels, weight):
+        """Labels [s, b] of [b, s], those that are no word as -100: a loss mask outside takes such tokens out, and it could not take out the
+        NaN that the operators answer them with."""
+        labels = labels.transpose(0, 1).long()
+        return labels.masked_fill((labels < 0) | (labels >= weight.shape[0] * self.output_layer.world), -100)
+
     def linear_language_model_loss(self, hidden, labels, weight=None):
-        """Per-token loss [b, s] by the fused output projection and cross entropy (--linear-cross-entropy-fusion), or None."""
+        """Per-token loss [b, s] by the fused output projection and cross entropy (--linear-cross-entropy-fusion), or None.  Labels that are
+        no word of the vocabulary, whatever padding they are, have loss 0."""
         ops = self._linear_loss_operands(hidden, weight) if self.config.linear_cross_entropy_fusion else None
         if ops is None:
             return None
         from ..ops.linear_cross_entropy import linear_cross_entropy
         h, w, how = ops
-        return linear_cross_entropy(h, w, labels.transpose(0, 1), **how).transpose(0, 1).contiguous()
+        return linear_cross_entropy(h, w, self._words_or_ignored(labels, w), **how).transpose(0, 1).contiguous()
 
     def distillation_loss(self, hidden, labels, targets, temperature, weight=None):
         """[2, b, s]: the divergence from a teacher's top words, ``targets`` = (logits, indices) [b, s, K], and next to it the cross entropy
@@ -197,7 +204,7 @@ class GPTModel(nn.Module):
         logits, indices = (t.transpose(0, 1) for t in targets)
         kl = linear_topk_distillation(h, w, logits, indices, temperature, **how)
         with torch.no_grad():
-            ce = linear_cross_entropy(h, w, labels.transpose(0, 1), group=how["group"])
+            ce = linear_cross_entropy(h, w, self._words_or_ignored(labels, w), group=how["group"])
         return torch.stack((kl, ce)).transpose(1, 2).contiguous()
 
     def sharded_state_dict(self, prefix="", sharded_offsets=(), metadata=None):

@@ -56,7 +56,8 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--attention-softmax-in-fp32", action="store_true")
     g.add_argument("--use-flash-attn", action="store_true")
     g.add_argument("--linear-cross-entropy-fusion", action="store_true",
-                   help="output projection and cross entropy in one operator that keeps a bounded part of the logits at most (bf16 / fp16 on a GPU)")
+                   help="output projection and cross entropy in one operator that keeps a bounded part of the logits at most (bf16 / fp16 on a GPU); "
+                        "tokens whose label is no word of the vocabulary have loss 0")
     g.add_argument("--linear-cross-entropy-memory-mb", type=int, default=0,
                    help="MiB that each call of --linear-cross-entropy-fusion or --kl-teacher-topk may hold for logits and their gradients; more of "
                         "it saves products, up to 2.8 GiB (0: as much as the 16-bit logits would take)")
