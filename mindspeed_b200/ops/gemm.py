@@ -33,14 +33,18 @@ def status_word(device) -> torch.Tensor:
 
 
 def check_status(device=None):
-    """Synchronising check; raises if any kernel recorded a time-out, or one of ``_MEANING``, since the last check."""
+    """Synchronising check; raises if any kernel recorded a time-out, or one of ``_MEANING``, since the last check.  Names every word that
+    is set, on all devices that are asked, and clears them."""
+    found = []
     for dev, t in _status.items():
         if device is not None and dev != device:
             continue
-        v = next((w for w in t[:2].tolist() if w != 0), 0)
-        if v != 0:
+        words = [v for v in t[:2].tolist() if v != 0]
+        if words:
             t.zero_()
-            raise RuntimeError(f"sm_100a kernel reported {_MEANING.get(v, 'a bounded-wait time-out')}, code 0x{v:x} on {dev}")
+            found += [f"{_MEANING.get(v, 'a bounded-wait time-out')}, code 0x{v:x} on {dev}" for v in words]
+    if found:
+        raise RuntimeError("sm_100a kernel reported " + "; ".join(found))
 
 
 class cta_limit:

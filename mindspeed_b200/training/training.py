@@ -408,8 +408,10 @@ def _moe_routers(model):
 def check_kernel_status():
     """Raise if a device-side bounded wait expired since the last check (GEMM mbarriers, all-gather / reduce-scatter
     flags, MoE, Ulysses, fused optimizer step): such a kernel returns early with its outputs not computed, so the step
-    that contained it is invalid.  The RuntimeError names the wait's code and reaches the TTP exception handler.
-    Call after the step's synchronize; costs one 4-byte read per device that has launched such kernels."""
+    that contained it is invalid.  Raise too for wrong input that a kernel met: a routing map with another number of entries
+    than stated, or a label or teacher index outside the vocabulary (whose token alone has no result).  The RuntimeError
+    names every code and reaches the TTP exception handler.  Call after the step's synchronize; costs one 8-byte read per
+    device that has launched such kernels."""
     from ..ops import gemm as G
     G.check_status()
 
