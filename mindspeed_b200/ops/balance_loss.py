@@ -113,7 +113,8 @@ def router_balance_loss(logits, routing_map, topk, coeff, score_function="softma
     if loader.use_kernels(logits):
         if logits.dtype not in CODE:
             raise TypeError(f"router_balance_loss: the sm_100a kernels take fp32, bf16 or fp16, not {logits.dtype}")
-        if E > MAX_EXPERTS or T > 1 << 24:
-            raise ValueError(f"router_balance_loss: {E} experts (at most {MAX_EXPERTS}), {T} tokens (at most 2^24)")
+        if E > MAX_EXPERTS or T > 1 << 24 or batch_size > 65535:
+            raise ValueError(f"router_balance_loss: {E} experts (at most {MAX_EXPERTS}), {T} tokens (at most 2^24), {batch_size} sequences (at "
+                             f"most 65535)")
         return _BalanceLoss.apply(logits, (routing_map, scale, int(sigmoid), int(batch_size)))
     return _balance_ref(logits, routing_map, scale, sigmoid, int(batch_size))

@@ -60,10 +60,11 @@ class TopKRouter(nn.Module):
     def _wants_aux(self):
         return self.config.moe_aux_loss_coeff > 0 and self.training and self.routing_type not in ("none", "sinkhorn")
 
-    def _fused_aux(self, logits):
-        """True where ops/balance_loss.py makes the balance loss and the counts (--moe-balance-loss-fusion)."""
-        return bool(self.config.moe_balance_loss_fusion and self._wants_aux() and (not logits.is_cuda or logits.dtype != torch.float64)
-                    and self.num_experts <= 1024)
+    def _fused_aux(self, logits, seq_shape):
+        """True where ops/balance_loss.py makes the balance loss and the counts (--moe-balance-loss-fusion): not for what its kernels refuse."""
+        if not self.config.moe_balance_loss_fusion or not self._wants_aux() or self.num_experts > 1024:
+            return False
+        return not logits.is_cuda or (logits.dtype != torch.float64 and logits.shape[0] <= 1 << 24 and seq_shape[1] <= 65535)
 
     def _aux(self, probs_for_loss, routing_map, tokens_per_expert, activation, seq_shape, aux_of=None):
         """Attaches the balance loss to ``activation``; ``aux_of(coeff, sequences)`` gives it where it is made by one operator."""
@@ -100,7 +101,7 @@ class TopKRouter(nn.Module):
             logits, self.topk, cfg.moe_expert_capacity_factor, cfg.moe_pad_expert_input_to_capacity, cfg.moe_token_drop_policy,
             cfg.moe_router_pre_softmax, cfg.moe_router_num_groups, cfg.moe_router_group_topk,
             cfg.moe_router_topk_scaling_factor, self.score_function, self.expert_bias)
-        if self._fused_aux(logits):
+        if self._fused_aux(logits, seq_shape):
             from ...ops.balance_loss import router_balance_loss
             counts = []
 
