@@ -85,7 +85,9 @@ def test_the_flag_does_not_raise_the_peak(one_rank, seq, heads):  # noqa: F811
         loss, peak = _peak(step)
         peaks.append(peak)
         losses.append(float(loss))
+        # RMSNorm makes hidden states of norm sqrt(1024): no logit is larger than this
+        z = 32 * float(m.output_layer.weight.detach().float().norm(dim=1).max())
         del m
     assert peaks[1] <= peaks[0], [p / MIB for p in peaks]
-    # bf16 logits move a loss by at most twice 2^-8 of the largest, here below 8
-    assert abs(losses[0] - losses[1]) <= 2 * 2.0 ** -8 * 8
+    # the layers are the same; bf16 logits move each loss by at most twice 2^-8 of the largest, the heads' as much times their factor of 0.1
+    assert abs(losses[0] - losses[1]) <= 1.1 * 2 * 2.0 ** -8 * z
