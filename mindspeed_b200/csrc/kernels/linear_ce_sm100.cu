@@ -15,7 +15,9 @@
 //           W are 2.1 GB, 0.3 ms as a kernel of its own and as much beside the GEMM.)
 //           The tensor cores cut every addition to their fp32 sums off: a logit comes out 0.26 (H / 16) 2^-24 of itself too small (0.258
 //           to 0.273 measured at H 1024 to 5120; half a unit in the last place for each of the H / 16 additions, of a sum that grows).
-//           The scale 1 / tau of such logits makes that good, and the join computes the largest logit of a row again as a dot product.
+//           The scale 1 / tau of such logits takes that up on average: it was fitted to sums that grow steadily on this chip, and a logit
+//           whose partial sums exceed it is corrected by too little (of the order of the error itself, 4e-6 at H 4096, which is what the
+//           bounds allow without it).  The join computes the largest logit of a row again as a dot product.
 // Backward: per piece of the vocabulary: the GEMM again, its epilogue now writing the 16-bit dz of the piece (with the label's -1; a
 //           list's q are subtracted by a kernel of its own) -> d hidden += dz W -> dW rows of the piece = dz^T hidden.  dz is rounded to
 //           the 16-bit type of the operands (the tensor cores take nothing wider next to them): half a step on each term, as much as the
@@ -23,9 +25,10 @@
 //           probabilities down to 2^-28 keep all their bits; the products' epilogues take the power out again in fp32.
 // Kept logits: the forward can keep the fp32 logits of the first words (transposed, [words, rows]: rows are the lanes of the epilogue),
 //           and an elementwise pass makes dz of them instead of the GEMM.  Few rows (at most 64, or the logits take at most an eighth of
-//           the weight's bytes, but for rows rounded up to 8) keep all: one reading of W less, a quarter of all traffic (96 x 128256 x 4096, both directions: 1043 ->
-//           755 us).  More rows keep what the caller's limit holds, where H is wide enough (KEEP_BYTES and KEEP_WIDTH in
-//           ops/linear_cross_entropy.py, with the figures of both sides).
+//           the weight's bytes, but for rows rounded up to 8) keep all: one reading of W less, a quarter of all
+//           traffic (96 x 128256 x 4096, both directions, with the kernels of that step: 1043 -> 755 us; 714 now).  More rows keep what the
+//           caller's limit holds, where H is wide enough (KEEP_BYTES and KEEP_WIDTH in ops/linear_cross_entropy.py, with the figures of
+//           both sides).
 //           Up to 64 rows dz goes in two 16-bit terms, as 128 rows: the products take no longer, and so few roundings do not average out.
 //
 // The products are the CTA-pair pipeline of gemm2_sm100.cu (same roles, barriers and bounded waits) with other work lists and epilogues.

@@ -98,7 +98,8 @@ def _core_args(p: argparse.ArgumentParser):
     g.add_argument("--moe-layer-recompute", action="store_true")
     g.add_argument("--moe-permute-fusion", action="store_true")
     g.add_argument("--moe-balance-loss-fusion", action="store_true",
-                   help="scores, counts, balance loss and its gradient in one pass over the router logits each way")
+                   help="balance loss of the router with its scores, per-expert counts and gradient in one operator, a pass over the "
+                        "logits each way (the routing itself still counts its map)")
     g.add_argument("--moe-per-layer-logging", action="store_true")
     g.add_argument("--first-k-dense-replace", type=int, default=0)
 
